@@ -18,7 +18,7 @@ if not os.path.exists(LIB_PATH):
 
 lib = C.CDLL(LIB_PATH)
 
-P, I64, I32, F32 = C.c_void_p, C.c_int64, C.c_int, C.c_float
+P, I64, I32, F32, F64 = C.c_void_p, C.c_int64, C.c_int, C.c_float, C.c_double
 
 
 class GSeg(C.Structure):
@@ -81,6 +81,12 @@ _SIGS = {
     "dd3d_avg_pool_bwd": (I32, [P, P, P, I64, I64, I32, P, P]),
     "dd3d_global_avg_pool_fwd": (I32, [P, I64, P, I32, I32, P, P]),
     "dd3d_global_avg_pool_bwd": (I32, [P, I64, P, I32, I32, P, P]),
+    "dd3d_group_norm_ws_bytes": (I64, [I64, I32, I32, I32, I32]),
+    "dd3d_group_norm_fwd": (I32, [P, I32, I64, I32, P, I32, I32, P, P, I32, F32, I32, F32, F64, P, P, P, P, P, I64, P]),
+    "dd3d_group_norm_bwd": (I32, [P, P, I32, I64, I32, P, I32, I32, P, P, I32, I32, F32, F64, P, P, P, P, P, P, P, I64, P]),
+    "dd3d_group_norm_bwd2": (I32, [P, P, P, P, P, I32, I64, I32, P, I32, I32, P, P, I32, I32, F32, F64, P, P, P, P, P, P, P, P, I64, P]),
+    "dd3d_dropout": (I32, [P, I32, I64, I64, F64, P, P, P]),
+    "dd3d_random_key": (I32, [P, P, P]),
     "dd3d_arp_bwd_ws_bytes": (I64, [I64, I32]),
     "dd3d_affine_relu_pool_bwd": (I32, [P, P, P, P, P, P, I32, I32, I64, P, I32, P, P, P, P, P, P, P, I64, P]),
     "dd3d_arp_inorm_bwd_ws_bytes": (I64, [I32]),

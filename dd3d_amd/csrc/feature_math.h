@@ -1,0 +1,151 @@
+// Element types, activations with two derivatives, and the counter-based random words shared by the group-norm and dropout kernels.
+#pragma once
+#include "common.h"
+#include <hip/hip_bf16.h>
+#include <hip/hip_fp16.h>
+
+// dtype / activation codes of include/dd3d.h
+#define DD3D_F32 0
+#define DD3D_F16 1
+#define DD3D_BF16 2
+#define DD3D_ACT_NONE 0
+#define DD3D_ACT_RELU 1
+#define DD3D_ACT_LEAKY 2
+#define DD3D_ACT_SILU 3
+#define DD3D_ACT_GELU 4
+
+// ---- element types: every value is widened to fp32 on the way in and rounded to nearest even once on the way out ----------------
+typedef _Float16 half_t;
+struct bf16_t {
+    uint16_t bits;
+};
+
+__device__ __forceinline__ float widen(float v) { return v; }
+__device__ __forceinline__ float widen(half_t v) { return (float)v; }
+__device__ __forceinline__ float widen(bf16_t v) { return __uint_as_float((uint32_t)v.bits << 16); }
+template <typename T>
+__device__ __forceinline__ T narrow(float v);
+template <>
+__device__ __forceinline__ float narrow<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ half_t narrow<half_t>(float v) { return (half_t)v; }
+template <>
+__device__ __forceinline__ bf16_t narrow<bf16_t>(float v) {
+    __bf16 h = (__bf16)v;  // gfx950 rounds to nearest even in hardware
+    bf16_t r;
+    __builtin_memcpy(&r.bits, &h, 2);
+    return r;
+}
+
+// parameter vectors (weight, bias and their gradients) are fp32 or of the rows' type: a code, uniform over the launch
+__device__ __forceinline__ float load_param(const void* p, int pdt, int64_t i) {
+    if (pdt == DD3D_F32) return ((const float*)p)[i];
+    if (pdt == DD3D_F16) return widen(((const half_t*)p)[i]);
+    return widen(((const bf16_t*)p)[i]);
+}
+__device__ __forceinline__ void store_param(void* p, int pdt, int64_t i, float v) {
+    if (pdt == DD3D_F32) ((float*)p)[i] = v;
+    else if (pdt == DD3D_F16) ((half_t*)p)[i] = narrow<half_t>(v);
+    else ((bf16_t*)p)[i] = narrow<bf16_t>(v);
+}
+
+// ---- activations --------------------------------------------------------------------------------------------------------------
+// Three families: piecewise linear (none / ReLU / leaky ReLU: slope 1, 0, s below zero, the border belonging to the lower side),
+// SiLU u sigma(u), and GELU u Phi(u) with the normal distribution's Phi.
+#define DD3D_FAM_LINEAR 0
+#define DD3D_FAM_SILU 1
+#define DD3D_FAM_GELU 2
+
+__host__ __device__ __forceinline__ int act_family(int act) { return act <= DD3D_ACT_LEAKY ? DD3D_FAM_LINEAR : act == DD3D_ACT_SILU ? DD3D_FAM_SILU : DD3D_FAM_GELU; }
+
+// Phi(u) and the density n(u).  The upper tail is n-shaped: Q(a) = exp(-a^2 / 2) t P(t) for a = |u|, t = 1 / (1 + 0.35 a), P a degree-8
+// polynomial fitted for least relative error over a in [0, 14] (3.2e-8), so the far tail keeps its relative accuracy and no
+// cancellation occurs on either side; one exponential serves Phi and n alike.
+__device__ __forceinline__ void normal_cdf_pdf(float u, float* cdf, float* pdf) {
+    const float a = fabsf(u), t = __builtin_amdgcn_rcpf(fmaf(0.35f, a, 1.f));
+    const float e = __builtin_amdgcn_exp2f(u * u * -0.72134752f);
+    float p = -0.029146108776330948f;
+    p = fmaf(p, t, 0.14397257566452026f);
+    p = fmaf(p, t, -0.25571608543395996f);
+    p = fmaf(p, t, 0.15917624533176422f);
+    p = fmaf(p, t, -0.02311127260327339f);
+    p = fmaf(p, t, 0.10550861060619354f);
+    p = fmaf(p, t, 0.11983271688222885f);
+    p = fmaf(p, t, 0.13986189663410187f);
+    p = fmaf(p, t, 0.13962140679359436f);
+    const float q = e * (p * t);
+    *cdf = u < 0.f ? q : 1.f - q;
+    *pdf = e * 0.39894228f;
+}
+
+// phi(u); with ORDER >= 1 also phi'(u) in *d1, with ORDER == 2 phi''(u) in *d2
+template <int FAM, int ORDER>
+__device__ __forceinline__ float activate(float u, float slope, float* d1, float* d2) {
+    if (FAM == DD3D_FAM_LINEAR) {
+        const bool up = u > 0.f;
+        if (ORDER >= 1) *d1 = up ? 1.f : slope;
+        if (ORDER == 2) *d2 = 0.f;
+        const float low = (slope == 0.f && u == u) ? 0.f : slope * u;  // ReLU of -inf is 0, of NaN is NaN
+        return up ? u : low;
+    }
+    if (FAM == DD3D_FAM_SILU) {
+        const float s = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(u * -1.44269504f));
+        const float ds = s * (1.f - s);
+        if (ORDER >= 1) *d1 = fmaf(u, ds, s);
+        if (ORDER == 2) *d2 = ds * fmaf(u, 1.f - 2.f * s, 2.f);
+        return u * s;
+    }
+    float cdf, pdf;
+    normal_cdf_pdf(u, &cdf, &pdf);
+    if (ORDER >= 1) *d1 = fmaf(u, pdf, cdf);
+    if (ORDER == 2) *d2 = pdf * fmaf(-u, u, 2.f);
+    return u * cdf;
+}
+
+// ---- random words ---------------------------------------------------------------------------------------------------------------
+// Philox4x32-10 (Salmon, Moraes, Dror, Shaw: "Parallel random numbers: as easy as 1, 2, 3", 2011).  The word of element (row, c) is word
+// c % 4 of the block at counter (row * ceil(C / 4) + c / 4, call) under key = seed, so it depends on neither launch shape nor type, and
+// whoever needs the mask again computes it again.
+struct Drop {
+    const int64_t* key;  // device: {seed, call}; NULL: keep everything
+    uint32_t thr;        // an element is dropped iff its word < thr, or always with `all`
+    int all;
+    float scale;         // 1 / (1 - p)
+};
+
+struct PhiloxKey {
+    uint32_t k0, k1, c2, c3;
+};
+
+__device__ __forceinline__ PhiloxKey philox_key(const int64_t* key) {
+    PhiloxKey k;
+    const uint64_t s = (uint64_t)key[0], c = (uint64_t)key[1];
+    k.k0 = (uint32_t)s, k.k1 = (uint32_t)(s >> 32), k.c2 = (uint32_t)c, k.c3 = (uint32_t)(c >> 32);
+    return k;
+}
+
+__device__ __forceinline__ uint4 philox_block(const PhiloxKey k, uint64_t block) {
+    uint32_t c0 = (uint32_t)block, c1 = (uint32_t)(block >> 32), c2 = k.c2, c3 = k.c3, k0 = k.k0, k1 = k.k1;
+#pragma unroll
+    for (int r = 0; r < 10; ++r) {
+        const uint64_t a = (uint64_t)c0 * 0xD2511F53u, b = (uint64_t)c2 * 0xCD9E8D57u;
+        c0 = (uint32_t)(b >> 32) ^ c1 ^ k0;
+        c1 = (uint32_t)b;
+        c2 = (uint32_t)(a >> 32) ^ c3 ^ k1;
+        c3 = (uint32_t)a;
+        k0 += 0x9E3779B9u;
+        k1 += 0xBB67AE85u;
+    }
+    return make_uint4(c0, c1, c2, c3);
+}
+
+// fills thr / all / scale from p in [0, 1]; false if p is none of that
+inline bool make_drop(double p, const int64_t* key, Drop* d) {
+    if (!(p >= 0.0 && p <= 1.0) || (p > 0.0 && !key)) return false;
+    const double t = __builtin_rint(p * 4294967296.0);
+    d->key = p > 0.0 ? key : nullptr;
+    d->all = t >= 4294967296.0;
+    d->thr = d->all ? 0xFFFFFFFFu : (uint32_t)t;
+    d->scale = d->all ? 0.f : (float)(1.0 / (1.0 - p));
+    return true;
+}

@@ -79,6 +79,56 @@ class MinkowskiInstanceNorm(nn.Module):
         return f"MinkowskiInstanceNorm(nchannels={self.num_features})"
 
 
+class MinkowskiGroupNorm(nn.Module):
+    """Group norm per cloud over ``num_groups`` groups of channels, with the activation behind it and, while training, dropout behind that
+    (``ops.group_norm``: one pass over the rows, differentiable twice).  weight = ones(1,C), bias = zeros(1,C), as MinkowskiInstanceNorm's;
+    rows in fp32, fp16 or bf16.  ``seed``: of the dropout masks (None: drawn from torch's default generator)."""
+
+    def __init__(self, num_groups, num_channels, eps=1e-5, affine=True, activation=None, negative_slope=0.01, dropout=0.0, seed=None):
+        super().__init__()
+        if num_groups <= 0 or num_channels % num_groups:
+            raise ValueError(f"{num_channels} channels do not divide into {num_groups} groups")
+        if activation not in ops._ACTIVATIONS:
+            raise ValueError(f"unknown activation {activation!r}: none, relu, leaky_relu, silu or gelu")
+        self.num_groups, self.num_channels, self.eps = num_groups, num_channels, eps
+        self.activation, self.negative_slope, self.dropout = activation, negative_slope, ops._check_p(dropout)
+        self.weight = nn.Parameter(torch.ones(1, num_channels)) if affine else None
+        self.bias = nn.Parameter(torch.zeros(1, num_channels)) if affine else None
+        self.register_buffer("rng_state", ops.random_state(seed) if self.dropout > 0.0 else None, persistent=False)
+
+    def forward(self, x: SparseTensor) -> SparseTensor:
+        cm, ts = x.coordinate_manager, x.tensor_stride
+        p = self.dropout if self.training else 0.0
+        out = ops.group_norm(x.F, cm.seg_off(ts), self.num_groups, self.weight, self.bias, self.eps, self.activation, self.negative_slope, p,
+                             ops.random_key(self.rng_state) if p > 0.0 else None)
+        return SparseTensor(out, cm, ts)
+
+    def __repr__(self):
+        return (f"MinkowskiGroupNorm(ngroups={self.num_groups}, nchannels={self.num_channels}, activation={self.activation or 'none'}, "
+                f"dropout={self.dropout})")
+
+
+class MinkowskiDropout(nn.Module):
+    """Dropout on the feature rows while training (``ops.dropout``: the mask is computed from a seed and a call count, never stored); takes
+    and returns a SparseTensor or the rows of MinkowskiGlobalAvgPooling.  ``seed`` as in MinkowskiGroupNorm."""
+
+    def __init__(self, p=0.5, seed=None):
+        super().__init__()
+        self.p = ops._check_p(p)
+        self.register_buffer("rng_state", ops.random_state(seed), persistent=False)
+
+    def forward(self, x):
+        if not self.training or self.p == 0.0:
+            return x
+        out = ops.dropout(x.F, self.p, ops.random_key(self.rng_state))
+        if isinstance(x, SparseTensor):
+            return SparseTensor(out, x.coordinate_manager, x.tensor_stride)
+        return PooledBatch(out, x.coordinate_manager)
+
+    def __repr__(self):
+        return f"MinkowskiDropout(p={self.p})"
+
+
 class MinkowskiReLU(nn.Module):
     def __init__(self, inplace=False):
         super().__init__()

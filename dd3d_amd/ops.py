@@ -12,10 +12,11 @@ buffers (its results carry no graph), while
 """
 from __future__ import annotations
 
-from typing import Optional
+from typing import NamedTuple, Optional
 
 import torch
 from torch.autograd import Function
+from torch.autograd.function import once_differentiable
 
 from . import _lib as L
 from .sparse import CoordinateManager
@@ -430,6 +431,222 @@ class NormActPoolFn(Function):
         Y, w, b = ctx.saved_tensors
         dY, dw, db = _NormActPoolBwdFn.apply(g, Y, w, b, ctx.st)
         return dY, dw, db, None, None, None, None, None, None, None, None
+
+
+# ----------------------------------------------------------------------------------------------- dropout, group norm + activation
+# No counterpart in MinkowskiEngine: like the torch-native pieces of the step they are differentiated twice whatever the second-order
+# mode, and they take fp32, fp16 and bf16 rows (arithmetic in fp32, one rounding at the end).
+_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+_ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "leaky_relu": 2, "silu": 3, "gelu": 4}
+_MAX_NORM_CHANNELS = 4096
+
+
+def _rows_dtype(t: torch.Tensor, name: str) -> int:
+    if t.dtype not in _DTYPES:
+        raise RuntimeError(f"{name} must be float32, float16 or bfloat16, got {t.dtype}")
+    return _DTYPES[t.dtype]
+
+
+def _dense(t: torch.Tensor) -> torch.Tensor:
+    t = t.detach()
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _same_device(x: torch.Tensor, **others):
+    if not x.is_cuda:
+        raise RuntimeError("dd3d_amd kernels need GPU tensors (no CPU fallback); got a tensor on " + str(x.device))
+    for name, t in others.items():
+        if t is not None and t.device != x.device:
+            raise ValueError(f"{name} is on {t.device}, the rows are on {x.device}")
+
+
+def _check_p(p) -> float:
+    if not 0.0 <= float(p) <= 1.0:
+        raise ValueError(f"dropout probability has to be between 0 and 1, got {p}")
+    return float(p)
+
+
+def _check_drop(p, key):
+    p = _check_p(p)
+    if p > 0.0 and (key is None or key.dtype != torch.int64 or key.numel() != 2 or not key.is_contiguous()):
+        raise ValueError("dropout needs a key: a contiguous int64 tensor (seed, call) on the rows' device (ops.random_key)")
+    return p
+
+
+def random_state(seed: Optional[int] = None, device=None) -> torch.Tensor:
+    """State of a stream of dropout keys: int64 (seed, number of keys drawn).  ``seed`` None: drawn from torch's default generator."""
+    if seed is None:
+        seed = int(torch.empty((), dtype=torch.int64).random_().item())
+    seed = (int(seed) + 2 ** 63) % 2 ** 64 - 2 ** 63   # any Python integer, modulo 2^64
+    return torch.tensor([seed, 0], dtype=torch.int64, device=device)
+
+
+def random_key(state: torch.Tensor) -> torch.Tensor:
+    """The next key (seed, call) of ``state``, whose call count goes up by one on the device: no host round trip, and a captured graph
+    draws a new key at every replay."""
+    if state.dtype != torch.int64 or state.numel() != 2 or not state.is_contiguous():
+        raise ValueError("the state of a key stream is a contiguous int64 tensor (seed, call)")
+    _same_device(state)
+    with torch.cuda.device(state.device):
+        key = torch.empty_like(state)
+        L.call("dd3d_random_key", L.ptr(state), L.ptr(key), L.stream())
+    return key
+
+
+class DropoutFn(Function):
+    """Dropout that computes its mask from (key, element) whenever it needs it; its own gradient, to any order."""
+
+    @staticmethod
+    def forward(ctx, x, p, key):
+        x = _dense(x)
+        y = torch.empty_like(x)
+        C = x.shape[-1] if x.dim() else 1
+        with torch.cuda.device(x.device):
+            L.call("dd3d_dropout", L.ptr(x), _DTYPES[x.dtype], x.numel() // max(C, 1), C, p, L.ptr(key), L.ptr(y), L.stream())
+        ctx.save_for_backward(key)
+        ctx.p = p
+        return y
+
+    @staticmethod
+    def backward(ctx, g):
+        return DropoutFn.apply(g, ctx.p, ctx.saved_tensors[0]), None, None
+
+
+def dropout(x: torch.Tensor, p: float, key: torch.Tensor) -> torch.Tensor:
+    """Zero every element of ``x`` with probability ``p`` and scale the others by 1 / (1 - p).  Element (row, c) of the rows
+    ``x.view(-1, x.shape[-1])`` is dropped iff its word of a counter-based generator under ``key`` = int64 (seed, call) is below
+    round(p * 2^32): the mask is never stored, a call with the same key drops the same elements, and a dropped element is zero even
+    where ``x`` is not finite.  p = 0 returns ``x``."""
+    _rows_dtype(x, "x")
+    p = _check_drop(p, key)
+    _same_device(x, key=key)
+    return x if p == 0.0 else DropoutFn.apply(x, p, key)
+
+
+class _NormMeta(NamedTuple):
+    """What does not change between the passes of one group norm."""
+    G: int
+    act: int
+    slope: float
+    p: float
+
+    def head(self, x, seg_off, w, b):
+        """The arguments the three entry points share, in their order: rows, then the norm's shape and parameters."""
+        pdt = _DTYPES[(w if w is not None else b if b is not None else x).dtype]
+        return (_DTYPES[x.dtype], x.shape[0], x.shape[1], L.ptr(seg_off), seg_off.numel() - 1, self.G, L.ptr(w), L.ptr(b), pdt)
+
+    def workspace(self, x, seg_off, order):
+        n = int(L.lib.dd3d_group_norm_ws_bytes(x.shape[0], x.shape[1], seg_off.numel() - 1, self.G, order))
+        # its own block for every call: two graphs captured on one stream may be replayed side by side
+        return torch.empty(n, dtype=torch.uint8, device=x.device) if n > 0 else None
+
+
+def _opt_dense(t):
+    return None if t is None else _dense(t)
+
+
+def _norm_fwd(x, w, b, seg_off, key, meta, eps, keep):
+    x, w, b = _dense(x), _opt_dense(w), _opt_dense(b)
+    with torch.cuda.device(x.device):
+        y = torch.empty_like(x)
+        stats = torch.empty((2, seg_off.numel() - 1, meta.G), dtype=_F32, device=x.device) if keep else None
+        mean, rstd = (stats[0], stats[1]) if keep else (None, None)
+        ws = meta.workspace(x, seg_off, 0)
+        L.call("dd3d_group_norm_fwd", L.ptr(x), *meta.head(x, seg_off, w, b), eps, meta.act, meta.slope, meta.p, L.ptr(key), L.ptr(y), L.ptr(mean),
+               L.ptr(rstd), L.ptr(ws), 0 if ws is None else ws.numel(), L.stream())
+    return y, stats
+
+
+class GroupNormFn(Function):
+    """dropout(act(group_norm(x))) as one op; keeps x and the fp32 statistics, everything else is computed again."""
+
+    @staticmethod
+    def forward(ctx, x, w, b, seg_off, key, meta, eps):
+        y, stats = _norm_fwd(x, w, b, seg_off, key, meta, eps, True)
+        ctx.save_for_backward(x, w, b, seg_off, key, stats)
+        ctx.meta = meta
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        x, w, b, seg_off, key, stats = ctx.saved_tensors
+        dx, dw, db = _GroupNormGradFn.apply(dy, x, w, b, seg_off, key, stats, ctx.meta, ctx.needs_input_grad[:3])
+        return dx, dw, db, None, None, None, None
+
+
+class _GroupNormGradFn(Function):
+    """(dy, x, w, b) -> (dx, dw, db); differentiable once more (the matching loss is a function of dw and db)."""
+
+    @staticmethod
+    def forward(ctx, dy, x, w, b, seg_off, key, stats, meta, need):
+        ctx.save_for_backward(dy, x, w, b, seg_off, key, stats)
+        ctx.meta = meta
+        ctx.set_materialize_grads(False)
+        dy, x, w, b = _dense(dy), _dense(x), _opt_dense(w), _opt_dense(b)
+        with torch.cuda.device(x.device):
+            dx = torch.empty_like(x) if need[0] else None
+            dw = torch.empty_like(w) if need[1] else None
+            db = torch.empty_like(b) if need[2] else None
+            ws = meta.workspace(x, seg_off, 1)
+            L.call("dd3d_group_norm_bwd", L.ptr(dy), L.ptr(x), *meta.head(x, seg_off, w, b), meta.act, meta.slope, meta.p, L.ptr(key), L.ptr(stats[0]),
+                   L.ptr(stats[1]), L.ptr(dx), L.ptr(dw), L.ptr(db), L.ptr(ws), 0 if ws is None else ws.numel(), L.stream())
+        return dx, dw, db
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, ggx, ggw, ggb):
+        dy, x, w, b, seg_off, key, stats = ctx.saved_tensors
+        meta, need = ctx.meta, ctx.needs_input_grad
+        dy, x, w, b, ggx, ggw, ggb = _dense(dy), _dense(x), *(_opt_dense(t) for t in (w, b, ggx, ggw, ggb))
+        with torch.cuda.device(x.device):
+            ddy = torch.empty_like(dy) if need[0] else None
+            ddx = torch.empty_like(x) if need[1] else None
+            ddw = torch.empty_like(w) if need[2] else None
+            ddb = torch.empty_like(b) if need[3] else None
+            ws = meta.workspace(x, seg_off, 2)
+            L.call("dd3d_group_norm_bwd2", L.ptr(ggx), L.ptr(ggw), L.ptr(ggb), L.ptr(dy), L.ptr(x), *meta.head(x, seg_off, w, b), meta.act, meta.slope,
+                   meta.p, L.ptr(key), L.ptr(stats[0]), L.ptr(stats[1]), L.ptr(ddy), L.ptr(ddx), L.ptr(ddw), L.ptr(ddb), L.ptr(ws),
+                   0 if ws is None else ws.numel(), L.stream())
+        return ddy, ddx, ddw, ddb, None, None, None, None, None
+
+
+def group_norm(x: torch.Tensor, seg_off: torch.Tensor, num_groups: int, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
+               eps: float = 1e-5, activation: Optional[str] = "none", negative_slope: float = 0.01, dropout: float = 0.0,
+               key: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """dropout(activation(group_norm(x) * weight + bias)) over the rows ``x`` [M, C] of a ragged batch, in one pass over them.
+
+    Cloud ``b`` owns the rows ``seg_off[b]:seg_off[b + 1]`` (int32 [B + 1] on the device, ascending: ``CoordinateManager.seg_off``); mean and
+    biased variance are taken over its rows and the ``C / num_groups`` channels of a group.  Rows in no cloud come out as zeros.
+    ``weight`` / ``bias``: C values in fp32 or the rows' type; ``activation``: none, relu, leaky_relu (``negative_slope``), silu, gelu (exact).
+    ``dropout`` > 0 needs ``key`` and drops the elements that ``ops.dropout`` drops under that key.  Differentiable twice."""
+    _rows_dtype(x, "x")
+    if x.dim() != 2:
+        raise ValueError(f"x has to be rows [M, C], got {tuple(x.shape)}")
+    M, C = x.shape
+    if not 0 < num_groups <= C or C % num_groups:
+        raise ValueError(f"{C} channels do not divide into {num_groups} groups")
+    if C > _MAX_NORM_CHANNELS or M >= 2 ** 31:
+        raise ValueError(f"group_norm takes up to {_MAX_NORM_CHANNELS} channels and 2^31 - 1 rows, got [{M}, {C}]")
+    if seg_off.dtype != torch.int32 or seg_off.dim() != 1 or seg_off.numel() < 1 or not seg_off.is_contiguous():
+        raise ValueError("seg_off has to be a contiguous int32 tensor [B + 1]")
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is not None and (t.numel() != C or t.dtype not in (_F32, x.dtype)):
+            raise ValueError(f"{name} has to hold {C} values in float32 or {x.dtype}")
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise ValueError("weight and bias have to be of one type")
+    if activation not in _ACTIVATIONS:
+        raise ValueError(f"unknown activation {activation!r}: none, relu, leaky_relu, silu or gelu")
+    if not eps > 0.0:
+        raise ValueError(f"eps has to be positive, got {eps}")
+    if negative_slope != negative_slope:
+        raise ValueError("negative_slope is not a number")
+    p = _check_drop(dropout, key)
+    _same_device(x, seg_off=seg_off, weight=weight, bias=bias, key=key)
+    meta = _NormMeta(int(num_groups), _ACTIVATIONS[activation], float(negative_slope), p)
+    key = key if p > 0.0 else None
+    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or (bias is not None and bias.requires_grad)):
+        return GroupNormFn.apply(x, weight, bias, seg_off, key, meta, float(eps))
+    return _norm_fwd(x, weight, bias, seg_off, key, meta, float(eps), False)[0]
 
 
 # ----------------------------------------------------------------------------------------------- classifier over the dense placement

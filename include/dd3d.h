@@ -261,6 +261,38 @@ int dd3d_avg_pool_bwd(const float* g, const int32_t* cnt, const int32_t* parent,
 int dd3d_global_avg_pool_fwd(const float* X, int64_t M, const int32_t* seg_off, int B, int C, float* out, void* stream);
 int dd3d_global_avg_pool_bwd(const float* g, int64_t M, const int32_t* seg_off, int B, int C, float* dX, void* stream);
 
+/* Group norm with an activation and, with p > 0, dropout behind it, over ragged channels-last rows: X[M,C] of type dtype (0 fp32, 1 fp16,
+ * 2 bf16), cloud b owns the rows [seg_off[b], seg_off[b+1]) (int32[B+1] on the device, ascending), group j the channels
+ * [j*C/G, (j+1)*C/G).  Biased variance over the rows of a cloud and the channels of a group; statistics, sums and the activation in fp32,
+ * one rounding to dtype at the end.  weight / bias: [C], nullable, both of type pdtype (0, or dtype).  act: 0 none, 1 ReLU, 2 leaky ReLU
+ * (slope below zero), 3 SiLU, 4 GELU (the normal distribution's).  p, key: as in dd3d_dropout (key nullable with p = 0).
+ * Rows of [0, M) that belong to no cloud come out as zeros; rows from M on are not touched.  C <= 4096, M < 2^31, eps > 0.
+ *   fwd : Y = dropout(act(xhat*weight + bias)); mean / rstd [B,G] fp32 are kept for the gradients (nullable pair; zeros for an empty cloud)
+ *   bwd : dX (nullable), dweight / dbias [C] in pdtype (each nullable) from dY
+ *   bwd2: the gradient of bwd: from the cotangents ggX[M,C], ggW[C], ggB[C] of its three results (each nullable) the cotangents of its
+ *         inputs dY, X, weight, bias (each result nullable)
+ * ws: dd3d_group_norm_ws_bytes(..., order) bytes, order 0 / 1 / 2 = fwd / bwd / bwd2.  Every sum has a fixed order: equal inputs, equal bits.
+ * No counterpart in the reference. */
+int64_t dd3d_group_norm_ws_bytes(int64_t M, int C, int B, int G, int order);
+int dd3d_group_norm_fwd(const void* X, int dtype, int64_t M, int C, const int32_t* seg_off, int B, int G, const void* weight, const void* bias,
+                        int pdtype, float eps, int act, float slope, double p, const int64_t* key, void* Y, float* mean, float* rstd, void* ws,
+                        int64_t ws_bytes, void* stream);
+int dd3d_group_norm_bwd(const void* dY, const void* X, int dtype, int64_t M, int C, const int32_t* seg_off, int B, int G, const void* weight,
+                        const void* bias, int pdtype, int act, float slope, double p, const int64_t* key, const float* mean, const float* rstd,
+                        void* dX, void* dweight, void* dbias, void* ws, int64_t ws_bytes, void* stream);
+int dd3d_group_norm_bwd2(const void* ggX, const void* ggW, const void* ggB, const void* dY, const void* X, int dtype, int64_t M, int C,
+                         const int32_t* seg_off, int B, int G, const void* weight, const void* bias, int pdtype, int act, float slope, double p,
+                         const int64_t* key, const float* mean, const float* rstd, void* ddY, void* ddX, void* ddweight, void* ddbias, void* ws,
+                         int64_t ws_bytes, void* stream);
+
+/* Y = dropout(X) over rows x C elements of type dtype, without a stored mask: element (row, c) is dropped (zero, whatever it held) iff word
+ * c%4 of Philox4x32-10 at counter (row*ceil(C/4) + c/4, call) under key seed is below round(p*2^32), else scaled by 1/(1-p); key =
+ * int64[2] {seed, call} on the device.  Its gradient is the same call on the incoming gradient.  0 <= p <= 1.  X == Y is allowed.
+ * dd3d_random_key: key = state, then state[1] += 1, on the stream: a replayed graph draws a new mask every time.
+ * No counterpart in the reference. */
+int dd3d_dropout(const void* X, int dtype, int64_t rows, int64_t C, double p, const int64_t* key, void* Y, void* stream);
+int dd3d_random_key(int64_t* state, int64_t* key, void* stream);
+
 /* backward of the same three ops for every input row; gw_w/gw_b[G,C] are the per-group affine gradients (nullable pair);
  * ga_out (nullable) keeps the ReLU-masked pooled gradient; ga_prev + gw_extra[G,C] (nullable pair) add ga_prev*gw_extra[group]. */
 int64_t dd3d_arp_bwd_ws_bytes(int64_t M_in, int G);

@@ -120,7 +120,8 @@ struct PhiloxKey {
 __device__ __forceinline__ PhiloxKey philox_key(const int64_t* key) {
     PhiloxKey k;
     const uint64_t s = (uint64_t)key[0], c = (uint64_t)key[1];
-    k.k0 = (uint32_t)s, k.k1 = (uint32_t)(s >> 32), k.c2 = (uint32_t)c, k.c3 = (uint32_t)(c >> 32);
+    const auto uniform = [](uint64_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)v); };   // scalar registers
+    k.k0 = uniform(s), k.k1 = uniform(s >> 32), k.c2 = uniform(c), k.c3 = uniform(c >> 32);
     return k;
 }
 

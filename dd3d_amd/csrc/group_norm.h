@@ -1,0 +1,678 @@
+// Device code of the group norm (formulas: group_norm.hip), shared by its three passes and instantiated per row type and pass in group_norm_*.hip.
+//
+// All three passes are bound by HBM: the arithmetic is a few dozen fp32 operations an element.  What they need is sums over (cloud, group)
+// before anything can be written, so a row has to be read twice unless it stays on chip in between.  Layout of the work:
+//   * a SLAB is a run of whole groups, at least one 128-byte line of a row wide; a workgroup owns one slab of one cloud after another.
+//     Thread t holds V channels (one 16-byte vector) of the rows rl, rl + RL, ...: the rows of a chunk of NR * RL are loaded at once into
+//     registers, so up to that many loads are in flight per thread, and stay there while the workgroup forms the sums -- HBM sees every
+//     row once.  Four waves a workgroup: with sixteen the instructions that every wave spends on the sums outweighed the rows
+//     (82-row clouds of 128 channels, fp32 forward: 97 us against 64).
+//   * a cloud longer than one chunk and up to `Tl` rows is walked again by the same workgroup (its slab mostly comes out of the caches).
+//   * a longer cloud ("large") is cut by WINDOWS of CH rows of the whole batch; Tl >= CH, so a window meets at most two large clouds: the
+//     one it begins in (slot 2w) and one that begins inside it (slot 2w + 1).  Windows write partial sums, a second launch joins them
+//     (every workgroup for itself, in window order) and walks the rows again.  Which clouds are large is read from seg_off on the device.
+// Sums are fp32: per thread over its rows, then lanes, waves, windows in a fixed order.  Variances come from differences to a mean
+// at every level (thread, workgroup, windows), never from a mean of squares.
+#pragma once
+#include "feature_math.h"
+
+namespace gn {
+
+struct Norm {
+    int M, C, B, G, Cg, pdt;   // M < 2^31: row numbers fit 32 bits, element offsets do not
+    const int* seg;
+    const void *W, *Bi;
+    float eps, slope;
+    Drop drop;
+};
+
+// n / d for n, d < 2^16 as one wide product
+struct Div {
+    uint32_t mul;
+    int d;
+};
+__device__ __forceinline__ int quot(int n, const Div& d) { return d.d == 1 ? n : (int)__umulhi((uint32_t)n, d.mul); }
+
+// launch geometry (plan() in group_norm.hip); everything is uniform
+struct Geo {
+    int k, nslab;        // groups per slab, slabs
+    int CL, RL, lcl;     // channel lanes (vectors per row of the slab), row lanes, log2(CL) if CL is a power of two <= 64, else -1
+    int fast;            // groups and slabs are powers of two of lanes: sums by shuffles
+    int cw;              // columns of one group: vectors where a vector lies inside one group, else channels
+    int U, NW, CH, Tl;   // cloud units, windows, rows per window, longest cloud that one workgroup takes
+    int units;           // of this launch
+    int quads;           // ceil(C / 4)
+    int kb;              // quantities reduced at once where the sums go through LDS
+    int red;             // floats of LDS for them
+    Div dCL, dCg;
+};
+
+// ---- one thread's V channels of one row --------------------------------------------------------------------------------------
+template <typename T, int V>
+struct Raw {
+    uint32_t __attribute__((ext_vector_type(V * (int)sizeof(T) / 4))) u;
+};
+__device__ __forceinline__ float raw_get(const Raw<float, 4>& r, int i) { return __uint_as_float(r.u[i]); }
+template <int V>
+__device__ __forceinline__ float raw_get(const Raw<half_t, V>& r, int i) {
+    const uint16_t h = (uint16_t)(r.u[i >> 1] >> ((i & 1) * 16));
+    half_t f;
+    __builtin_memcpy(&f, &h, 2);
+    return (float)f;
+}
+template <int V>
+__device__ __forceinline__ float raw_get(const Raw<bf16_t, V>& r, int i) {
+    return __uint_as_float((i & 1) ? r.u[i >> 1] & 0xFFFF0000u : r.u[i >> 1] << 16);
+}
+
+// AL: the vector is whole, aligned and loaded at once; otherwise channels [lo, hi) of it exist and are moved one by one
+template <typename T, int V, bool AL>
+__device__ __forceinline__ Raw<T, V> load_row(const T* p, int lo, int hi) {
+    Raw<T, V> r;
+    if (AL) {
+        __builtin_memcpy(&r, __builtin_assume_aligned(p, V * sizeof(T)), sizeof(r));
+    } else {
+        T e[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) e[i] = (i >= lo && i < hi) ? p[i] : narrow<T>(0.f);
+        __builtin_memcpy(&r, e, sizeof(r));
+    }
+    return r;
+}
+template <typename T, int V, bool AL>
+__device__ __forceinline__ void store_row(T* p, const float (&v)[V], int lo, int hi) {
+    T e[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) e[i] = narrow<T>(v[i]);
+    if (AL) {
+        __builtin_memcpy(__builtin_assume_aligned(p, V * sizeof(T)), e, sizeof(e));
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (i >= lo && i < hi) p[i] = e[i];
+    }
+}
+
+// ---- where this thread stands ---------------------------------------------------------------------------------------------------
+// The compile-time side of a launch.  UNI: every vector lies inside one group (Cg % V == 0), so a thread has one set of statistics;
+// otherwise its channels may belong to up to four groups.  AL: whole, aligned vectors.
+template <typename T_, int V_, bool AL_, bool UNI_, int FAM_, int THREADS_, int NR_>
+struct Cfg {
+    typedef T_ T;
+    static constexpr int V = V_, FAM = FAM_, THREADS = THREADS_, NR = NR_, NS = UNI_ ? 1 : V_, WAVES = THREADS_ / 64;
+    static constexpr bool AL = AL_, UNI = UNI_;
+    static constexpr int at(int i) { return UNI_ ? 0 : i; }
+    typedef Raw<T_, V_> Row;
+};
+
+template <typename Z>
+struct Spot {
+    int unit, slab;
+    int cl, rl, wave, lane;
+    int s0, s1, gs;       // channels [s0, s1) of the slab, groups
+    int c0, lo, hi;       // first channel of this thread, which of its V exist in the slab
+    bool on;              // this thread has rows at all
+    int buf;              // which half of the sums' LDS is next
+    uint32_t off, step;   // elements from a chunk's first row to this thread's first vector, and from one of its rows to the next
+    uint32_t word;        // the same in blocks of random words
+    uint32_t cc;          // c0, or for a thread without channels some vector that exists
+    int j[Z::NS];         // group (within the slab) of its channels
+    float w[Z::V], b[Z::V];
+};
+
+template <int V>
+__device__ __forceinline__ void load_params(const void* p, int pdt, int c0, int lo, int hi, float otherwise, float (&v)[V]) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = otherwise;
+    if (!p) return;
+    if (pdt == DD3D_F32) {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (i >= lo && i < hi) v[i] = ((const float*)p)[c0 + i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (i >= lo && i < hi) v[i] = load_param(p, pdt, c0 + i);
+    }
+}
+
+// consecutive workgroups go to consecutive XCDs: the slabs of one unit are eight workgroups apart, on one XCD, so lines that two slabs
+// share are fetched into one L2
+__device__ __forceinline__ bool place(const Geo& g, int& unit, int& slab) {
+    const int lo = blockIdx.x & 7, rest = blockIdx.x >> 3, hi = g.nslab == 1 ? rest : rest / g.nslab;
+    slab = rest - hi * g.nslab;
+    unit = hi * 8 + lo;
+    return unit < g.units;
+}
+
+template <typename Z>
+__device__ __forceinline__ void locate(const Norm& a, const Geo& g, int unit, int slab, Spot<Z>& s) {
+    s.unit = unit, s.slab = slab;
+    s.lane = threadIdx.x & 63, s.wave = threadIdx.x >> 6;
+    s.rl = quot(threadIdx.x, g.dCL), s.cl = threadIdx.x - s.rl * g.CL;
+    s.s0 = s.slab * g.k * a.Cg;
+    s.gs = min(g.k, a.G - s.slab * g.k);
+    s.s1 = s.s0 + s.gs * a.Cg;
+    s.c0 = (s.s0 & ~3) + s.cl * Z::V;   // from a multiple of four, where the random words' blocks begin
+    s.lo = s.s0 - s.c0, s.hi = s.s1 - s.c0;
+    s.on = s.rl < g.RL && s.hi > 0;
+    s.buf = 0;
+    s.cc = Z::AL ? min(s.c0, s.s1 - Z::V) : s.c0;
+    s.off = s.rl * a.C + s.cc, s.step = g.RL * a.C;
+    s.word = s.rl * g.quads + s.c0 / 4;
+#pragma unroll
+    for (int i = 0; i < Z::NS; ++i) s.j[i] = min(quot(max(s.c0 + i - s.s0, 0), g.dCg), s.gs - 1);
+    load_params<Z::V>(a.W, a.pdt, s.c0, s.on ? s.lo : Z::V, s.hi, 1.f, s.w);
+    load_params<Z::V>(a.Bi, a.pdt, s.c0, s.on ? s.lo : Z::V, s.hi, 0.f, s.b);
+}
+
+// a value the compiler must not compute ahead of the loop it is used in: a chunk's eight offsets are one addition each, and kept over the
+// whole kernel they would push the rows out of the registers
+__device__ __forceinline__ uint32_t here(uint32_t v) {
+    asm volatile("" : "+v"(v));
+    return v;
+}
+
+// 1 / sqrt(v) of a normal v > 0: the hardware's value and one Newton step, within about a half step of the exact one at a seventh of the
+// instructions of a division by a square root
+__device__ __forceinline__ float rsqrt_newton(float v) {
+    const float r = __builtin_amdgcn_rsqf(v);
+    return fmaf(r * 0.5f, fmaf(-v * r, r, 1.f), r);
+}
+
+// ---- rows of a cloud ------------------------------------------------------------------------------------------------------------
+struct Range {
+    int r0, r1;
+};
+__device__ __forceinline__ Range cloud_rows(const Norm& a, int b) {
+    // uniform, and kept in scalar registers: the compiler cannot know it of a value loaded through seg
+    Range r;
+    r.r0 = min(max(__builtin_amdgcn_readfirstlane(a.seg[b]), 0), a.M);
+    r.r1 = min(max(__builtin_amdgcn_readfirstlane(a.seg[b + 1]), r.r0), a.M);
+    return r;
+}
+
+// the cloud that row `at` belongs to (-1 or B: none): 64-ary search, every wave for itself
+__device__ __forceinline__ int cloud_of(const Norm& a, int at) {
+    int lo = 0, n = a.B + 1;   // seg[lo - 1] <= at < seg[lo + n], over the entries seg[0 .. B]
+    const int lane = threadIdx.x & 63;
+    while (n > 0) {
+        const int step = (n + 63) / 64, i = lo + lane * step;
+        const unsigned long long m = __ballot(i < lo + n && a.seg[min(i, a.B)] <= at);
+        const int c = __popcll(m);   // entries lo, lo + step, .. are <= at for the first c lanes
+        if (c == 0) break;
+        const int first = lo + (c - 1) * step + 1, end = min(lo + n, lo + c * step);
+        lo = first, n = end - first;
+    }
+    return __builtin_amdgcn_readfirstlane(lo) - 1;
+}
+
+// a window's part of a large cloud
+struct Piece {
+    int b, slot;
+    Range all, part;
+};
+// the number of pieces; the first launch looks for them and notes the number in found[w], the later ones read it
+template <bool LOOK>
+__device__ __forceinline__ int window_pieces(const Norm& a, const Geo& g, int w, int* found, Piece (&p)[2]) {
+    if (!LOOK && __builtin_amdgcn_readfirstlane(found[w]) == 0) return 0;
+    const int a0 = w * g.CH, a1 = a0 + min(g.CH, a.M - a0);
+    int n = 0;
+    const int b0 = cloud_of(a, a0), b1 = cloud_of(a, a1 - 1);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int b = i ? b1 : b0;
+        if (b < 0 || b >= a.B || (i && b1 == b0)) continue;
+        const Range r = cloud_rows(a, b);
+        if (r.r1 - r.r0 <= g.Tl) continue;
+        Piece q;
+        q.b = b, q.all = r, q.slot = 2 * w + (r.r0 < a0 ? 0 : 1);
+        q.part.r0 = max(r.r0, a0), q.part.r1 = min(r.r1, a1);
+        if (n) p[1] = q;
+        else p[0] = q;
+        ++n;
+    }
+    if (LOOK && threadIdx.x == 0) found[w] = n;   // (by every slab's workgroup, the same number)
+    return n;
+}
+// the slots of a large cloud, in window order
+__device__ __forceinline__ int piece_count(const Geo& g, const Range& r) { return (r.r1 - 1) / g.CH - r.r0 / g.CH + 1; }
+__device__ __forceinline__ int piece_slot(const Geo& g, const Range& r, int i) { return 2 * (r.r0 / g.CH + i) + (i == 0 ? 1 : 0); }
+__device__ __forceinline__ int piece_rows(const Geo& g, const Range& r, int i) {
+    const int w0 = (r.r0 / g.CH + i) * g.CH;
+    return min(r.r1 - w0, g.CH) - max(r.r0 - w0, 0);
+}
+
+// rows of [0, M) in no cloud: zeros, shared out over all workgroups of the launch
+template <typename T>
+__device__ __forceinline__ void zero_rest(const Norm& a, T* Y) {
+    if (!Y) return;
+    const int lo = min(max(a.seg[0], 0), a.M), hi = min(max(a.seg[a.B], lo), a.M);
+    const int64_t n0 = (int64_t)lo * a.C, n = n0 + (int64_t)(a.M - hi) * a.C;
+    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x)
+        Y[i < n0 ? i : (int64_t)hi * a.C + (i - n0)] = narrow<T>(0.f);
+}
+
+// ---- sums -----------------------------------------------------------------------------------------------------------------------
+// v[q][i], per thread and (with !UNI) channel -> the sum over the rows of the workgroup and the channels of the group that thread and channel
+// belong to.  Lanes without rows bring zeros.
+template <int K, typename Z>
+__device__ __forceinline__ void group_sums(float (&v)[K][Z::NS], const Norm& a, const Geo& g, Spot<Z>& s, float* lds) {
+    if (Z::UNI && g.fast) {
+        // the group's lanes, then the wave's row lanes; one value per wave and group through LDS.  Two buffers in turn: one barrier a call
+        for (int o = 1; o < g.cw; o <<= 1) {
+#pragma unroll
+            for (int q = 0; q < K; ++q) v[q][0] += __shfl_xor(v[q][0], o, 64);
+        }
+        for (int o = g.CL; o < 64; o <<= 1) {
+#pragma unroll
+            for (int q = 0; q < K; ++q) v[q][0] += __shfl_xor(v[q][0], o, 64);
+        }
+        float* red = lds + s.buf * K * Z::WAVES * g.k;
+        s.buf ^= 1;
+        if (s.lane < g.CL && (s.lane & (g.cw - 1)) == 0 && s.hi > 0) {
+#pragma unroll
+            for (int q = 0; q < K; ++q) red[(q * Z::WAVES + s.wave) * g.k + s.j[0]] = v[q][0];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int q = 0; q < K; ++q) {
+            float t = 0.f;
+#pragma unroll
+            for (int p = 0; p < Z::WAVES; ++p) t += red[(q * Z::WAVES + p) * g.k + s.j[0]];
+            v[q][0] = t;
+        }
+        return;
+    }
+    // through LDS: [row lane][column], summed per column, then per group
+    const int cols = g.CL * Z::NS, c_first = Z::UNI ? 0 : s.s0 & 3;   // the slab's first column
+    float *tot = lds + g.red, *out = tot + g.kb * cols;
+    for (int k0 = 0; k0 < K; k0 += g.kb) {
+        const int kn = min(K - k0, g.kb);
+        __syncthreads();
+        if (s.rl < g.RL) {
+#pragma unroll
+            for (int q = 0; q < K; ++q)
+                if (q >= k0 && q < k0 + kn) {
+#pragma unroll
+                    for (int i = 0; i < Z::NS; ++i) lds[((q - k0) * g.RL + s.rl) * cols + s.cl * Z::NS + i] = v[q][i];
+                }
+        }
+        __syncthreads();
+        for (int c = threadIdx.x; c < kn * cols; c += Z::THREADS) {
+            const int q = c / cols;
+            const float* from = lds + q * g.RL * cols + (c - q * cols);
+            float t = 0.f;
+            for (int p = 0; p < g.RL; ++p) t += from[p * cols];
+            tot[c] = t;
+        }
+        __syncthreads();
+        // eight lanes a group
+        for (int jb = threadIdx.x >> 3; jb < kn * s.gs; jb += Z::THREADS / 8) {
+            const int q = jb / s.gs, j = jb - q * s.gs;
+            float t = 0.f;
+            for (int i = threadIdx.x & 7; i < g.cw; i += 8) t += tot[q * cols + c_first + j * g.cw + i];
+            t += __shfl_xor(t, 1, 64);
+            t += __shfl_xor(t, 2, 64);
+            t += __shfl_xor(t, 4, 64);
+            if ((threadIdx.x & 7) == 0) out[(k0 + q) * g.k + j] = t;
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < K; ++q)
+#pragma unroll
+        for (int i = 0; i < Z::NS; ++i) v[q][i] = out[q * g.k + s.j[i]];
+}
+
+// acc[q][i] per thread and channel -> slot[q * C + c], the sum over the workgroup's rows (parameter gradients, once a workgroup)
+template <int K, typename Z>
+__device__ __forceinline__ void column_sums(float (&acc)[K][Z::V], const Norm& a, const Geo& g, const Spot<Z>& s, float* lds, float* slot) {
+    int np = g.RL;
+    const int cols = g.CL * Z::V;
+    if (g.lcl >= 0) {
+        for (int o = g.CL; o < 64; o <<= 1) {
+#pragma unroll
+            for (int q = 0; q < K; ++q)
+#pragma unroll
+                for (int i = 0; i < Z::V; ++i) acc[q][i] += __shfl_xor(acc[q][i], o, 64);
+        }
+        np = Z::WAVES;
+    }
+    const int p = g.lcl >= 0 ? s.wave : s.rl;
+    const bool writes = g.lcl >= 0 ? s.lane < g.CL : s.rl < g.RL;
+#pragma unroll
+    for (int q = 0; q < K; ++q) {
+        __syncthreads();
+        if (writes) {
+#pragma unroll
+            for (int i = 0; i < Z::V; ++i) lds[p * cols + s.cl * Z::V + i] = acc[q][i];
+        }
+        __syncthreads();
+        for (int c = threadIdx.x; c < cols; c += Z::THREADS) {
+            const int ch = (s.s0 & ~3) + c;
+            float t = 0.f;
+            for (int r = 0; r < np; ++r) t += lds[r * cols + c];
+            if (ch >= s.s0 && ch < s.s1) slot[(int64_t)q * a.C + ch] = t;
+        }
+    }
+}
+
+// part[slot][G][K]: this thread's channel that writes for its group
+template <typename Z>
+__device__ __forceinline__ bool writes_group(const Norm& a, const Spot<Z>& s, int i) {
+    return s.rl == 0 && s.on && i >= s.lo && i < s.hi && s.j[i] * a.Cg == s.c0 + i - s.s0;
+}
+template <int K, typename Z>
+__device__ __forceinline__ void put_part(float* part, int slot, const float (&v)[K][Z::NS], const Norm& a, const Geo& g, const Spot<Z>& s) {
+#pragma unroll
+    for (int i = 0; i < Z::NS; ++i)
+        if (writes_group(a, s, i)) {
+            float* to = part + ((int64_t)slot * a.G + s.slab * g.k + s.j[i]) * K;
+#pragma unroll
+            for (int q = 0; q < K; ++q) to[q] = v[q][i];
+        }
+}
+
+// the sums of a large cloud's pieces, in window order: a wave a group, lanes over pieces
+template <int K, typename Z>
+__device__ __forceinline__ void join_parts(const float* part, const Range& r, float (&v)[K][Z::NS], const Norm& a, const Geo& g, const Spot<Z>& s, float* lds) {
+    float* out = lds + g.red + g.kb * g.CL * Z::NS;
+    const int n = piece_count(g, r);
+    __syncthreads();
+    for (int j = s.wave; j < s.gs; j += Z::WAVES) {
+        float t[K];
+#pragma unroll
+        for (int q = 0; q < K; ++q) t[q] = 0.f;
+        for (int o = s.lane; o < n; o += 64) {
+            const float* from = part + ((int64_t)piece_slot(g, r, o) * a.G + s.slab * g.k + j) * K;
+#pragma unroll
+            for (int q = 0; q < K; ++q) t[q] += from[q];
+        }
+#pragma unroll
+        for (int q = 0; q < K; ++q) {
+            t[q] = wave_sum(t[q]);
+            if (s.lane == 0) out[q * g.k + j] = t[q];
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < K; ++q)
+#pragma unroll
+        for (int i = 0; i < Z::NS; ++i) v[q][i] = out[q * g.k + s.j[i]];
+}
+
+// the elements of this thread's vector that dropout keeps, as bits
+template <int V>
+__device__ __forceinline__ uint32_t keep_bits(const Drop& d, const PhiloxKey& k, uint64_t block) {
+    uint32_t m = 0;
+    if (d.all) return 0;
+#pragma unroll
+    for (int h = 0; h < V / 4; ++h) {
+        const uint4 w = philox_block(k, block + h);
+        m |= (uint32_t)(w.x >= d.thr) << (4 * h) | (uint32_t)(w.y >= d.thr) << (4 * h + 1) | (uint32_t)(w.z >= d.thr) << (4 * h + 2) |
+             (uint32_t)(w.w >= d.thr) << (4 * h + 3);
+    }
+    return m;
+}
+__device__ __forceinline__ PhiloxKey drop_key(const Drop& d) {
+    PhiloxKey k = {0, 0, 0, 0};
+    if (d.key) k = philox_key(d.key);
+    return k;
+}
+
+// the thread's rows of the chunk that begins at `from` with `left` rows before the end.  No load waits behind a branch of its own: threads
+// past the end (and threads without channels) read the last row again.
+template <typename Z>
+__device__ __forceinline__ void load_chunk(const typename Z::T* from, int C, int left, const Geo& g, const Spot<Z>& s, typename Z::Row (&x)[Z::NR]) {
+    const uint32_t last = (uint32_t)(left - 1) * (uint32_t)C + s.cc, off = here(s.off);
+#pragma unroll
+    for (int n = 0; n < Z::NR; ++n) {
+        if (n * g.RL < left)
+            x[n] = load_row<typename Z::T, Z::V, Z::AL>(
+                (const typename Z::T*)((const char*)from + min(off + n * s.step, last) * (uint32_t)sizeof(typename Z::T)), s.on ? s.lo : Z::V, s.hi);
+    }
+}
+template <typename Z>
+__device__ __forceinline__ void store_at(typename Z::T* to, uint32_t off, const float (&v)[Z::V], const Spot<Z>& s) {
+    store_row<typename Z::T, Z::V, Z::AL>((typename Z::T*)((char*)to + off * (uint32_t)sizeof(typename Z::T)), v, s.lo, s.hi);
+}
+// element offset of row `base`, and its first block of random words
+__device__ __forceinline__ int64_t row_at(const Norm& a, int base) { return (int64_t)base * a.C; }
+__device__ __forceinline__ uint64_t words_at(const Geo& g, int base) { return (uint64_t)(uint32_t)base * (uint32_t)g.quads; }
+
+// one row after the other: the scheduler would otherwise work on all of a chunk's rows at once and run out of registers
+__device__ __forceinline__ void row_border() { __builtin_amdgcn_sched_barrier(0); }
+
+// ---- forward --------------------------------------------------------------------------------------------------------------------
+template <typename Z>
+struct Fwd {
+    typedef typename Z::T T;
+    static constexpr int V = Z::V, NR = Z::NR, NS = Z::NS;
+    const Norm& a;
+    const Geo& g;
+    Spot<Z>& s;
+    const T* X;
+    T* Y;
+    float* lds;
+    PhiloxKey key;
+
+    // per-thread count, mean and centred sum of squares, joined with those of one more chunk
+    __device__ __forceinline__ void add_rows(int all, const typename Z::Row (&z)[NR], float& cnt, float (&mu)[NS], float (&m2)[1][NS]) {
+        const int left = s.on ? all : 0;
+        float n1 = 0.f, sx[NS], q[NS];
+#pragma unroll
+        for (int i = 0; i < NS; ++i) sx[i] = q[i] = 0.f;
+#pragma unroll
+        for (int n = 0; n < NR; ++n)
+            if (s.rl + n * g.RL < left) {
+                n1 += (float)(V / NS);
+#pragma unroll
+                for (int i = 0; i < V; ++i) sx[Z::at(i)] += raw_get(z[n], i);
+            }
+        if (n1 == 0.f) return;
+        // (reciprocals to a step: any shift near the mean serves the sum of squares)
+        const float inv = __builtin_amdgcn_rcpf(n1), sum = cnt + n1, part = n1 * __builtin_amdgcn_rcpf(sum), cross = cnt * part;
+#pragma unroll
+        for (int i = 0; i < NS; ++i) sx[i] *= inv;
+#pragma unroll
+        for (int n = 0; n < NR; ++n)
+            if (s.rl + n * g.RL < left) {
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    const float d = raw_get(z[n], i) - sx[Z::at(i)];
+                    q[Z::at(i)] = fmaf(d, d, q[Z::at(i)]);
+                }
+            }
+#pragma unroll
+        for (int i = 0; i < NS; ++i) {
+            const float d = sx[i] - mu[i];
+            mu[i] = fmaf(d, part, mu[i]);
+            m2[0][i] += fmaf(d * d, cross, q[i]);
+        }
+        cnt = sum;
+    }
+
+    // the thread's part -> v[0] = mean, v[1] = centred sum of squares of its groups over `rows` rows
+    __device__ __forceinline__ void join(int rows, float cnt, const float (&mu)[NS], float (&m2)[1][NS], float (&v)[2][NS]) {
+        const float inv = 1.f / ((float)rows * (float)a.Cg);
+        float sum[1][NS];
+#pragma unroll
+        for (int i = 0; i < NS; ++i) sum[0][i] = cnt * mu[i];
+        group_sums<1, Z>(sum, a, g, s, lds);
+#pragma unroll
+        for (int i = 0; i < NS; ++i) {
+            v[0][i] = sum[0][i] * inv;
+            const float d = mu[i] - v[0][i];
+            m2[0][i] = cnt > 0.f ? fmaf(d * cnt, d, m2[0][i]) : 0.f;
+        }
+        group_sums<1, Z>(m2, a, g, s, lds);
+#pragma unroll
+        for (int i = 0; i < NS; ++i) v[1][i] = m2[0][i];
+    }
+
+    // statistics of rows that take several chunks
+    __device__ __forceinline__ void stats(const Range& r, float (&v)[2][NS]) {
+        float cnt = 0.f, mu[NS], m2[1][NS];
+#pragma unroll
+        for (int i = 0; i < NS; ++i) mu[i] = m2[0][i] = 0.f;
+        for (int base = r.r0; base < r.r1; base += NR * g.RL) {
+            typename Z::Row z[NR];
+            load_chunk<Z>(X + row_at(a, base), a.C, r.r1 - base, g, s, z);
+            add_rows(r.r1 - base, z, cnt, mu, m2);
+        }
+        join(r.r1 - r.r0, cnt, mu, m2, v);
+    }
+
+    // 1 / standard deviation from v of a whole cloud of `rows` rows; `keep`: this workgroup writes the statistics
+    __device__ __forceinline__ void finish(const float (&v)[2][NS], int b, int rows, bool keep, float* mean_out, float* rstd_out, float (&rstd)[NS]) {
+        const float inv = 1.f / ((float)rows * (float)a.Cg);
+#pragma unroll
+        for (int i = 0; i < NS; ++i) {
+            rstd[i] = rsqrt_newton(fmaf(v[1][i], inv, a.eps));
+            if (mean_out && keep && writes_group(a, s, i)) {
+                const int64_t at = (int64_t)b * a.G + s.slab * g.k + s.j[i];
+                mean_out[at] = v[0][i], rstd_out[at] = rstd[i];
+            }
+        }
+    }
+
+    // y of rows that take several chunks
+    __device__ __forceinline__ void apply(const Range& r, const float (&mean)[NS], const float (&rstd)[NS]) {
+        for (int base = r.r0; base < r.r1; base += NR * g.RL) {
+            typename Z::Row z[NR];
+            load_chunk<Z>(X + row_at(a, base), a.C, r.r1 - base, g, s, z);
+            rows_out(base, r.r1 - base, mean, rstd, z);
+        }
+    }
+
+    // a cloud that one chunk holds: its rows are read once
+    __device__ __forceinline__ void short_cloud(const Range& r, int b, float* mean_out, float* rstd_out) {
+        const int rows = r.r1 - r.r0;
+        typename Z::Row z[NR];
+        load_chunk<Z>(X + row_at(a, r.r0), a.C, rows, g, s, z);
+        float cnt = 0.f, mu[NS], m2[1][NS], v[2][NS], rstd[NS];
+#pragma unroll
+        for (int i = 0; i < NS; ++i) mu[i] = m2[0][i] = 0.f;
+        add_rows(rows, z, cnt, mu, m2);
+        join(rows, cnt, mu, m2, v);
+        finish(v, b, rows, true, mean_out, rstd_out, rstd);
+        rows_out(r.r0, rows, v[0], rstd, z);
+    }
+
+    __device__ __forceinline__ void rows_out(int base, int all, const float (&mean)[NS], const float (&rstd)[NS], const typename Z::Row (&z)[NR]) {
+        const int left = s.on ? all : 0;
+        T* to = Y + row_at(a, base);
+        const uint64_t words = words_at(g, base);
+        const uint32_t off = here(s.off), word = here(s.word);
+#pragma unroll
+        for (int n = 0; n < NR; ++n) {
+            row_border();
+            if (s.rl + n * g.RL >= left) continue;
+            float y[V], d1, d2;
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                y[i] = activate<Z::FAM, 0>(fmaf((raw_get(z[n], i) - mean[Z::at(i)]) * rstd[Z::at(i)], s.w[i], s.b[i]), a.slope, &d1, &d2);
+            if (a.drop.key) {
+                const uint32_t keep = keep_bits<V>(a.drop, key, words + (word + n * (uint32_t)(g.RL * g.quads)));
+#pragma unroll
+                for (int i = 0; i < V; ++i) y[i] = keep >> i & 1 ? y[i] * a.drop.scale : 0.f;
+            }
+            store_at<Z>(to, off + n * s.step, y, s);
+        }
+    }
+};
+
+// part [2 * NW][G][2]: mean and centred sum of squares of a window's piece of a large cloud.  MODE 0: the clouds, and the windows' partial
+// sums; MODE 1: the windows' rows
+template <typename Z, int MODE>
+__global__ __launch_bounds__(Z::THREADS, Z::NR > 8 ? 3 : 4) void k_fwd(Norm a, Geo g, const typename Z::T* X, typename Z::T* Y, float* mean_out, float* rstd_out,
+                                                                                  float* part, int* found) {
+    extern __shared__ __align__(16) float lds[];
+    if (MODE == 0) zero_rest(a, Y);
+    int unit, slab;
+    if (!place(g, unit, slab)) return;
+    const bool whole = MODE == 0 && unit < g.U;   // this unit's clouds, or a window's pieces
+    Piece p[2];
+    const int np = whole ? 0 : window_pieces<MODE == 0>(a, g, unit - (MODE == 0 ? g.U : 0), found, p);
+    if (!whole && np == 0) return;
+    Spot<Z> s;
+    locate(a, g, unit, slab, s);
+    Fwd<Z> f{a, g, s, X, Y, lds, drop_key(a.drop)};
+    float v[2][Z::NS], rstd[Z::NS];
+    for (int i = 0, b = s.unit;; ++i, b += g.U) {
+        if (MODE == 0) {
+            Range r;
+            if (whole) {
+                if (b >= a.B) break;
+                r = cloud_rows(a, b);
+                if (r.r1 - r.r0 > g.Tl) continue;
+                if (r.r1 == r.r0) {   // no statistics: zeros
+                    if (mean_out)
+                        for (int j = threadIdx.x; j < s.gs; j += Z::THREADS) {
+                            const int64_t at = (int64_t)b * a.G + s.slab * g.k + j;
+                            mean_out[at] = rstd_out[at] = 0.f;
+                        }
+                    continue;
+                }
+            } else {
+                if (i >= np) break;
+                r = i ? p[1].part : p[0].part;
+            }
+            if (whole && r.r1 - r.r0 <= Z::NR * g.RL) {
+                f.short_cloud(r, b, mean_out, rstd_out);
+                continue;
+            }
+            f.stats(r, v);
+            if (whole) {
+                f.finish(v, b, r.r1 - r.r0, true, mean_out, rstd_out, rstd);
+                f.apply(r, v[0], rstd);
+            } else {
+                put_part<2, Z>(part, i ? p[1].slot : p[0].slot, v, a, g, s);
+            }
+            continue;
+        }
+        if (i >= np) break;
+        const Piece q = i ? p[1] : p[0];
+        // the whole cloud's mean, then its centred sum of squares: a wave a group, lanes over pieces
+        const int n = piece_count(g, q.all), rows = q.all.r1 - q.all.r0;
+        float* out = lds + g.red + g.kb * g.CL * Z::NS;
+        __syncthreads();
+        for (int j = s.wave; j < s.gs; j += Z::WAVES) {
+            const float* from = part + (s.slab * g.k + j) * 2;
+            const float inv = 1.f / (float)rows;
+            float m = 0.f, m2 = 0.f;
+            for (int o = s.lane; o < n; o += 64) m = fmaf(from[(int64_t)piece_slot(g, q.all, o) * a.G * 2], (float)piece_rows(g, q.all, o) * inv, m);
+            m = wave_sum(m);
+            for (int o = s.lane; o < n; o += 64) {
+                const float* z = from + (int64_t)piece_slot(g, q.all, o) * a.G * 2;
+                const float d = z[0] - m;
+                m2 += fmaf(d * d, (float)piece_rows(g, q.all, o) * (float)a.Cg, z[1]);
+            }
+            m2 = wave_sum(m2);
+            if (s.lane == 0) out[j] = m, out[g.k + j] = m2;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int h = 0; h < Z::NS; ++h) v[0][h] = out[s.j[h]], v[1][h] = out[g.k + s.j[h]];
+        f.finish(v, q.b, rows, q.all.r0 == q.part.r0, mean_out, rstd_out, rstd);
+        f.apply(q.part, v[0], rstd);
+    }
+}
+
+// ---- launches (one translation unit per row type and pass) ----------------------------------------------------------------------
+// vectors a thread holds, in the variants for short and for long clouds: as many as leave four (two) waves a SIMD
+constexpr int FWD_NRS = 8, FWD_NRL = 16;
+
+struct Plan {
+    Geo g;
+    int V, fam, size;            // size: 0 few rows a thread, 1 many, 2 sixteen waves (slabs of more than 256 vectors)
+    bool al, uni;
+    unsigned blocks0, blocks1;   // workgroups of the first launch and of the windows' launches
+    size_t lds;
+};
+
+template <typename T>
+int launch_fwd(const Norm& a, const Plan& p, const void* X, void* Y, float* mean, float* rstd, float* part, int* found, hipStream_t st);
+
+}  // namespace gn

@@ -7,17 +7,17 @@
 //   X = -r (h m(P xh) + P m(h xh)) + q g + w ub
 //   d(x) = r (X - m(X) - xh (m(X xh) + r (m(P h) - m(P) m(h) - m(P xh) m(h xh)))),  d(w) = sum_rows (g v + ub xh),  d(b) = sum_rows ub
 // The simplest form: one workgroup per (cloud, group), one pass over the data per sum.
-#include "feature_math.h"
+#include "group_norm.h"
+
+#include <stdlib.h>
+
+#include <algorithm>
+#include <initializer_list>
 
 namespace {
 
-struct GN {
-    int64_t M;
-    int C, B, G, Cg, pdt, act;
-    const int* seg;
-    const void *W, *Bi;
-    float eps, slope;
-    Drop drop;
+struct GN : gn::Norm {
+    int act;
 };
 
 __device__ __forceinline__ float block_sum(float v, float* s_red) {
@@ -45,46 +45,19 @@ __device__ __forceinline__ float drop_factor(const GN& a, int64_t row, int c) {
 __device__ __forceinline__ float dropped(float d, float v) { return d == 0.f ? 0.f : d * v; }
 
 __device__ __forceinline__ void cloud_rows(const GN& a, int b, int64_t* r0, int64_t* r1) {
-    *r0 = min(max((int64_t)a.seg[b], (int64_t)0), a.M);
-    *r1 = min(max((int64_t)a.seg[b + 1], *r0), a.M);
+    *r0 = min(max(a.seg[b], 0), a.M);
+    *r1 = min(max(a.seg[b + 1], (int)*r0), a.M);
 }
 
 // rows of [0, M) that belong to no cloud are written as zeros
 template <typename T>
 __global__ __launch_bounds__(256) void k_zero_rest(GN a, T* Y, T* Y2) {
-    const int64_t lo = a.B ? min(max((int64_t)a.seg[0], (int64_t)0), a.M) : 0, hi = a.B ? min(max((int64_t)a.seg[a.B], lo), a.M) : 0;
+    const int64_t lo = a.B ? min(max(a.seg[0], 0), a.M) : 0, hi = a.B ? min(max(a.seg[a.B], (int)lo), a.M) : 0;
     const int64_t n0 = lo * a.C, n1 = (a.M - hi) * a.C;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n0 + n1; i += (int64_t)gridDim.x * 256) {
         const int64_t at = i < n0 ? i : hi * a.C + (i - n0);
         if (Y) Y[at] = narrow<T>(0.f);
         if (Y2) Y2[at] = narrow<T>(0.f);
-    }
-}
-
-template <typename T>
-__global__ __launch_bounds__(256) void k_fwd(GN a, const T* X, T* Y, float* mean_out, float* rstd_out) {
-    __shared__ float s_red[4];
-    const int b = blockIdx.x / a.G, j = blockIdx.x % a.G;
-    int64_t r0, r1;
-    cloud_rows(a, b, &r0, &r1);
-    const int64_t n = (r1 - r0) * a.Cg;
-    float s = 0.f;
-    for (int64_t i = threadIdx.x; i < n; i += 256) s += widen(X[(r0 + i / a.Cg) * a.C + j * a.Cg + i % a.Cg]);
-    const float mean = n ? block_sum(s, s_red) / (float)n : 0.f;
-    s = 0.f;
-    for (int64_t i = threadIdx.x; i < n; i += 256) {
-        const float d = widen(X[(r0 + i / a.Cg) * a.C + j * a.Cg + i % a.Cg]) - mean;
-        s += d * d;
-    }
-    const float rstd = n ? 1.f / sqrtf(block_sum(s, s_red) / (float)n + a.eps) : 0.f;
-    if (threadIdx.x == 0 && mean_out) mean_out[blockIdx.x] = mean, rstd_out[blockIdx.x] = rstd;
-    for (int64_t i = threadIdx.x; i < n; i += 256) {
-        const int64_t row = r0 + i / a.Cg;
-        const int c = j * a.Cg + (int)(i % a.Cg);
-        const float u = (a.W ? load_param(a.W, a.pdt, c) : 1.f) * ((widen(X[row * a.C + c]) - mean) * rstd) + (a.Bi ? load_param(a.Bi, a.pdt, c) : 0.f);
-        float d1, d2;
-        const float f = act_eval(a.act, u, a.slope, &d1, &d2);
-        Y[row * a.C + c] = narrow<T>(dropped(drop_factor(a, row, c), f));
     }
 }
 
@@ -251,19 +224,96 @@ inline int check(int dtype, int64_t M, int C, const int32_t* seg, int B, int G, 
     if (M >= (1ll << 31) || C > 4096 || (int64_t)B * G >= (1ll << 31)) return DD3D_ESIZE;
     if (dtype < DD3D_F32 || dtype > DD3D_BF16 || (pdt != DD3D_F32 && pdt != dtype) || act < DD3D_ACT_NONE || act > DD3D_ACT_GELU) return DD3D_EARG;
     if (slope != slope || (B > 0 && !seg) || !make_drop(p, key, &a->drop)) return DD3D_EARG;
-    a->M = M, a->C = C, a->B = B, a->G = G, a->Cg = C / G, a->pdt = pdt, a->act = act, a->seg = seg, a->W = W, a->Bi = Bi;
+    a->M = (int)M, a->C = C, a->B = B, a->G = G, a->Cg = C / G, a->pdt = pdt, a->act = act, a->seg = seg, a->W = W, a->Bi = Bi;
     a->slope = act == DD3D_ACT_NONE ? 1.f : act == DD3D_ACT_RELU ? 0.f : slope;
     a->eps = 0.f;
     return 0;
 }
 
+// ---- launch geometry --------------------------------------------------------------------------------------------------------------
+// windows of the whole batch: enough to fill the chip with the slabs of a row, never so many that joining them shows
+inline int max_windows(int C) { return C >= 1024 ? 64 : C <= 64 ? 1024 : 65536 / C; }
+constexpr int MIN_WINDOW = 512;
+
+inline int gcd(int a, int b) { return b ? gcd(b, a % b) : a; }
+
+inline gn::Div divide_by(int d) {
+    gn::Div r;
+    r.d = d, r.mul = d == 1 ? 0 : (uint32_t)((0x100000000ull + d - 1) / d);
+    return r;
+}
+
+// K: quantities summed at once; nrs / nrl: vectors a thread holds
+inline gn::Plan plan(const gn::Norm& a, int act, int esize, bool aligned, int K, int nrs, int nrl, bool params) {
+    gn::Plan p;
+    gn::Geo& g = p.g;
+    p.fam = act_family(act);
+    p.V = esize == 2 && aligned && a.Cg % 8 == 0 && a.Cg <= 2048 ? 8 : 4;
+    const int m0 = 4 / gcd(a.Cg, 4);   // groups whose channels fill whole vectors of four
+    p.al = aligned && a.C % p.V == 0 && m0 * a.Cg <= 4096;
+    p.uni = p.al && a.Cg % p.V == 0;
+    auto lanes = [&](int k) { return p.al || k >= a.G || k * a.Cg % 4 == 0 ? (k * a.Cg + p.V - 1) / p.V : (k * a.Cg + 6) / 4; };
+    auto whole = [&](int k) { return k >= a.G ? a.G : p.al ? std::min(a.G, (k + m0 - 1) / m0 * m0) : k; };
+    // Slab width: 64 bytes of a row at least (its neighbour reads the other half of the line into the same L2), doubled while a short
+    // cloud still fits one chunk and 1024 workgroups remain to fill the chip.  fp32 forward, 128 channels, us at 64 / 128 / 256 / 512
+    // bytes: 2560 clouds of 82 rows 106 / 65 / 52 / 58, 100 of 216 rows 13.7 / 15.3 / 19.8 / 28.7, 400 of 750 rows (long variant)
+    // 87 / 96 / 112 / 123.
+    const int kmin = whole((64 / esize + a.Cg - 1) / a.Cg);
+    const int64_t mean = a.B ? a.M / a.B : 0;
+    int k = kmin;
+    p.size = 0;
+    if (lanes(kmin) > 256) {
+        p.size = 2;
+    } else {
+        for (int w = whole(2 * k); k < a.G && lanes(w) <= 64 && (int64_t)nrs * (256 / lanes(w)) >= mean && (int64_t)a.B * ((a.G + w - 1) / w) >= 1024; w = whole(2 * k)) k = w;
+        if (p.uni && p.V == 4 && (int64_t)nrs * (256 / lanes(kmin)) < mean) p.size = 1;
+    }
+    if (getenv("GN_T")) p.size = p.uni && p.V == 4 ? atoi(getenv("GN_T")) : 0;
+    if (getenv("GN_W")) k = whole(std::max(1, atoi(getenv("GN_W")) / a.Cg));
+    const int threads = p.size == 2 ? 1024 : 256, nr = p.size == 1 ? nrl : nrs;
+    g.k = k;
+    g.nslab = (a.G + k - 1) / k;
+    g.CL = lanes(k);
+    g.RL = threads / g.CL;
+    g.lcl = -1;
+    for (int i = 0; i <= 6; ++i)
+        if (g.CL == 1 << i) g.lcl = i;
+    g.cw = p.uni ? a.Cg / p.V : a.Cg;
+    g.fast = p.uni && g.lcl >= 0 && (g.cw & (g.cw - 1)) == 0;
+    g.quads = (a.C + 3) / 4;
+    g.dCL = divide_by(g.CL), g.dCg = divide_by(a.Cg);
+    const int64_t cap = (int64_t)nr * g.RL;
+    g.NW = (int)std::min<int64_t>(ceil_div64(a.M, MIN_WINDOW), max_windows(a.C));
+    g.CH = g.NW ? (int)ceil_div64(a.M, g.NW) : 1;
+    g.Tl = (int)std::max<int64_t>(std::max<int64_t>(2 * cap, 1024), g.CH);
+    g.NW = a.M <= g.Tl ? 0 : (int)ceil_div64(a.M, g.CH);
+    g.U = a.B;
+    g.units = 0;
+    p.blocks0 = (unsigned)(align_up64((int64_t)g.U + g.NW, 8) * g.nslab);
+    p.blocks1 = (unsigned)(align_up64(g.NW, 8) * g.nslab);
+    // LDS: row partials of kb quantities (or two buffers of the waves' sums, or the columns of one parameter gradient), the columns' totals
+    // of kb quantities, the groups' sums of all
+    const int ns = p.uni ? 1 : p.V, cols = g.CL * ns;
+    g.kb = std::max(1, std::min(K, 8192 / (g.RL * cols)));
+    g.red = g.fast ? 2 * K * (threads / 64) * g.k : g.kb * g.RL * cols;
+    if (params) g.red = std::max(g.red, (g.lcl >= 0 ? threads / 64 : g.RL) * g.CL * p.V);
+    p.lds = sizeof(float) * ((size_t)g.red + g.kb * cols + K * g.k);
+    return p;
+}
+
+inline bool aligned16(std::initializer_list<const void*> ps) {
+    uintptr_t m = 0;
+    for (const void* p : ps) m |= (uintptr_t)p;
+    return (m & 15) == 0;
+}
+
 template <typename T>
-int fwd(const GN& a, const void* X, void* Y, float* mean, float* rstd, hipStream_t st) {
+int zero(const GN& a, void* Y, hipStream_t st) {
     if (a.M) k_zero_rest<T><<<rest_blocks(a.M, a.C), 256, 0, st>>>(a, (T*)Y, nullptr);
-    if (a.B) k_fwd<T><<<(unsigned)(a.B * a.G), 256, 0, st>>>(a, (const T*)X, (T*)Y, mean, rstd);
     DD3D_CHECK_LAUNCH();
     return 0;
 }
+
 template <typename T>
 int bwd(const GN& a, const void* dY, const void* X, const float* mean, const float* rstd, void* dX, void* dW, void* dB, hipStream_t st) {
     if (a.M && dX) {
@@ -292,6 +342,8 @@ int bwd2(const GN& a, const void* P, const void* q, const void* s, const void* d
 DD3D_API int64_t dd3d_group_norm_ws_bytes(int64_t M, int C, int B, int G, int order) {
     if (M < 0 || B < 0 || C <= 0 || G <= 0 || C % G != 0 || order < 0 || order > 2) return DD3D_EARG;
     if (M >= (1ll << 31) || C > 4096 || (int64_t)B * G >= (1ll << 31)) return DD3D_ESIZE;
+    const int64_t slots = 2 * (M > MIN_WINDOW ? std::min<int64_t>(ceil_div64(M, MIN_WINDOW), max_windows(C)) : 0);
+    if (order == 0) return slots * (G * 2 * (int64_t)sizeof(float) + (int64_t)sizeof(int));
     return order == 2 ? (int64_t)B * G * sizeof(Means) : 0;
 }
 
@@ -303,8 +355,14 @@ DD3D_API int dd3d_group_norm_fwd(const void* X, int dtype, int64_t M, int C, con
     if (rc) return rc;
     if (!(eps > 0.f) || (!mean != !rstd) || (M > 0 && (!X || !Y))) return DD3D_EARG;
     a.eps = eps;
+    if (M == 0 && B == 0) return 0;
     hipStream_t st = (hipStream_t)stream;
-    return dtype == DD3D_F32 ? fwd<float>(a, X, Y, mean, rstd, st) : dtype == DD3D_F16 ? fwd<half_t>(a, X, Y, mean, rstd, st) : fwd<bf16_t>(a, X, Y, mean, rstd, st);
+    if (ws_bytes < dd3d_group_norm_ws_bytes(M, C, B, G, 0) || (ws_bytes > 0 && !ws)) return DD3D_EWS;
+    if (B == 0) return dtype == DD3D_F32 ? zero<float>(a, Y, st) : zero<half_t>(a, Y, st);
+    const gn::Plan q = plan(a, act, dtype == DD3D_F32 ? 4 : 2, aligned16({X, Y}), 2, gn::FWD_NRS, gn::FWD_NRL, false);
+    return dtype == DD3D_F32   ? gn::launch_fwd<float>(a, q, X, Y, mean, rstd, (float*)ws, (int*)((float*)ws + 4ll * q.g.NW * G), st)
+           : dtype == DD3D_F16 ? gn::launch_fwd<half_t>(a, q, X, Y, mean, rstd, (float*)ws, (int*)((float*)ws + 4ll * q.g.NW * G), st)
+                               : gn::launch_fwd<bf16_t>(a, q, X, Y, mean, rstd, (float*)ws, (int*)((float*)ws + 4ll * q.g.NW * G), st);
 }
 
 DD3D_API int dd3d_group_norm_bwd(const void* dY, const void* X, int dtype, int64_t M, int C, const int32_t* seg_off, int B, int G, const void* weight,

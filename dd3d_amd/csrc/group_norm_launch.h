@@ -1,0 +1,64 @@
+// Picks the compiled variant a plan names and launches it (included by each group_norm_*.hip for one row type).
+#pragma once
+#include "group_norm.h"
+
+namespace gn {
+
+template <typename Z>
+struct Tag {
+    typedef Z type;
+};
+
+// NRS / NRL: vectors a thread holds in the variants for short and for long clouds
+template <typename T, int NRS, int NRL, int V, bool AL, bool UNI, int FAM, typename F>
+int with_size(const Plan& p, F f) {
+    if (p.size == 2) {
+        if constexpr (V == 4) return f(Tag<Cfg<T, V, AL, UNI, FAM, 1024, NRS>>());
+    }
+    if constexpr (UNI && V == 4) {
+        if (p.size == 1) return f(Tag<Cfg<T, V, AL, UNI, FAM, 256, NRL>>());
+    }
+    return f(Tag<Cfg<T, V, AL, UNI, FAM, 256, NRS>>());
+}
+template <typename T, int NRS, int NRL, int V, bool AL, bool UNI, typename F>
+int with_family(const Plan& p, F f) {
+    return p.fam == DD3D_FAM_LINEAR ? with_size<T, NRS, NRL, V, AL, UNI, DD3D_FAM_LINEAR>(p, f)
+           : p.fam == DD3D_FAM_SILU ? with_size<T, NRS, NRL, V, AL, UNI, DD3D_FAM_SILU>(p, f)
+                                    : with_size<T, NRS, NRL, V, AL, UNI, DD3D_FAM_GELU>(p, f);
+}
+template <typename T, int NRS, int NRL, typename F>
+int with_variant(const Plan& p, F f) {
+    if constexpr (sizeof(T) == 2) {
+        if (p.V == 8) return with_family<T, NRS, NRL, 8, true, true>(p, f);
+    }
+    if (!p.al) return with_family<T, NRS, NRL, 4, false, false>(p, f);
+    return p.uni ? with_family<T, NRS, NRL, 4, true, true>(p, f) : with_family<T, NRS, NRL, 4, true, false>(p, f);
+}
+
+template <typename K>
+int set_lds(K kernel, size_t lds) {
+    if (lds > 64 * 1024) DD3D_HIP(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+    return 0;
+}
+
+template <typename T>
+int launch_fwd(const Norm& a, const Plan& p, const void* X, void* Y, float* mean, float* rstd, float* part, int* found, hipStream_t st) {
+    return with_variant<T, FWD_NRS, FWD_NRL>(p, [&](auto tag) {
+        typedef typename decltype(tag)::type Z;
+        int rc = set_lds(k_fwd<Z, 0>, p.lds);
+        if (rc) return rc;
+        Geo g = p.g;
+        g.units = g.U + g.NW;
+        k_fwd<Z, 0><<<p.blocks0, Z::THREADS, p.lds, st>>>(a, g, (const T*)X, (T*)Y, mean, rstd, part, found);
+        if (g.NW) {
+            rc = set_lds(k_fwd<Z, 1>, p.lds);
+            if (rc) return rc;
+            g.units = g.NW;
+            k_fwd<Z, 1><<<p.blocks1, Z::THREADS, p.lds, st>>>(a, g, (const T*)X, (T*)Y, mean, rstd, part, found);
+        }
+        DD3D_CHECK_LAUNCH();
+        return 0;
+    });
+}
+
+}  // namespace gn

@@ -96,11 +96,17 @@ __device__ __forceinline__ void store_row(T* p, const float (&v)[V], int lo, int
 // ---- where this thread stands ---------------------------------------------------------------------------------------------------
 // The compile-time side of a launch.  UNI: every vector lies inside one group (Cg % V == 0), so a thread has one set of statistics;
 // otherwise its channels may belong to up to four groups.  AL: whole, aligned vectors.
+// Vectors a thread holds in the three passes, in the variants for short (first) and long clouds, and the waves per SIMD that the
+// registers of that many rows leave.
+constexpr int NR_FWD[2] = {8, 16}, NR_BWD[2] = {8, 16}, NR_BWD2[2] = {4, 8};
+
 template <typename T_, int V_, bool AL_, bool UNI_, int FAM_, int THREADS_, int NR_>
 struct Cfg {
     typedef T_ T;
     static constexpr int V = V_, FAM = FAM_, THREADS = THREADS_, NR = NR_, NS = UNI_ ? 1 : V_, WAVES = THREADS_ / 64;
     static constexpr bool AL = AL_, UNI = UNI_;
+    static constexpr int FWD_WAVES = THREADS_ > 256 || NR_ <= 8 ? 4 : 3, BWD_WAVES = THREADS_ > 256 ? 4 : NR_ > 8 ? 2 : V_ == 8 ? 3 : 4,
+                         BWD2_WAVES = THREADS_ > 256 ? 4 : NR_ > 4 || V_ == 8 ? 3 : 4;
     static constexpr int at(int i) { return UNI_ ? 0 : i; }
     typedef Raw<T_, V_> Row;
 };
@@ -268,7 +274,7 @@ __device__ __forceinline__ void group_sums(float (&v)[K][Z::NS], const Norm& a, 
 #pragma unroll
             for (int q = 0; q < K; ++q) v[q][0] += __shfl_xor(v[q][0], o, 64);
         }
-        float* red = lds + s.buf * K * Z::WAVES * g.k;
+        float* red = lds + s.buf * (g.red >> 1);   // (a fixed half: calls of different K follow each other)
         s.buf ^= 1;
         if (s.lane < g.CL && (s.lane & (g.cw - 1)) == 0 && s.hi > 0) {
 #pragma unroll
@@ -586,7 +592,7 @@ struct Fwd {
 // part [2 * NW][G][2]: mean and centred sum of squares of a window's piece of a large cloud.  MODE 0: the clouds, and the windows' partial
 // sums; MODE 1: the windows' rows
 template <typename Z, int MODE>
-__global__ __launch_bounds__(Z::THREADS, Z::NR > 8 ? 3 : 4) void k_fwd(Norm a, Geo g, const typename Z::T* X, typename Z::T* Y, float* mean_out, float* rstd_out,
+__global__ __launch_bounds__(Z::THREADS, Z::FWD_WAVES) void k_fwd(Norm a, Geo g, const typename Z::T* X, typename Z::T* Y, float* mean_out, float* rstd_out,
                                                                                   float* part, int* found) {
     extern __shared__ __align__(16) float lds[];
     if (MODE == 0) zero_rest(a, Y);
@@ -660,10 +666,486 @@ __global__ __launch_bounds__(Z::THREADS, Z::NR > 8 ? 3 : 4) void k_fwd(Norm a, G
     }
 }
 
-// ---- launches (one translation unit per row type and pass) ----------------------------------------------------------------------
-// vectors a thread holds, in the variants for short and for long clouds: as many as leave four (two) waves a SIMD
-constexpr int FWD_NRS = 8, FWD_NRL = 16;
+// ---- first gradient -------------------------------------------------------------------------------------------------------------
+// What a thread keeps of a row between the sums and the result: the normalised values and g (fp32 rows: in the registers the loaded rows
+// had), or the rows as loaded and the bits dropout kept (half-width rows: half the registers, the derivative is computed again).
+template <typename Z>
+struct Bwd {
+    typedef typename Z::T T;
+    static constexpr int V = Z::V, NR = Z::NR, NS = Z::NS;
+    static constexpr bool HOLD = sizeof(T) == 4;
+    const Norm& a;
+    const Geo& g;
+    Spot<Z>& s;
+    const T *dY, *X;
+    T* dX;
+    float* lds;
+    PhiloxKey key;
+    float mean[NS], rstd[NS], par[2][V];   // parameter gradients of this thread's channels: dw, db
 
+    struct Held {
+        typename Z::Row x[NR], d[NR];
+        float xh[HOLD ? NR : 1][V], gr[HOLD ? NR : 1][V];
+        uint32_t keep[HOLD ? 1 : (NR * V + 31) / 32];
+    };
+
+    __device__ __forceinline__ void load_stats(int b, const float* mean_in, const float* rstd_in) {
+        const int64_t at = (int64_t)b * a.G + s.slab * g.k;
+#pragma unroll
+        for (int i = 0; i < NS; ++i) mean[i] = mean_in[at + s.j[i]], rstd[i] = rstd_in[at + s.j[i]];
+    }
+
+    __device__ __forceinline__ void load(int base, int all, Held& h) {
+        load_chunk<Z>(X + row_at(a, base), a.C, all, g, s, h.x);
+        load_chunk<Z>(dY + row_at(a, base), a.C, all, g, s, h.d);
+    }
+
+    // xh and g of one row
+    __device__ __forceinline__ void element(const typename Z::Row& x, const typename Z::Row& d, uint32_t keep, float (&xh)[V], float (&gr)[V]) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            float d1, d2;
+            xh[i] = (raw_get(x, i) - mean[Z::at(i)]) * rstd[Z::at(i)];
+            activate<Z::FAM, 1>(fmaf(xh[i], s.w[i], s.b[i]), a.slope, &d1, &d2);
+            float dy = raw_get(d, i);
+            if (a.drop.key) dy = keep >> i & 1 ? dy * a.drop.scale : 0.f;
+            gr[i] = dy * d1;
+        }
+    }
+
+    // the chunk's part of v = sums of h and h xh per group, and of the parameter gradients
+    __device__ __forceinline__ void add_rows(int base, int all, Held& h, float (&v)[2][NS]) {
+        const int left = s.on ? all : 0;
+        const uint64_t words = words_at(g, base);
+        const uint32_t word = here(s.word);
+#pragma unroll
+        for (int i = 0; i < (HOLD ? 1 : (NR * V + 31) / 32); ++i) h.keep[i] = 0;
+#pragma unroll
+        for (int n = 0; n < NR; ++n) {
+            row_border();
+            if (s.rl + n * g.RL >= left) continue;
+            uint32_t keep = 0;
+            if (a.drop.key) {
+                keep = keep_bits<V>(a.drop, key, words + (word + n * (uint32_t)(g.RL * g.quads)));
+                if (!HOLD) h.keep[n * V / 32] |= keep << (n * V % 32);
+            }
+            float xh[V], gr[V];
+            element(h.x[n], h.d[n], keep, xh, gr);
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const float t = gr[i] * s.w[i];
+                v[0][Z::at(i)] += t;
+                v[1][Z::at(i)] = fmaf(t, xh[i], v[1][Z::at(i)]);
+                par[0][i] = fmaf(gr[i], xh[i], par[0][i]);
+                par[1][i] += gr[i];
+                if (HOLD) h.xh[n][i] = xh[i], h.gr[n][i] = gr[i];
+            }
+        }
+    }
+
+    __device__ __forceinline__ void rows_out(int base, int all, const Held& h, bool fresh, const float (&m1)[NS], const float (&m2)[NS]) {
+        const int left = s.on ? all : 0;
+        T* to = dX + row_at(a, base);
+        const uint64_t words = words_at(g, base);
+        const uint32_t off = here(s.off), word = here(s.word);
+#pragma unroll
+        for (int n = 0; n < NR; ++n) {
+            row_border();
+            if (s.rl + n * g.RL >= left) continue;
+            float xh[V], gr[V], dx[V];
+            if (HOLD && !fresh) {
+#pragma unroll
+                for (int i = 0; i < V; ++i) xh[i] = h.xh[n][i], gr[i] = h.gr[n][i];
+            } else {
+                uint32_t keep = 0;
+                if (a.drop.key) {
+                    if (fresh) keep = keep_bits<V>(a.drop, key, words + (word + n * (uint32_t)(g.RL * g.quads)));
+                    else keep = h.keep[HOLD ? 0 : n * V / 32] >> (n * V % 32);
+                }
+                element(h.x[n], h.d[n], keep, xh, gr);
+            }
+#pragma unroll
+            for (int i = 0; i < V; ++i) dx[i] = rstd[Z::at(i)] * fmaf(gr[i], s.w[i], -fmaf(xh[i], m2[Z::at(i)], m1[Z::at(i)]));
+            store_at<Z>(to, off + n * s.step, dx, s);
+        }
+    }
+
+    __device__ __forceinline__ void means(float (&v)[2][NS], int rows) {
+        const float inv = 1.f / ((float)rows * (float)a.Cg);
+#pragma unroll
+        for (int i = 0; i < NS; ++i) v[0][i] *= inv, v[1][i] *= inv;
+    }
+
+    __device__ __forceinline__ void short_cloud(const Range& r) {
+        const int rows = r.r1 - r.r0;
+        Held h;
+        float v[2][NS];
+#pragma unroll
+        for (int i = 0; i < NS; ++i) v[0][i] = v[1][i] = 0.f;
+        load(r.r0, rows, h);
+        add_rows(r.r0, rows, h, v);
+        if (!dX) return;
+        group_sums<2, Z>(v, a, g, s, lds);
+        means(v, rows);
+        rows_out(r.r0, rows, h, false, v[0], v[1]);
+    }
+
+    __device__ __forceinline__ void sums(const Range& r, float (&v)[2][NS]) {
+#pragma unroll
+        for (int i = 0; i < NS; ++i) v[0][i] = v[1][i] = 0.f;
+        for (int base = r.r0; base < r.r1; base += NR * g.RL) {
+            Held h;
+            load(base, r.r1 - base, h);
+            add_rows(base, r.r1 - base, h, v);
+        }
+        group_sums<2, Z>(v, a, g, s, lds);
+    }
+
+    __device__ __forceinline__ void apply(const Range& r, const float (&m1)[NS], const float (&m2)[NS]) {
+        for (int base = r.r0; base < r.r1; base += NR * g.RL) {
+            Held h;
+            load(base, r.r1 - base, h);
+            rows_out(base, r.r1 - base, h, true, m1, m2);
+        }
+    }
+};
+
+// part [2 * NW][G][2]: sums of h and h xh over a piece; slots [U + NW][2][C]: parameter gradients of a unit (NULL: not asked for)
+template <typename Z, int MODE>
+__global__ __launch_bounds__(Z::THREADS, Z::BWD_WAVES) void k_bwd(Norm a, Geo g, const typename Z::T* dY, const typename Z::T* X, const float* mean_in,
+                                                                 const float* rstd_in, typename Z::T* dX, float* part, int* found, float* slots) {
+    extern __shared__ __align__(16) float lds[];
+    if (MODE == 0) zero_rest(a, dX);
+    int unit, slab;
+    if (!place(g, unit, slab)) return;
+    const bool whole = MODE == 0 && unit < g.U;
+    Piece p[2];
+    const int np = whole ? 0 : window_pieces<MODE == 0>(a, g, unit - (MODE == 0 ? g.U : 0), found, p);
+    if (!whole && np == 0) return;
+    Spot<Z> s;
+    locate(a, g, unit, slab, s);
+    Bwd<Z> f{a, g, s, dY, X, dX, lds, drop_key(a.drop)};
+#pragma unroll
+    for (int i = 0; i < Z::V; ++i) f.par[0][i] = f.par[1][i] = 0.f;
+    float v[2][Z::NS];
+    for (int i = 0, b = unit;; ++i, b += g.U) {
+        if (MODE == 0) {
+            Range r;
+            if (whole) {
+                if (b >= a.B) break;
+                r = cloud_rows(a, b);
+                if (r.r1 - r.r0 > g.Tl || r.r1 == r.r0) continue;
+            } else {
+                if (i >= np) break;
+                r = i ? p[1].part : p[0].part;
+            }
+            f.load_stats(whole ? b : i ? p[1].b : p[0].b, mean_in, rstd_in);
+            if (whole && r.r1 - r.r0 <= Z::NR * g.RL) {
+                f.short_cloud(r);
+                continue;
+            }
+            f.sums(r, v);
+            if (!whole) {
+                put_part<2, Z>(part, i ? p[1].slot : p[0].slot, v, a, g, s);
+            } else if (dX) {
+                f.means(v, r.r1 - r.r0);
+                f.apply(r, v[0], v[1]);
+            }
+            continue;
+        }
+        if (i >= np) break;
+        const Piece q = i ? p[1] : p[0];
+        f.load_stats(q.b, mean_in, rstd_in);
+        join_parts<2, Z>(part, q.all, v, a, g, s, lds);
+        f.means(v, q.all.r1 - q.all.r0);
+        f.apply(q.part, v[0], v[1]);
+    }
+    if (MODE == 0 && slots) column_sums<2, Z>(f.par, a, g, s, lds, slots + (int64_t)unit * 2 * a.C);
+}
+
+// ---- second gradient ------------------------------------------------------------------------------------------------------------
+// The three matrices stay as loaded; the activation's derivatives are computed again in every pass over them.
+template <typename Z>
+struct Bwd2 {
+    typedef typename Z::T T;
+    static constexpr int V = Z::V, NR = Z::NR, NS = Z::NS, KW = (NR * V + 31) / 32;
+    const Norm& a;
+    const Geo& g;
+    Spot<Z>& s;
+    const T *P, *dY, *X;
+    T *ddY, *ddX;
+    float* lds;
+    PhiloxKey key;
+    float q[V], t[V];                      // cotangents of dw and db
+    float mean[NS], rstd[NS], par[2][V];   // d(w), d(b)
+
+    struct Held {
+        typename Z::Row x[NR], d[NR], p[NR];
+        uint32_t keep[KW];
+    };
+    // means over the cloud of h, h xh, P, P xh, P h, q g, q g xh
+    enum { H, HX, MP, PX, PH, QG, QX, KS };
+
+    __device__ __forceinline__ void load_stats(int b, const float* mean_in, const float* rstd_in) {
+        const int64_t at = (int64_t)b * a.G + s.slab * g.k;
+#pragma unroll
+        for (int i = 0; i < NS; ++i) mean[i] = mean_in[at + s.j[i]], rstd[i] = rstd_in[at + s.j[i]];
+    }
+
+    __device__ __forceinline__ void load(int base, int all, Held& h) {
+        load_chunk<Z>(X + row_at(a, base), a.C, all, g, s, h.x);
+        load_chunk<Z>(dY + row_at(a, base), a.C, all, g, s, h.d);
+        if (P) load_chunk<Z>(P + row_at(a, base), a.C, all, g, s, h.p);
+#pragma unroll
+        for (int i = 0; i < KW; ++i) h.keep[i] = 0;
+        if (!a.drop.key) return;
+        const uint64_t words = words_at(g, base);
+        const uint32_t word = here(s.word);
+#pragma unroll
+        for (int n = 0; n < NR; ++n) {
+            row_border();
+            if (n * g.RL < all) h.keep[n * V / 32] |= keep_bits<V>(a.drop, key, words + (word + n * (uint32_t)(g.RL * g.quads))) << (n * V % 32);
+        }
+    }
+
+    struct Elem {
+        float xh, p, dy, D, d1, d2;   // dy: after dropout
+    };
+    template <int ORDER>
+    __device__ __forceinline__ Elem element(const Held& h, int n, int i) {
+        Elem e;
+        e.xh = (raw_get(h.x[n], i) - mean[Z::at(i)]) * rstd[Z::at(i)];
+        e.p = P ? raw_get(h.p[n], i) : 0.f;
+        e.D = 1.f;
+        e.dy = raw_get(h.d[n], i);
+        if (a.drop.key) {
+            const bool kept = h.keep[n * V / 32] >> (n * V % 32 + i) & 1;
+            e.D = kept ? a.drop.scale : 0.f;
+            e.dy = kept ? e.dy * a.drop.scale : 0.f;
+        }
+        activate<Z::FAM, ORDER>(fmaf(e.xh, s.w[i], s.b[i]), a.slope, &e.d1, &e.d2);
+        return e;
+    }
+
+    __device__ __forceinline__ void add_rows(int all, const Held& h, float (&v)[KS][NS]) {
+        const int left = s.on ? all : 0;
+#pragma unroll
+        for (int n = 0; n < NR; ++n) {
+            row_border();
+            if (s.rl + n * g.RL >= left) continue;
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const int c = Z::at(i);
+                const Elem e = element<1>(h, n, i);
+                const float gr = e.dy * e.d1, hh = gr * s.w[i], qg = gr * q[i];
+                v[H][c] += hh;
+                v[HX][c] = fmaf(hh, e.xh, v[HX][c]);
+                v[MP][c] += e.p;
+                v[PX][c] = fmaf(e.p, e.xh, v[PX][c]);
+                v[PH][c] = fmaf(e.p, hh, v[PH][c]);
+                v[QG][c] += qg;
+                v[QX][c] = fmaf(qg, e.xh, v[QX][c]);
+            }
+        }
+    }
+
+    // cotangent of g
+    __device__ __forceinline__ float gbar(const Elem& e, const float (&m)[KS][NS], int i, float& vv) {
+        const int c = Z::at(i);
+        vv = rstd[c] * (e.p - fmaf(e.xh, m[PX][c], m[MP][c]));
+        return fmaf(s.w[i], vv, fmaf(q[i], e.xh, t[i]));
+    }
+
+    // sums of w ub and w ub xh
+    __device__ __forceinline__ void add_rows2(int all, const Held& h, const float (&m)[KS][NS], float (&v)[2][NS]) {
+        const int left = s.on ? all : 0;
+#pragma unroll
+        for (int n = 0; n < NR; ++n) {
+            row_border();
+            if (s.rl + n * g.RL >= left) continue;
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const Elem e = element<2>(h, n, i);
+                float vv;
+                const float wub = gbar(e, m, i, vv) * e.dy * e.d2 * s.w[i];
+                v[0][Z::at(i)] += wub;
+                v[1][Z::at(i)] = fmaf(wub, e.xh, v[1][Z::at(i)]);
+            }
+        }
+    }
+
+    __device__ __forceinline__ void rows_out(int base, int all, const Held& h, const float (&m)[KS][NS], const float (&u)[2][NS]) {
+        const int left = s.on ? all : 0;
+        T *to_y = ddY + row_at(a, base), *to_x = ddX + row_at(a, base);
+        const uint32_t off = here(s.off);
+#pragma unroll
+        for (int n = 0; n < NR; ++n) {
+            row_border();
+            if (s.rl + n * g.RL >= left) continue;
+            float oy[V], ox[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const int c = Z::at(i);
+                const Elem e = element<2>(h, n, i);
+                float vv;
+                const float gb = gbar(e, m, i, vv), gr = e.dy * e.d1, hh = gr * s.w[i], ub = Z::FAM == DD3D_FAM_LINEAR ? 0.f : gb * e.dy * e.d2;
+                const float X = fmaf(q[i], gr, s.w[i] * ub) - rstd[c] * fmaf(hh, m[PX][c], e.p * m[HX][c]);
+                oy[i] = e.D == 0.f ? 0.f : gb * e.d1 * e.D;
+                ox[i] = rstd[c] * (X - fmaf(e.xh, u[1][c], u[0][c]));
+                par[0][i] += fmaf(gr, vv, ub * e.xh);
+                par[1][i] += ub;
+            }
+            if (ddY) store_at<Z>(to_y, off + n * s.step, oy, s);
+            if (ddX) store_at<Z>(to_x, off + n * s.step, ox, s);
+        }
+    }
+
+    __device__ __forceinline__ void means(float (&m)[KS][NS], int rows) {
+        const float inv = 1.f / ((float)rows * (float)a.Cg);
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+#pragma unroll
+            for (int i = 0; i < NS; ++i) m[k][i] *= inv;
+    }
+    // sums of w ub and w ub xh -> the mean of X, and what multiplies xh
+    __device__ __forceinline__ void finish(const float (&m)[KS][NS], float (&u)[2][NS], int rows) {
+        const float inv = 1.f / ((float)rows * (float)a.Cg);
+#pragma unroll
+        for (int i = 0; i < NS; ++i) {
+            u[0][i] = fmaf(u[0][i], inv, m[QG][i]) - rstd[i] * fmaf(m[PX][i], m[H][i], m[HX][i] * m[MP][i]);
+            u[1][i] = fmaf(u[1][i], inv, m[QX][i]) + rstd[i] * (m[PH][i] - m[MP][i] * m[H][i] - 3.f * (m[PX][i] * m[HX][i]));
+        }
+    }
+
+    __device__ __forceinline__ void clear(float (&u)[2][NS]) {
+#pragma unroll
+        for (int i = 0; i < NS; ++i) u[0][i] = u[1][i] = 0.f;
+    }
+    __device__ __forceinline__ void clear(float (&m)[KS][NS]) {
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+#pragma unroll
+            for (int i = 0; i < NS; ++i) m[k][i] = 0.f;
+    }
+
+    __device__ __forceinline__ void short_cloud(const Range& r) {
+        const int rows = r.r1 - r.r0;
+        Held h;
+        float m[KS][NS], u[2][NS];
+        clear(m), clear(u);
+        load(r.r0, rows, h);
+        add_rows(rows, h, m);
+        group_sums<KS, Z>(m, a, g, s, lds);
+        means(m, rows);
+        if (Z::FAM != DD3D_FAM_LINEAR) {
+            add_rows2(rows, h, m, u);
+            group_sums<2, Z>(u, a, g, s, lds);
+        }
+        finish(m, u, rows);
+        rows_out(r.r0, rows, h, m, u);
+    }
+    __device__ __forceinline__ void sums(const Range& r, float (&m)[KS][NS]) {
+        clear(m);
+        for (int base = r.r0; base < r.r1; base += NR * g.RL) {
+            Held h;
+            load(base, r.r1 - base, h);
+            add_rows(r.r1 - base, h, m);
+        }
+        group_sums<KS, Z>(m, a, g, s, lds);
+    }
+    __device__ __forceinline__ void sums2(const Range& r, const float (&m)[KS][NS], float (&u)[2][NS]) {
+        clear(u);
+        if (Z::FAM == DD3D_FAM_LINEAR) return;
+        for (int base = r.r0; base < r.r1; base += NR * g.RL) {
+            Held h;
+            load(base, r.r1 - base, h);
+            add_rows2(r.r1 - base, h, m, u);
+        }
+        group_sums<2, Z>(u, a, g, s, lds);
+    }
+    __device__ __forceinline__ void apply(const Range& r, const float (&m)[KS][NS], const float (&u)[2][NS]) {
+        for (int base = r.r0; base < r.r1; base += NR * g.RL) {
+            Held h;
+            load(base, r.r1 - base, h);
+            rows_out(base, r.r1 - base, h, m, u);
+        }
+    }
+};
+
+// part1 [2 * NW][G][7], part2 [2 * NW][G][2]: a piece's sums of the first and second pass.  MODE 0: the clouds, and the windows' first
+// sums; MODE 1: the windows' second sums; MODE 2: the windows' rows
+template <typename Z, int MODE>
+__global__ __launch_bounds__(Z::THREADS, Z::BWD2_WAVES) void k_bwd2(Norm a, Geo g, const typename Z::T* P, const void* ggw, const void* ggb, const typename Z::T* dY,
+                                                                   const typename Z::T* X, const float* mean_in, const float* rstd_in, typename Z::T* ddY,
+                                                                   typename Z::T* ddX, float* part1, float* part2, int* found, float* slots) {
+    extern __shared__ __align__(16) float lds[];
+    if (MODE == 0) {
+        zero_rest(a, ddY);
+        zero_rest(a, ddX);
+    }
+    int unit, slab;
+    if (!place(g, unit, slab)) return;
+    const bool whole = MODE == 0 && unit < g.U;
+    Piece p[2];
+    const int np = whole ? 0 : window_pieces<MODE == 0>(a, g, unit - (MODE == 0 ? g.U : 0), found, p);
+    if (!whole && np == 0) return;
+    Spot<Z> s;
+    locate(a, g, unit, slab, s);
+    typedef Bwd2<Z> F;
+    F f{a, g, s, P, dY, X, ddY, ddX, lds, drop_key(a.drop)};
+    load_params<Z::V>(ggw, a.pdt, s.c0, s.on ? s.lo : Z::V, s.hi, 0.f, f.q);
+    load_params<Z::V>(ggb, a.pdt, s.c0, s.on ? s.lo : Z::V, s.hi, 0.f, f.t);
+#pragma unroll
+    for (int i = 0; i < Z::V; ++i) f.par[0][i] = f.par[1][i] = 0.f;
+    float m[F::KS][Z::NS], u[2][Z::NS];
+    for (int i = 0, b = unit;; ++i, b += g.U) {
+        if (MODE == 0) {
+            Range r;
+            if (whole) {
+                if (b >= a.B) break;
+                r = cloud_rows(a, b);
+                if (r.r1 - r.r0 > g.Tl || r.r1 == r.r0) continue;
+            } else {
+                if (i >= np) break;
+                r = i ? p[1].part : p[0].part;
+            }
+            f.load_stats(whole ? b : i ? p[1].b : p[0].b, mean_in, rstd_in);
+            if (whole && r.r1 - r.r0 <= Z::NR * g.RL) {
+                f.short_cloud(r);
+                continue;
+            }
+            f.sums(r, m);
+            if (!whole) {
+                put_part<F::KS, Z>(part1, i ? p[1].slot : p[0].slot, m, a, g, s);
+                continue;
+            }
+            f.means(m, r.r1 - r.r0);
+            f.sums2(r, m, u);
+            f.finish(m, u, r.r1 - r.r0);
+            f.apply(r, m, u);
+            continue;
+        }
+        if (i >= np) break;
+        const Piece q = i ? p[1] : p[0];
+        const int rows = q.all.r1 - q.all.r0;
+        f.load_stats(q.b, mean_in, rstd_in);
+        join_parts<F::KS, Z>(part1, q.all, m, a, g, s, lds);
+        f.means(m, rows);
+        if (MODE == 1) {
+            f.sums2(q.part, m, u);
+            put_part<2, Z>(part2, q.slot, u, a, g, s);
+            continue;
+        }
+        f.clear(u);
+        if (Z::FAM != DD3D_FAM_LINEAR) join_parts<2, Z>(part2, q.all, u, a, g, s, lds);
+        f.finish(m, u, rows);
+        f.apply(q.part, m, u);
+    }
+    // a window's parameter gradients belong to its rows' last pass
+    if (slots && (MODE == 2 || whole)) column_sums<2, Z>(f.par, a, g, s, lds, slots + (int64_t)(MODE == 2 ? g.U + unit : unit) * 2 * a.C);
+}
+
+// ---- launches (one translation unit per row type and pass) ----------------------------------------------------------------------
 struct Plan {
     Geo g;
     int V, fam, size;            // size: 0 few rows a thread, 1 many, 2 sixteen waves (slabs of more than 256 vectors)
@@ -672,7 +1154,17 @@ struct Plan {
     size_t lds;
 };
 
+struct Work {   // the caller's workspace
+    float *part1, *part2, *slots, *folded;
+    int* found;
+};
+
 template <typename T>
-int launch_fwd(const Norm& a, const Plan& p, const void* X, void* Y, float* mean, float* rstd, float* part, int* found, hipStream_t st);
+int launch_fwd(const Norm& a, const Plan& p, const void* X, void* Y, float* mean, float* rstd, const Work& w, hipStream_t st);
+template <typename T>
+int launch_bwd(const Norm& a, const Plan& p, const void* dY, const void* X, const float* mean, const float* rstd, void* dX, const Work& w, hipStream_t st);
+template <typename T>
+int launch_bwd2(const Norm& a, const Plan& p, const void* P, const void* ggw, const void* ggb, const void* dY, const void* X, const float* mean, const float* rstd,
+                void* ddY, void* ddX, const Work& w, hipStream_t st);
 
 }  // namespace gn

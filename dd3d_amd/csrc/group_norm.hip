@@ -6,7 +6,8 @@
 //   v = r (P - m(P) - xh m(P xh)),  gb = w v + q xh + s,  d(dy) = gb D phi',  ub = gb dy D phi''
 //   X = -r (h m(P xh) + P m(h xh)) + q g + w ub
 //   d(x) = r (X - m(X) - xh (m(X xh) + r (m(P h) - m(P) m(h) - m(P xh) m(h xh)))),  d(w) = sum_rows (g v + ub xh),  d(b) = sum_rows ub
-// The simplest form: one workgroup per (cloud, group), one pass over the data per sum.
+// m(X) and m(X xh) follow from the first pass's means and those of w ub and w ub xh, which take a second pass over the rows (none where
+// phi is piecewise linear and ub = 0).  The kernels: group_norm.h.  Here: argument checks, launch geometry, parameter gradients.
 #include "group_norm.h"
 
 #include <stdlib.h>
@@ -16,224 +17,57 @@
 
 namespace {
 
-struct GN : gn::Norm {
-    int act;
-};
+// rows of [0, M) that belong to no cloud: all of them when there is no cloud
+__global__ __launch_bounds__(256) void k_zero(uint32_t* y, int64_t words) {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < words; i += (int64_t)gridDim.x * 256) y[i] = 0;
+}
+__global__ void k_zero_half(uint16_t* y, int64_t n) {
+    if (threadIdx.x == 0 && n > 0) y[n - 1] = 0;   // the odd last element of a half-width matrix
+}
 
-__device__ __forceinline__ float block_sum(float v, float* s_red) {
-    v = wave_sum(v);
+// ---- parameter gradients: out[q][c] = sum over the units' slots [slot][2][C], slots in a fixed order ------------------------------
+// One column a thread, four row lanes a workgroup, `parts` workgroups a column block; they write their sums to `folded` for a second
+// launch of the same kernel, or with parts = 1 the result.
+__global__ __launch_bounds__(256) void k_fold(const float* slots, int n, int U, const int* found, int cols, int parts, float* folded, void* dw, void* db, int C,
+                                              int pdt) {
+    __shared__ float s_red[256];
+    const int c = blockIdx.x * 64 + (threadIdx.x & 63), part = blockIdx.y, lane = threadIdx.x >> 6;
+    float t = 0.f;
+    if (c < cols)
+#pragma unroll 8
+        for (int i = part + lane * parts; i < n; i += 4 * parts)
+            if (i < U || found[i - U]) t += slots[(int64_t)i * cols + c];   // (a window without a large cloud has written nothing)
+    s_red[threadIdx.x] = t;
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) s_red[threadIdx.x >> 6] = v;
-    __syncthreads();
-    return s_red[0] + s_red[1] + s_red[2] + s_red[3];
+    if (lane || c >= cols) return;
+    t = s_red[threadIdx.x] + s_red[threadIdx.x + 64] + s_red[threadIdx.x + 128] + s_red[threadIdx.x + 192];
+    if (parts > 1) {
+        folded[(int64_t)part * cols + c] = t;
+        return;
+    }
+    void* to = c < C ? dw : db;
+    if (to) store_param(to, pdt, c < C ? c : c - C, t);
 }
 
-__device__ __forceinline__ float act_eval(int act, float u, float slope, float* d1, float* d2) {
-    switch (act_family(act)) {
-        case DD3D_FAM_LINEAR: return activate<DD3D_FAM_LINEAR, 2>(u, slope, d1, d2);
-        case DD3D_FAM_SILU: return activate<DD3D_FAM_SILU, 2>(u, slope, d1, d2);
-        default: return activate<DD3D_FAM_GELU, 2>(u, slope, d1, d2);
+constexpr int FOLD = 32;
+
+inline int fold(const gn::Norm& a, const gn::Geo& g, const gn::Work& w, void* dw, void* db, hipStream_t st) {
+    const int n = g.U + g.NW, cols = 2 * a.C;
+    const unsigned blocks = (unsigned)ceil_div64(cols, 64);
+    if (n <= 128) {
+        k_fold<<<blocks, 256, 0, st>>>(w.slots, n, g.U, w.found, cols, 1, nullptr, dw, db, a.C, a.pdt);
+    } else {
+        k_fold<<<dim3(blocks, FOLD), 256, 0, st>>>(w.slots, n, g.U, w.found, cols, FOLD, w.folded, nullptr, nullptr, a.C, a.pdt);
+        k_fold<<<blocks, 256, 0, st>>>(w.folded, FOLD, FOLD, nullptr, cols, 1, nullptr, dw, db, a.C, a.pdt);
     }
-}
-
-__device__ __forceinline__ float drop_factor(const GN& a, int64_t row, int c) {
-    if (!a.drop.key) return 1.f;
-    const uint4 w = philox_block(philox_key(a.drop.key), (uint64_t)row * (uint64_t)((a.C + 3) / 4) + (uint64_t)(c / 4));
-    const uint32_t r = (c & 3) == 0 ? w.x : (c & 3) == 1 ? w.y : (c & 3) == 2 ? w.z : w.w;
-    return !a.drop.all && r >= a.drop.thr ? a.drop.scale : 0.f;
-}
-__device__ __forceinline__ float dropped(float d, float v) { return d == 0.f ? 0.f : d * v; }
-
-__device__ __forceinline__ void cloud_rows(const GN& a, int b, int64_t* r0, int64_t* r1) {
-    *r0 = min(max(a.seg[b], 0), a.M);
-    *r1 = min(max(a.seg[b + 1], (int)*r0), a.M);
-}
-
-// rows of [0, M) that belong to no cloud are written as zeros
-template <typename T>
-__global__ __launch_bounds__(256) void k_zero_rest(GN a, T* Y, T* Y2) {
-    const int64_t lo = a.B ? min(max(a.seg[0], 0), a.M) : 0, hi = a.B ? min(max(a.seg[a.B], (int)lo), a.M) : 0;
-    const int64_t n0 = lo * a.C, n1 = (a.M - hi) * a.C;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n0 + n1; i += (int64_t)gridDim.x * 256) {
-        const int64_t at = i < n0 ? i : hi * a.C + (i - n0);
-        if (Y) Y[at] = narrow<T>(0.f);
-        if (Y2) Y2[at] = narrow<T>(0.f);
-    }
-}
-
-// what the gradients need of one element
-struct Elem {
-    float xh, w, dyd, g, h, d1, d2, D;
-};
-template <typename T>
-__device__ __forceinline__ Elem element(const GN& a, const T* dY, const T* X, int64_t row, int c, float mean, float rstd) {
-    Elem e;
-    e.w = a.W ? load_param(a.W, a.pdt, c) : 1.f;
-    e.xh = (widen(X[row * a.C + c]) - mean) * rstd;
-    act_eval(a.act, e.w * e.xh + (a.Bi ? load_param(a.Bi, a.pdt, c) : 0.f), a.slope, &e.d1, &e.d2);
-    e.D = drop_factor(a, row, c);
-    e.dyd = dropped(e.D, widen(dY[row * a.C + c]));
-    e.g = e.dyd * e.d1;
-    e.h = e.g * e.w;
-    return e;
-}
-
-template <typename T>
-__global__ __launch_bounds__(256) void k_bwd_x(GN a, const T* dY, const T* X, const float* mean_in, const float* rstd_in, T* dX) {
-    __shared__ float s_red[4];
-    const int b = blockIdx.x / a.G, j = blockIdx.x % a.G;
-    int64_t r0, r1;
-    cloud_rows(a, b, &r0, &r1);
-    const int64_t n = (r1 - r0) * a.Cg;
-    if (n == 0) return;
-    const float mean = mean_in[blockIdx.x], rstd = rstd_in[blockIdx.x];
-    float s1 = 0.f, s2 = 0.f;
-    for (int64_t i = threadIdx.x; i < n; i += 256) {
-        const Elem e = element(a, dY, X, r0 + i / a.Cg, j * a.Cg + (int)(i % a.Cg), mean, rstd);
-        s1 += e.h;
-        s2 += e.h * e.xh;
-    }
-    const float m1 = block_sum(s1, s_red) / (float)n, m2 = block_sum(s2, s_red) / (float)n;
-    for (int64_t i = threadIdx.x; i < n; i += 256) {
-        const int64_t row = r0 + i / a.Cg;
-        const int c = j * a.Cg + (int)(i % a.Cg);
-        const Elem e = element(a, dY, X, row, c, mean, rstd);
-        dX[row * a.C + c] = narrow<T>(rstd * (e.h - m1 - e.xh * m2));
-    }
-}
-
-// one workgroup per channel
-template <typename T>
-__global__ __launch_bounds__(256) void k_bwd_p(GN a, const T* dY, const T* X, const float* mean_in, const float* rstd_in, void* dW, void* dB) {
-    __shared__ float s_red[4];
-    const int c = blockIdx.x;
-    float sw = 0.f, sb = 0.f;
-    for (int b = 0; b < a.B; ++b) {
-        int64_t r0, r1;
-        cloud_rows(a, b, &r0, &r1);
-        for (int64_t row = r0 + threadIdx.x; row < r1; row += 256) {
-            const Elem e = element(a, dY, X, row, c, mean_in[(int64_t)b * a.G + c / a.Cg], rstd_in[(int64_t)b * a.G + c / a.Cg]);
-            sw += e.g * e.xh;
-            sb += e.g;
-        }
-    }
-    sw = block_sum(sw, s_red);
-    sb = block_sum(sb, s_red);
-    if (threadIdx.x == 0) {
-        if (dW) store_param(dW, a.pdt, c, sw);
-        if (dB) store_param(dB, a.pdt, c, sb);
-    }
-}
-
-template <typename T>
-struct Second {
-    const T* P;
-    const void *q, *s;
-};
-
-struct Means {
-    float mp, mp2, mph, m1, m2;
-};
-
-struct Elem2 {
-    Elem e;
-    float P, q, v, gb, ub, X;
-};
-template <typename T>
-__device__ __forceinline__ Elem2 element2(const GN& a, const Second<T>& z, const T* dY, const T* X, int64_t row, int c, float mean, float rstd, const Means& m) {
-    Elem2 o;
-    o.e = element(a, dY, X, row, c, mean, rstd);
-    o.P = z.P ? widen(z.P[row * a.C + c]) : 0.f;
-    o.q = z.q ? load_param(z.q, a.pdt, c) : 0.f;
-    o.v = rstd * (o.P - m.mp - o.e.xh * m.mp2);
-    o.gb = o.e.w * o.v + o.q * o.e.xh + (z.s ? load_param(z.s, a.pdt, c) : 0.f);
-    o.ub = o.gb * o.e.dyd * o.e.d2;
-    o.X = -rstd * (o.e.h * m.mp2 + o.P * m.m2) + o.q * o.e.g + o.e.w * o.ub;
-    return o;
-}
-
-// writes d(dy), d(x) and the five means of the (cloud, group) for the parameter kernel behind it
-template <typename T>
-__global__ __launch_bounds__(256) void k_bwd2_x(GN a, Second<T> z, const T* dY, const T* X, const float* mean_in, const float* rstd_in, T* ddY, T* ddX,
-                                                Means* means) {
-    __shared__ float s_red[4];
-    const int b = blockIdx.x / a.G, j = blockIdx.x % a.G;
-    int64_t r0, r1;
-    cloud_rows(a, b, &r0, &r1);
-    const int64_t n = (r1 - r0) * a.Cg;
-    if (n == 0) return;
-    const float mean = mean_in[blockIdx.x], rstd = rstd_in[blockIdx.x], inv = 1.f / (float)n;
-    Means m = {0.f, 0.f, 0.f, 0.f, 0.f};
-    for (int64_t i = threadIdx.x; i < n; i += 256) {
-        const int64_t row = r0 + i / a.Cg;
-        const int c = j * a.Cg + (int)(i % a.Cg);
-        const Elem e = element(a, dY, X, row, c, mean, rstd);
-        const float P = z.P ? widen(z.P[row * a.C + c]) : 0.f;
-        m.mp += P, m.mp2 += P * e.xh, m.mph += P * e.h, m.m1 += e.h, m.m2 += e.h * e.xh;
-    }
-    m.mp = block_sum(m.mp, s_red) * inv, m.mp2 = block_sum(m.mp2, s_red) * inv, m.mph = block_sum(m.mph, s_red) * inv;
-    m.m1 = block_sum(m.m1, s_red) * inv, m.m2 = block_sum(m.m2, s_red) * inv;
-    if (threadIdx.x == 0) means[blockIdx.x] = m;
-    float t1 = 0.f, t2 = 0.f;
-    for (int64_t i = threadIdx.x; i < n; i += 256) {
-        const Elem2 o = element2(a, z, dY, X, r0 + i / a.Cg, j * a.Cg + (int)(i % a.Cg), mean, rstd, m);
-        t1 += o.X;
-        t2 += o.X * o.e.xh;
-    }
-    t1 = block_sum(t1, s_red) * inv;
-    t2 = block_sum(t2, s_red) * inv + rstd * (m.mph - m.mp * m.m1 - m.mp2 * m.m2);
-    for (int64_t i = threadIdx.x; i < n; i += 256) {
-        const int64_t row = r0 + i / a.Cg;
-        const int c = j * a.Cg + (int)(i % a.Cg);
-        const Elem2 o = element2(a, z, dY, X, row, c, mean, rstd, m);
-        if (ddY) ddY[row * a.C + c] = narrow<T>(dropped(o.e.D, o.gb * o.e.d1));
-        if (ddX) ddX[row * a.C + c] = narrow<T>(rstd * (o.X - t1 - o.e.xh * t2));
-    }
-}
-
-template <typename T>
-__global__ __launch_bounds__(256) void k_bwd2_p(GN a, Second<T> z, const T* dY, const T* X, const float* mean_in, const float* rstd_in, const Means* means,
-                                                void* dW, void* dB) {
-    __shared__ float s_red[4];
-    const int c = blockIdx.x;
-    float sw = 0.f, sb = 0.f;
-    for (int b = 0; b < a.B; ++b) {
-        int64_t r0, r1;
-        cloud_rows(a, b, &r0, &r1);
-        const int64_t at = (int64_t)b * a.G + c / a.Cg;
-        for (int64_t row = r0 + threadIdx.x; row < r1; row += 256) {
-            const Elem2 o = element2(a, z, dY, X, row, c, mean_in[at], rstd_in[at], means[at]);
-            sw += o.e.g * o.v + o.ub * o.e.xh;
-            sb += o.ub;
-        }
-    }
-    sw = block_sum(sw, s_red);
-    sb = block_sum(sb, s_red);
-    if (threadIdx.x == 0) {
-        if (dW) store_param(dW, a.pdt, c, sw);
-        if (dB) store_param(dB, a.pdt, c, sb);
-    }
-}
-
-inline int rest_blocks(int64_t M, int C) { return (int)(ceil_div64(M * C, 256) < 1024 ? ceil_div64(M * C, 256) : 1024); }
-
-// argument checks shared by the three entry points; 0 = fill in `a` and go on
-inline int check(int dtype, int64_t M, int C, const int32_t* seg, int B, int G, const void* W, const void* Bi, int pdt, int act, float slope, double p,
-                 const int64_t* key, GN* a) {
-    if (M < 0 || B < 0 || C <= 0 || G <= 0 || C % G != 0) return DD3D_EARG;
-    if (M >= (1ll << 31) || C > 4096 || (int64_t)B * G >= (1ll << 31)) return DD3D_ESIZE;
-    if (dtype < DD3D_F32 || dtype > DD3D_BF16 || (pdt != DD3D_F32 && pdt != dtype) || act < DD3D_ACT_NONE || act > DD3D_ACT_GELU) return DD3D_EARG;
-    if (slope != slope || (B > 0 && !seg) || !make_drop(p, key, &a->drop)) return DD3D_EARG;
-    a->M = (int)M, a->C = C, a->B = B, a->G = G, a->Cg = C / G, a->pdt = pdt, a->act = act, a->seg = seg, a->W = W, a->Bi = Bi;
-    a->slope = act == DD3D_ACT_NONE ? 1.f : act == DD3D_ACT_RELU ? 0.f : slope;
-    a->eps = 0.f;
+    DD3D_CHECK_LAUNCH();
     return 0;
 }
 
 // ---- launch geometry --------------------------------------------------------------------------------------------------------------
 // windows of the whole batch: enough to fill the chip with the slabs of a row, never so many that joining them shows
 inline int max_windows(int C) { return C >= 1024 ? 64 : C <= 64 ? 1024 : 65536 / C; }
-constexpr int MIN_WINDOW = 512;
+constexpr int MIN_WINDOW = 512, MAX_UNITS = 2048;
 
 inline int gcd(int a, int b) { return b ? gcd(b, a % b) : a; }
 
@@ -243,8 +77,12 @@ inline gn::Div divide_by(int d) {
     return r;
 }
 
-// K: quantities summed at once; nrs / nrl: vectors a thread holds
-inline gn::Plan plan(const gn::Norm& a, int act, int esize, bool aligned, int K, int nrs, int nrl, bool params) {
+// workgroups that take whole clouds: one a cloud, or (where each leaves its part of the parameter gradients) as few as deal the clouds
+// out evenly and stay below MAX_UNITS
+inline int cloud_units(int B, bool params) { return params && B > MAX_UNITS ? (int)ceil_div64(B, ceil_div64(B, MAX_UNITS)) : B; }
+
+// sums: quantities summed at once; nr: vectors a thread holds in the variants for short and long clouds; params: column_sums is called
+inline gn::Plan plan(const gn::Norm& a, int act, int esize, bool aligned, int sums, const int (&nr)[2], bool params) {
     gn::Plan p;
     gn::Geo& g = p.g;
     p.fam = act_family(act);
@@ -265,12 +103,12 @@ inline gn::Plan plan(const gn::Norm& a, int act, int esize, bool aligned, int K,
     if (lanes(kmin) > 256) {
         p.size = 2;
     } else {
-        for (int w = whole(2 * k); k < a.G && lanes(w) <= 64 && (int64_t)nrs * (256 / lanes(w)) >= mean && (int64_t)a.B * ((a.G + w - 1) / w) >= 1024; w = whole(2 * k)) k = w;
-        if (p.uni && p.V == 4 && (int64_t)nrs * (256 / lanes(kmin)) < mean) p.size = 1;
+        for (int w = whole(2 * k); k < a.G && lanes(w) <= 64 && (int64_t)nr[0] * (256 / lanes(w)) >= mean && (int64_t)a.B * ((a.G + w - 1) / w) >= 1024; w = whole(2 * k)) k = w;
+        if (p.uni && p.V == 4 && (int64_t)nr[0] * (256 / lanes(kmin)) < mean) p.size = 1;
     }
     if (getenv("GN_T")) p.size = p.uni && p.V == 4 ? atoi(getenv("GN_T")) : 0;
     if (getenv("GN_W")) k = whole(std::max(1, atoi(getenv("GN_W")) / a.Cg));
-    const int threads = p.size == 2 ? 1024 : 256, nr = p.size == 1 ? nrl : nrs;
+    const int threads = p.size == 2 ? 1024 : 256;
     g.k = k;
     g.nslab = (a.G + k - 1) / k;
     g.CL = lanes(k);
@@ -282,23 +120,53 @@ inline gn::Plan plan(const gn::Norm& a, int act, int esize, bool aligned, int K,
     g.fast = p.uni && g.lcl >= 0 && (g.cw & (g.cw - 1)) == 0;
     g.quads = (a.C + 3) / 4;
     g.dCL = divide_by(g.CL), g.dCg = divide_by(a.Cg);
-    const int64_t cap = (int64_t)nr * g.RL;
+    const int64_t cap = (int64_t)nr[p.size == 1] * g.RL;
     g.NW = (int)std::min<int64_t>(ceil_div64(a.M, MIN_WINDOW), max_windows(a.C));
     g.CH = g.NW ? (int)ceil_div64(a.M, g.NW) : 1;
-    g.Tl = (int)std::max<int64_t>(std::max<int64_t>(2 * cap, 1024), g.CH);
+    g.Tl = (int)std::max<int64_t>(2 * cap, g.CH);
     g.NW = a.M <= g.Tl ? 0 : (int)ceil_div64(a.M, g.CH);
-    g.U = a.B;
+    g.U = cloud_units(a.B, params);
     g.units = 0;
     p.blocks0 = (unsigned)(align_up64((int64_t)g.U + g.NW, 8) * g.nslab);
     p.blocks1 = (unsigned)(align_up64(g.NW, 8) * g.nslab);
     // LDS: row partials of kb quantities (or two buffers of the waves' sums, or the columns of one parameter gradient), the columns' totals
     // of kb quantities, the groups' sums of all
     const int ns = p.uni ? 1 : p.V, cols = g.CL * ns;
-    g.kb = std::max(1, std::min(K, 8192 / (g.RL * cols)));
-    g.red = g.fast ? 2 * K * (threads / 64) * g.k : g.kb * g.RL * cols;
+    g.kb = std::max(1, std::min(sums, 8192 / (g.RL * cols)));
+    g.red = g.fast ? 2 * sums * (threads / 64) * g.k : g.kb * g.RL * cols;
     if (params) g.red = std::max(g.red, (g.lcl >= 0 ? threads / 64 : g.RL) * g.CL * p.V);
-    p.lds = sizeof(float) * ((size_t)g.red + g.kb * cols + K * g.k);
+    p.lds = sizeof(float) * ((size_t)g.red + g.kb * cols + sums * g.k);
     return p;
+}
+
+// The workspace: piece sums, units' slots and their folded sums, pieces per window.  Sized by bounds that hold for every type and alignment.
+struct Layout {
+    int64_t part1, part2, slots, folded, found, bytes;
+};
+inline Layout layout(int64_t M, int C, int B, int G, int order) {
+    const int64_t windows = M > MIN_WINDOW ? std::min<int64_t>(ceil_div64(M, MIN_WINDOW), max_windows(C)) : 0;
+    const int64_t units = order ? cloud_units(B, true) + windows : 0, pieces = 2 * windows * G;
+    Layout l;
+    int64_t at = 0;
+    auto take = [&](int64_t floats) {
+        const int64_t here = at;
+        at = align_up64(at + floats * 4, 256);
+        return here;
+    };
+    l.part1 = take(pieces * (order == 2 ? 7 : 2));
+    l.part2 = take(order == 2 ? pieces * 2 : 0);
+    l.slots = take(units * 2 * C);
+    l.folded = take(order && units > 128 ? (int64_t)FOLD * 2 * C : 0);
+    l.found = take(windows);
+    l.bytes = at;
+    return l;
+}
+inline gn::Work work_at(void* ws, const Layout& l, bool params) {
+    char* p = (char*)ws;
+    gn::Work w;
+    w.part1 = (float*)(p + l.part1), w.part2 = (float*)(p + l.part2), w.slots = params ? (float*)(p + l.slots) : nullptr;
+    w.folded = (float*)(p + l.folded), w.found = (int*)(p + l.found);
+    return w;
 }
 
 inline bool aligned16(std::initializer_list<const void*> ps) {
@@ -307,34 +175,33 @@ inline bool aligned16(std::initializer_list<const void*> ps) {
     return (m & 15) == 0;
 }
 
-template <typename T>
-int zero(const GN& a, void* Y, hipStream_t st) {
-    if (a.M) k_zero_rest<T><<<rest_blocks(a.M, a.C), 256, 0, st>>>(a, (T*)Y, nullptr);
-    DD3D_CHECK_LAUNCH();
+// argument checks shared by the three entry points; 0 = fill in `a` and go on
+inline int check(int dtype, int64_t M, int C, const int32_t* seg, int B, int G, const void* W, const void* Bi, int pdt, int act, float slope, double p,
+                 const int64_t* key, gn::Norm* a) {
+    if (M < 0 || B < 0 || C <= 0 || G <= 0 || C % G != 0) return DD3D_EARG;
+    if (M >= (1ll << 31) || C > 4096 || (int64_t)B * G >= (1ll << 31)) return DD3D_ESIZE;
+    if (dtype < DD3D_F32 || dtype > DD3D_BF16 || (pdt != DD3D_F32 && pdt != dtype) || act < DD3D_ACT_NONE || act > DD3D_ACT_GELU) return DD3D_EARG;
+    if (slope != slope || (B > 0 && !seg) || !make_drop(p, key, &a->drop)) return DD3D_EARG;
+    a->M = (int)M, a->C = C, a->B = B, a->G = G, a->Cg = C / G, a->pdt = pdt, a->seg = seg, a->W = W, a->Bi = Bi;
+    a->slope = act == DD3D_ACT_NONE ? 1.f : act == DD3D_ACT_RELU ? 0.f : slope;
+    a->eps = 0.f;
     return 0;
 }
 
-template <typename T>
-int bwd(const GN& a, const void* dY, const void* X, const float* mean, const float* rstd, void* dX, void* dW, void* dB, hipStream_t st) {
-    if (a.M && dX) {
-        k_zero_rest<T><<<rest_blocks(a.M, a.C), 256, 0, st>>>(a, (T*)dX, nullptr);
-        if (a.B) k_bwd_x<T><<<(unsigned)(a.B * a.G), 256, 0, st>>>(a, (const T*)dY, (const T*)X, mean, rstd, (T*)dX);
-    }
-    if (dW || dB) k_bwd_p<T><<<a.C, 256, 0, st>>>(a, (const T*)dY, (const T*)X, mean, rstd, dW, dB);
+inline int zero(void* y, const gn::Norm& a, int esize, hipStream_t st) {
+    const int64_t n = (int64_t)a.M * a.C, words = n * esize / 4;
+    if (!y || n == 0) return 0;
+    if (words) k_zero<<<(unsigned)std::min<int64_t>(ceil_div64(words, 256), 2048), 256, 0, st>>>((uint32_t*)y, words);
+    if (n * esize % 4) k_zero_half<<<1, 64, 0, st>>>((uint16_t*)y, n);
     DD3D_CHECK_LAUNCH();
     return 0;
 }
-template <typename T>
-int bwd2(const GN& a, const void* P, const void* q, const void* s, const void* dY, const void* X, const float* mean, const float* rstd, void* ddY, void* ddX,
-         void* dW, void* dB, void* ws, hipStream_t st) {
-    const Second<T> z = {(const T*)P, q, s};
-    if (a.M && (ddY || ddX)) k_zero_rest<T><<<rest_blocks(a.M, a.C), 256, 0, st>>>(a, (T*)ddY, (T*)ddX);
-    if (a.B)
-        k_bwd2_x<T><<<(unsigned)(a.B * a.G), 256, 0, st>>>(a, z, (const T*)dY, (const T*)X, mean, rstd, (T*)ddY, (T*)ddX, (Means*)ws);
-    if (dW || dB) k_bwd2_p<T><<<a.C, 256, 0, st>>>(a, z, (const T*)dY, (const T*)X, mean, rstd, (const Means*)ws, dW, dB);
+inline int zero_params(const gn::Norm& a, void* dw, void* db, hipStream_t st) {
+    if (dw || db) k_fold<<<(unsigned)ceil_div64(2 * a.C, 64), 256, 0, st>>>(nullptr, 0, 0, nullptr, 2 * a.C, 1, nullptr, dw, db, a.C, a.pdt);
     DD3D_CHECK_LAUNCH();
     return 0;
 }
+inline int esize_of(int dtype) { return dtype == DD3D_F32 ? 4 : 2; }
 
 }  // namespace
 
@@ -342,53 +209,74 @@ int bwd2(const GN& a, const void* P, const void* q, const void* s, const void* d
 DD3D_API int64_t dd3d_group_norm_ws_bytes(int64_t M, int C, int B, int G, int order) {
     if (M < 0 || B < 0 || C <= 0 || G <= 0 || C % G != 0 || order < 0 || order > 2) return DD3D_EARG;
     if (M >= (1ll << 31) || C > 4096 || (int64_t)B * G >= (1ll << 31)) return DD3D_ESIZE;
-    const int64_t slots = 2 * (M > MIN_WINDOW ? std::min<int64_t>(ceil_div64(M, MIN_WINDOW), max_windows(C)) : 0);
-    if (order == 0) return slots * (G * 2 * (int64_t)sizeof(float) + (int64_t)sizeof(int));
-    return order == 2 ? (int64_t)B * G * sizeof(Means) : 0;
+    return layout(M, C, B, G, order).bytes;
 }
 
 DD3D_API int dd3d_group_norm_fwd(const void* X, int dtype, int64_t M, int C, const int32_t* seg_off, int B, int G, const void* weight, const void* bias,
                                  int pdtype, float eps, int act, float slope, double p, const int64_t* key, void* Y, float* mean, float* rstd, void* ws,
                                  int64_t ws_bytes, void* stream) {
-    GN a;
+    gn::Norm a;
     const int rc = check(dtype, M, C, seg_off, B, G, weight, bias, pdtype, act, slope, p, key, &a);
     if (rc) return rc;
     if (!(eps > 0.f) || (!mean != !rstd) || (M > 0 && (!X || !Y))) return DD3D_EARG;
     a.eps = eps;
-    if (M == 0 && B == 0) return 0;
+    const Layout l = layout(M, C, B, G, 0);
+    if (ws_bytes < l.bytes || (l.bytes > 0 && !ws)) return DD3D_EWS;
     hipStream_t st = (hipStream_t)stream;
-    if (ws_bytes < dd3d_group_norm_ws_bytes(M, C, B, G, 0) || (ws_bytes > 0 && !ws)) return DD3D_EWS;
-    if (B == 0) return dtype == DD3D_F32 ? zero<float>(a, Y, st) : zero<half_t>(a, Y, st);
-    const gn::Plan q = plan(a, act, dtype == DD3D_F32 ? 4 : 2, aligned16({X, Y}), 2, gn::FWD_NRS, gn::FWD_NRL, false);
-    return dtype == DD3D_F32   ? gn::launch_fwd<float>(a, q, X, Y, mean, rstd, (float*)ws, (int*)((float*)ws + 4ll * q.g.NW * G), st)
-           : dtype == DD3D_F16 ? gn::launch_fwd<half_t>(a, q, X, Y, mean, rstd, (float*)ws, (int*)((float*)ws + 4ll * q.g.NW * G), st)
-                               : gn::launch_fwd<bf16_t>(a, q, X, Y, mean, rstd, (float*)ws, (int*)((float*)ws + 4ll * q.g.NW * G), st);
+    if (B == 0) return zero(Y, a, esize_of(dtype), st);
+    const gn::Plan q = plan(a, act, esize_of(dtype), aligned16({X, Y}), 2, gn::NR_FWD, false);
+    const gn::Work w = work_at(ws, l, false);
+    return dtype == DD3D_F32   ? gn::launch_fwd<float>(a, q, X, Y, mean, rstd, w, st)
+           : dtype == DD3D_F16 ? gn::launch_fwd<half_t>(a, q, X, Y, mean, rstd, w, st)
+                               : gn::launch_fwd<bf16_t>(a, q, X, Y, mean, rstd, w, st);
 }
 
 DD3D_API int dd3d_group_norm_bwd(const void* dY, const void* X, int dtype, int64_t M, int C, const int32_t* seg_off, int B, int G, const void* weight,
                                  const void* bias, int pdtype, int act, float slope, double p, const int64_t* key, const float* mean, const float* rstd,
                                  void* dX, void* dweight, void* dbias, void* ws, int64_t ws_bytes, void* stream) {
-    GN a;
-    const int rc = check(dtype, M, C, seg_off, B, G, weight, bias, pdtype, act, slope, p, key, &a);
+    gn::Norm a;
+    int rc = check(dtype, M, C, seg_off, B, G, weight, bias, pdtype, act, slope, p, key, &a);
     if (rc) return rc;
     if ((M > 0 && (!X || !dY)) || (B > 0 && (!mean || !rstd))) return DD3D_EARG;
+    const Layout l = layout(M, C, B, G, 1);
+    if (ws_bytes < l.bytes || (l.bytes > 0 && !ws)) return DD3D_EWS;
     hipStream_t st = (hipStream_t)stream;
-    return dtype == DD3D_F32   ? bwd<float>(a, dY, X, mean, rstd, dX, dweight, dbias, st)
-           : dtype == DD3D_F16 ? bwd<half_t>(a, dY, X, mean, rstd, dX, dweight, dbias, st)
-                               : bwd<bf16_t>(a, dY, X, mean, rstd, dX, dweight, dbias, st);
+    if (B == 0) {
+        rc = zero(dX, a, esize_of(dtype), st);
+        return rc ? rc : zero_params(a, dweight, dbias, st);
+    }
+    const bool params = dweight || dbias;
+    if (!params && !dX) return 0;
+    const gn::Plan q = plan(a, act, esize_of(dtype), aligned16({X, dY, dX}), 2, gn::NR_BWD, params);
+    const gn::Work w = work_at(ws, l, params);
+    rc = dtype == DD3D_F32   ? gn::launch_bwd<float>(a, q, dY, X, mean, rstd, dX, w, st)
+         : dtype == DD3D_F16 ? gn::launch_bwd<half_t>(a, q, dY, X, mean, rstd, dX, w, st)
+                             : gn::launch_bwd<bf16_t>(a, q, dY, X, mean, rstd, dX, w, st);
+    return rc || !params ? rc : fold(a, q.g, w, dweight, dbias, st);
 }
 
 DD3D_API int dd3d_group_norm_bwd2(const void* ggX, const void* ggW, const void* ggB, const void* dY, const void* X, int dtype, int64_t M, int C,
                                   const int32_t* seg_off, int B, int G, const void* weight, const void* bias, int pdtype, int act, float slope, double p,
                                   const int64_t* key, const float* mean, const float* rstd, void* ddY, void* ddX, void* ddweight, void* ddbias, void* ws,
                                   int64_t ws_bytes, void* stream) {
-    GN a;
-    const int rc = check(dtype, M, C, seg_off, B, G, weight, bias, pdtype, act, slope, p, key, &a);
+    gn::Norm a;
+    int rc = check(dtype, M, C, seg_off, B, G, weight, bias, pdtype, act, slope, p, key, &a);
     if (rc) return rc;
     if ((M > 0 && (!X || !dY)) || (B > 0 && (!mean || !rstd))) return DD3D_EARG;
-    if (ws_bytes < dd3d_group_norm_ws_bytes(M, C, B, G, 2) || (B > 0 && !ws)) return DD3D_EWS;
+    const Layout l = layout(M, C, B, G, 2);
+    if (ws_bytes < l.bytes || (l.bytes > 0 && !ws)) return DD3D_EWS;
     hipStream_t st = (hipStream_t)stream;
-    return dtype == DD3D_F32   ? bwd2<float>(a, ggX, ggW, ggB, dY, X, mean, rstd, ddY, ddX, ddweight, ddbias, ws, st)
-           : dtype == DD3D_F16 ? bwd2<half_t>(a, ggX, ggW, ggB, dY, X, mean, rstd, ddY, ddX, ddweight, ddbias, ws, st)
-                               : bwd2<bf16_t>(a, ggX, ggW, ggB, dY, X, mean, rstd, ddY, ddX, ddweight, ddbias, ws, st);
+    if (B == 0) {
+        rc = zero(ddY, a, esize_of(dtype), st);
+        if (!rc) rc = zero(ddX, a, esize_of(dtype), st);
+        return rc ? rc : zero_params(a, ddweight, ddbias, st);
+    }
+    const bool params = ddweight || ddbias;
+    if (!params && !ddY && !ddX) return 0;
+    const gn::Plan q = plan(a, act, esize_of(dtype), aligned16({X, dY, ggX, ddY, ddX}), 7, gn::NR_BWD2, params);
+    const gn::Work w = work_at(ws, l, params);
+    rc = dtype == DD3D_F32   ? gn::launch_bwd2<float>(a, q, ggX, ggW, ggB, dY, X, mean, rstd, ddY, ddX, w, st)
+         : dtype == DD3D_F16 ? gn::launch_bwd2<half_t>(a, q, ggX, ggW, ggB, dY, X, mean, rstd, ddY, ddX, w, st)
+                             : gn::launch_bwd2<bf16_t>(a, q, ggX, ggW, ggB, dY, X, mean, rstd, ddY, ddX, w, st);
+    return rc || !params ? rc : fold(a, q.g, w, ddweight, ddbias, st);
 }

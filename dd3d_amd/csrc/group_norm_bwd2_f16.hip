@@ -1,0 +1,6 @@
+// The group norm's second gradient for fp16 rows (group_norm.h).
+#include "group_norm_launch.h"
+
+namespace gn {
+template int launch_bwd2<half_t>(const Norm&, const Plan&, const void*, const void*, const void*, const void*, const void*, const float*, const float*, void*, void*, const Work&, hipStream_t);
+}  // namespace gn

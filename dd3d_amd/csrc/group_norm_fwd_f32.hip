@@ -1,0 +1,6 @@
+// The group norm's forward pass for fp32 rows (group_norm.h).
+#include "group_norm_launch.h"
+
+namespace gn {
+template int launch_fwd<float>(const Norm&, const Plan&, const void*, void*, float*, float*, const Work&, hipStream_t);
+}  // namespace gn

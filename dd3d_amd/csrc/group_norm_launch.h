@@ -42,19 +42,66 @@ int set_lds(K kernel, size_t lds) {
 }
 
 template <typename T>
-int launch_fwd(const Norm& a, const Plan& p, const void* X, void* Y, float* mean, float* rstd, float* part, int* found, hipStream_t st) {
-    return with_variant<T, FWD_NRS, FWD_NRL>(p, [&](auto tag) {
+int launch_fwd(const Norm& a, const Plan& p, const void* X, void* Y, float* mean, float* rstd, const Work& w, hipStream_t st) {
+    return with_variant<T, NR_FWD[0], NR_FWD[1]>(p, [&](auto tag) {
         typedef typename decltype(tag)::type Z;
         int rc = set_lds(k_fwd<Z, 0>, p.lds);
         if (rc) return rc;
         Geo g = p.g;
         g.units = g.U + g.NW;
-        k_fwd<Z, 0><<<p.blocks0, Z::THREADS, p.lds, st>>>(a, g, (const T*)X, (T*)Y, mean, rstd, part, found);
+        k_fwd<Z, 0><<<p.blocks0, Z::THREADS, p.lds, st>>>(a, g, (const T*)X, (T*)Y, mean, rstd, w.part1, w.found);
         if (g.NW) {
             rc = set_lds(k_fwd<Z, 1>, p.lds);
             if (rc) return rc;
             g.units = g.NW;
-            k_fwd<Z, 1><<<p.blocks1, Z::THREADS, p.lds, st>>>(a, g, (const T*)X, (T*)Y, mean, rstd, part, found);
+            k_fwd<Z, 1><<<p.blocks1, Z::THREADS, p.lds, st>>>(a, g, (const T*)X, (T*)Y, mean, rstd, w.part1, w.found);
+        }
+        DD3D_CHECK_LAUNCH();
+        return 0;
+    });
+}
+
+template <typename T>
+int launch_bwd(const Norm& a, const Plan& p, const void* dY, const void* X, const float* mean, const float* rstd, void* dX, const Work& w, hipStream_t st) {
+    return with_variant<T, NR_BWD[0], NR_BWD[1]>(p, [&](auto tag) {
+        typedef typename decltype(tag)::type Z;
+        int rc = set_lds(k_bwd<Z, 0>, p.lds);
+        if (rc) return rc;
+        Geo g = p.g;
+        g.units = g.U + g.NW;
+        k_bwd<Z, 0><<<p.blocks0, Z::THREADS, p.lds, st>>>(a, g, (const T*)dY, (const T*)X, mean, rstd, (T*)dX, w.part1, w.found, w.slots);
+        if (g.NW && dX) {
+            rc = set_lds(k_bwd<Z, 1>, p.lds);
+            if (rc) return rc;
+            g.units = g.NW;
+            k_bwd<Z, 1><<<p.blocks1, Z::THREADS, p.lds, st>>>(a, g, (const T*)dY, (const T*)X, mean, rstd, (T*)dX, w.part1, w.found, w.slots);
+        }
+        DD3D_CHECK_LAUNCH();
+        return 0;
+    });
+}
+
+template <typename T>
+int launch_bwd2(const Norm& a, const Plan& p, const void* P, const void* ggw, const void* ggb, const void* dY, const void* X, const float* mean, const float* rstd,
+                void* ddY, void* ddX, const Work& w, hipStream_t st) {
+    return with_variant<T, NR_BWD2[0], NR_BWD2[1]>(p, [&](auto tag) {
+        typedef typename decltype(tag)::type Z;
+        Geo g = p.g;
+        auto go = [&](auto* kernel, unsigned blocks) {
+            const int rc = set_lds(kernel, p.lds);
+            if (rc) return rc;
+            kernel<<<blocks, Z::THREADS, p.lds, st>>>(a, g, (const T*)P, ggw, ggb, (const T*)dY, (const T*)X, mean, rstd, (T*)ddY, (T*)ddX, w.part1, w.part2, w.found,
+                                                      w.slots);
+            return 0;
+        };
+        g.units = g.U + g.NW;
+        int rc = go(k_bwd2<Z, 0>, p.blocks0);
+        if (rc) return rc;
+        if (g.NW) {
+            g.units = g.NW;
+            if (Z::FAM != DD3D_FAM_LINEAR) rc = go(k_bwd2<Z, 1>, p.blocks1);
+            if (!rc) rc = go(k_bwd2<Z, 2>, p.blocks1);
+            if (rc) return rc;
         }
         DD3D_CHECK_LAUNCH();
         return 0;

@@ -37,6 +37,12 @@ __device__ __forceinline__ bf16_t narrow<bf16_t>(float v) {
     return r;
 }
 
+__device__ __forceinline__ float widen_bits(uint16_t h, int dt) {
+    half_t f;
+    __builtin_memcpy(&f, &h, 2);
+    return dt == DD3D_F16 ? (float)f : __uint_as_float((uint32_t)h << 16);
+}
+
 // parameter vectors (weight, bias and their gradients) are fp32 or of the rows' type: a code, uniform over the launch
 __device__ __forceinline__ float load_param(const void* p, int pdt, int64_t i) {
     if (pdt == DD3D_F32) return ((const float*)p)[i];

@@ -44,6 +44,7 @@ struct Geo {
     int quads;           // ceil(C / 4)
     int kb;              // quantities reduced at once where the sums go through LDS
     int red;             // floats of LDS for them
+    int tickets;         // column blocks of the parameter gradients
     Div dCL, dCg;
 };
 
@@ -63,6 +64,19 @@ __device__ __forceinline__ float raw_get(const Raw<half_t, V>& r, int i) {
 template <int V>
 __device__ __forceinline__ float raw_get(const Raw<bf16_t, V>& r, int i) {
     return __uint_as_float((i & 1) ? r.u[i >> 1] & 0xFFFF0000u : r.u[i >> 1] << 16);
+}
+
+// The same row to the compiler's eye new: what an earlier pass computed from it is computed again, not kept in registers (half a dozen
+// values an element) until the later pass comes.
+template <typename R>
+__device__ __forceinline__ R again(R r) {
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(r.u) / 4); ++i) {
+        uint32_t v = r.u[i];
+        asm volatile("" : "+v"(v));
+        r.u[i] = v;
+    }
+    return r;
 }
 
 // AL: the vector is whole, aligned and loaded at once; otherwise channels [lo, hi) of it exist and are moved one by one
@@ -98,15 +112,14 @@ __device__ __forceinline__ void store_row(T* p, const float (&v)[V], int lo, int
 // otherwise its channels may belong to up to four groups.  AL: whole, aligned vectors.
 // Vectors a thread holds in the three passes, in the variants for short (first) and long clouds, and the waves per SIMD that the
 // registers of that many rows leave.
-constexpr int NR_FWD[2] = {8, 16}, NR_BWD[2] = {8, 16}, NR_BWD2[2] = {4, 8};
+constexpr int NR_FWD[2] = {8, 16}, NR_BWD[2] = {8, 16}, NR_BWD2[2] = {4, 2};
 
 template <typename T_, int V_, bool AL_, bool UNI_, int FAM_, int THREADS_, int NR_>
 struct Cfg {
     typedef T_ T;
     static constexpr int V = V_, FAM = FAM_, THREADS = THREADS_, NR = NR_, NS = UNI_ ? 1 : V_, WAVES = THREADS_ / 64;
     static constexpr bool AL = AL_, UNI = UNI_;
-    static constexpr int FWD_WAVES = THREADS_ > 256 || NR_ <= 8 ? 4 : 3, BWD_WAVES = THREADS_ > 256 ? 4 : NR_ > 8 ? 2 : V_ == 8 ? 3 : 4,
-                         BWD2_WAVES = THREADS_ > 256 ? 4 : NR_ > 4 || V_ == 8 ? 3 : 4;
+    static constexpr int FWD_WAVES = THREADS_ > 256 || NR_ <= 8 ? 4 : 3, BWD_WAVES = THREADS_ > 256 ? 4 : NR_ > 8 ? 2 : 3, BWD2_WAVES = THREADS_ > 256 ? 4 : UNI_ ? 3 : 2;
     static constexpr int at(int i) { return UNI_ ? 0 : i; }
     typedef Raw<T_, V_> Row;
 };
@@ -126,19 +139,21 @@ struct Spot {
     float w[Z::V], b[Z::V];
 };
 
+// V values from channel c0 of a parameter vector; channels outside the slab [s0, s1) read one that is in it
 template <int V>
-__device__ __forceinline__ void load_params(const void* p, int pdt, int c0, int lo, int hi, float otherwise, float (&v)[V]) {
+__device__ __forceinline__ void load_params(const void* p, int pdt, int c0, int s0, int s1, float otherwise, float (&v)[V]) {
 #pragma unroll
     for (int i = 0; i < V; ++i) v[i] = otherwise;
     if (!p) return;
     if (pdt == DD3D_F32) {
 #pragma unroll
-        for (int i = 0; i < V; ++i)
-            if (i >= lo && i < hi) v[i] = ((const float*)p)[c0 + i];
+        for (int i = 0; i < V; ++i) v[i] = ((const float*)p)[min(max(c0 + i, s0), s1 - 1)];
     } else {
+        uint16_t h[V];
 #pragma unroll
-        for (int i = 0; i < V; ++i)
-            if (i >= lo && i < hi) v[i] = load_param(p, pdt, c0 + i);
+        for (int i = 0; i < V; ++i) h[i] = ((const uint16_t*)p)[min(max(c0 + i, s0), s1 - 1)];
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] = widen_bits(h[i], pdt);
     }
 }
 
@@ -168,8 +183,8 @@ __device__ __forceinline__ void locate(const Norm& a, const Geo& g, int unit, in
     s.word = s.rl * g.quads + s.c0 / 4;
 #pragma unroll
     for (int i = 0; i < Z::NS; ++i) s.j[i] = min(quot(max(s.c0 + i - s.s0, 0), g.dCg), s.gs - 1);
-    load_params<Z::V>(a.W, a.pdt, s.c0, s.on ? s.lo : Z::V, s.hi, 1.f, s.w);
-    load_params<Z::V>(a.Bi, a.pdt, s.c0, s.on ? s.lo : Z::V, s.hi, 0.f, s.b);
+    load_params<Z::V>(a.W, a.pdt, s.c0, s.s0, s.s1, 1.f, s.w);
+    load_params<Z::V>(a.Bi, a.pdt, s.c0, s.s0, s.s1, 0.f, s.b);
 }
 
 // a value the compiler must not compute ahead of the loop it is used in: a chunk's eight offsets are one addition each, and kept over the
@@ -184,6 +199,12 @@ __device__ __forceinline__ uint32_t here(uint32_t v) {
 __device__ __forceinline__ float rsqrt_newton(float v) {
     const float r = __builtin_amdgcn_rsqf(v);
     return fmaf(r * 0.5f, fmaf(-v * r, r, 1.f), r);
+}
+
+// a result that is finished here, not moved behind a branch that only some launches take: everything it is made of would live until there
+__device__ __forceinline__ float done(float v) {
+    asm volatile("" : "+v"(v));
+    return v;
 }
 
 // ---- rows of a cloud ------------------------------------------------------------------------------------------------------------
@@ -259,6 +280,65 @@ __device__ __forceinline__ void zero_rest(const Norm& a, T* Y) {
         Y[i < n0 ? i : (int64_t)hi * a.C + (i - n0)] = narrow<T>(0.f);
 }
 
+// ---- lanes' sums without the LDS crossbar ---------------------------------------------------------------------------------------
+template <int CTRL>
+__device__ __forceinline__ float dpp_add(float v) {
+    return v + __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), CTRL, 0xF, 0xF, true));
+}
+// v + the value 16 (32) lanes away: a row swap of v with itself leaves the two halves of every pair side by side
+__device__ __forceinline__ float add_row16(float v) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float add_row32(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+// sum over aligned blocks of `n` lanes (a power of two); all lanes of a block hold it
+template <int K>
+__device__ __forceinline__ void add_block(float (&v)[K], int n) {
+    if (n > 1)
+#pragma unroll
+        for (int k = 0; k < K; ++k) v[k] = dpp_add<0xB1>(v[k]);    // quad_perm 1 0 3 2
+    if (n > 2)
+#pragma unroll
+        for (int k = 0; k < K; ++k) v[k] = dpp_add<0x4E>(v[k]);    // quad_perm 2 3 0 1
+    if (n > 4)
+#pragma unroll
+        for (int k = 0; k < K; ++k) v[k] = dpp_add<0x141>(v[k]);   // row_half_mirror: the other quad of eight
+    if (n > 8)
+#pragma unroll
+        for (int k = 0; k < K; ++k) v[k] = dpp_add<0x140>(v[k]);   // row_mirror: the other eight of sixteen
+    if (n > 16)
+#pragma unroll
+        for (int k = 0; k < K; ++k) v[k] = add_row16(v[k]);
+    if (n > 32)
+#pragma unroll
+        for (int k = 0; k < K; ++k) v[k] = add_row32(v[k]);
+}
+// sum over the lanes that are equal modulo `n` (a power of two); all of them hold it
+template <int K>
+__device__ __forceinline__ void add_strided(float (&v)[K], int n) {
+    if (n <= 1)
+#pragma unroll
+        for (int k = 0; k < K; ++k) v[k] = dpp_add<0xB1>(v[k]);
+    if (n <= 2)
+#pragma unroll
+        for (int k = 0; k < K; ++k) v[k] = dpp_add<0x4E>(v[k]);
+    if (n <= 4)
+#pragma unroll
+        for (int k = 0; k < K; ++k) v[k] = dpp_add<0x124>(v[k]);   // row_ror 4, then 8: the four lanes of a class in sixteen
+    if (n <= 8)
+#pragma unroll
+        for (int k = 0; k < K; ++k) v[k] = dpp_add<0x128>(v[k]);
+    if (n <= 16)
+#pragma unroll
+        for (int k = 0; k < K; ++k) v[k] = add_row16(v[k]);
+    if (n <= 32)
+#pragma unroll
+        for (int k = 0; k < K; ++k) v[k] = add_row32(v[k]);
+}
+
 // ---- sums -----------------------------------------------------------------------------------------------------------------------
 // v[q][i], per thread and (with !UNI) channel -> the sum over the rows of the workgroup and the channels of the group that thread and channel
 // belong to.  Lanes without rows bring zeros.
@@ -266,27 +346,23 @@ template <int K, typename Z>
 __device__ __forceinline__ void group_sums(float (&v)[K][Z::NS], const Norm& a, const Geo& g, Spot<Z>& s, float* lds) {
     if (Z::UNI && g.fast) {
         // the group's lanes, then the wave's row lanes; one value per wave and group through LDS.  Two buffers in turn: one barrier a call
-        for (int o = 1; o < g.cw; o <<= 1) {
+        float t[K];
 #pragma unroll
-            for (int q = 0; q < K; ++q) v[q][0] += __shfl_xor(v[q][0], o, 64);
-        }
-        for (int o = g.CL; o < 64; o <<= 1) {
-#pragma unroll
-            for (int q = 0; q < K; ++q) v[q][0] += __shfl_xor(v[q][0], o, 64);
-        }
+        for (int q = 0; q < K; ++q) t[q] = v[q][0];
+        add_block(t, g.cw);
+        add_strided(t, g.CL);
         float* red = lds + s.buf * (g.red >> 1);   // (a fixed half: calls of different K follow each other)
         s.buf ^= 1;
         if (s.lane < g.CL && (s.lane & (g.cw - 1)) == 0 && s.hi > 0) {
 #pragma unroll
-            for (int q = 0; q < K; ++q) red[(q * Z::WAVES + s.wave) * g.k + s.j[0]] = v[q][0];
+            for (int q = 0; q < K; ++q) red[(q * Z::WAVES + s.wave) * g.k + s.j[0]] = t[q];
         }
         __syncthreads();
 #pragma unroll
         for (int q = 0; q < K; ++q) {
-            float t = 0.f;
+            v[q][0] = 0.f;
 #pragma unroll
-            for (int p = 0; p < Z::WAVES; ++p) t += red[(q * Z::WAVES + p) * g.k + s.j[0]];
-            v[q][0] = t;
+            for (int p = 0; p < Z::WAVES; ++p) v[q][0] += red[(q * Z::WAVES + p) * g.k + s.j[0]];
         }
         return;
     }
@@ -421,6 +497,13 @@ __device__ __forceinline__ uint32_t keep_bits(const Drop& d, const PhiloxKey& k,
     }
     return m;
 }
+// dropout of one row's values, behind one uniform branch
+template <int V>
+__device__ __forceinline__ void drop_row(const Drop& d, uint32_t keep, float (&v)[V]) {
+    if (!d.key) return;
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = keep >> i & 1 ? v[i] * d.scale : 0.f;
+}
 __device__ __forceinline__ PhiloxKey drop_key(const Drop& d) {
     PhiloxKey k = {0, 0, 0, 0};
     if (d.key) k = philox_key(d.key);
@@ -449,6 +532,61 @@ __device__ __forceinline__ uint64_t words_at(const Geo& g, int base) { return (u
 
 // one row after the other: the scheduler would otherwise work on all of a chunk's rows at once and run out of registers
 __device__ __forceinline__ void row_border() { __builtin_amdgcn_sched_barrier(0); }
+
+// ---- the caller's workspace, and the parameter gradients in it --------------------------------------------------------------------
+struct Work {
+    float *part, *slots, *folded;   // pieces' sums; [units][2][C]; [FOLD][2][C]
+    int *found, *tickets;           // pieces per window; arrivals per column block
+};
+constexpr int FOLD = 32;            // workgroups that share a block of 64 columns
+
+// where the folding workgroups of a launch begin, and what they write
+struct Fold {
+    unsigned first;
+    int parts;
+    void *dw, *db;
+};
+
+__device__ __forceinline__ void clear_tickets(const Geo& g, const Work& w) {
+    if (blockIdx.x == 0 && w.slots)
+        for (int i = threadIdx.x; i < g.tickets; i += blockDim.x) w.tickets[i] = 0;
+}
+
+// out[q][c] = the sum over units of slots[unit][q][c]: workgroup (column block, part) adds every parts-th unit, a thread a column and every
+// WAVES-th of those; the last of a column block to arrive adds the parts, in part order, so the result does not depend on who is last.
+template <int THREADS>
+__device__ __forceinline__ void fold_slots(const Norm& a, const Geo& g, const Work& w, const Fold& f, unsigned block, float* lds) {
+    constexpr int WAVES = THREADS / 64;
+    const int cols = 2 * a.C, blocks = (cols + 63) / 64, cb = block % blocks, part = block / blocks;
+    const int c = cb * 64 + (threadIdx.x & 63), lane = threadIdx.x >> 6, n = g.U + g.NW;
+    float t = 0.f;
+    if (c < cols)
+#pragma unroll 8
+        for (int i = part + lane * f.parts; i < n; i += WAVES * f.parts)
+            if (i < g.U || w.found[i - g.U]) t += w.slots[(int64_t)i * cols + c];   // (a window without a large cloud has written nothing)
+    lds[threadIdx.x] = t;
+    __syncthreads();
+    if (lane == 0) {
+        for (int i = 1; i < WAVES; ++i) t += lds[threadIdx.x + i * 64];
+        if (f.parts > 1 && c < cols) w.folded[(int64_t)part * cols + c] = t;
+    }
+    if (f.parts > 1) {
+        __threadfence();
+        __syncthreads();
+        int* last = (int*)lds + THREADS;
+        if (threadIdx.x == 0) *last = atomicAdd(&w.tickets[cb], 1) == f.parts - 1;
+        __syncthreads();
+        if (!*last) return;
+        __threadfence();
+        t = 0.f;
+        if (lane == 0 && c < cols)
+#pragma unroll 8
+            for (int i = 0; i < f.parts; ++i) t += __hip_atomic_load(&w.folded[(int64_t)i * cols + c], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    if (lane || c >= cols) return;
+    void* to = c < a.C ? f.dw : f.db;
+    if (to) store_param(to, a.pdt, c < a.C ? c : c - a.C, t);
+}
 
 // ---- forward --------------------------------------------------------------------------------------------------------------------
 template <typename Z>
@@ -484,9 +622,10 @@ struct Fwd {
 #pragma unroll
         for (int n = 0; n < NR; ++n)
             if (s.rl + n * g.RL < left) {
+                const typename Z::Row x = again(z[n]);
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
-                    const float d = raw_get(z[n], i) - sx[Z::at(i)];
+                    const float d = raw_get(x, i) - sx[Z::at(i)];
                     q[Z::at(i)] = fmaf(d, d, q[Z::at(i)]);
                 }
             }
@@ -576,13 +715,12 @@ struct Fwd {
             row_border();
             if (s.rl + n * g.RL >= left) continue;
             float y[V], d1, d2;
+            const typename Z::Row x = again(z[n]);
 #pragma unroll
             for (int i = 0; i < V; ++i)
-                y[i] = activate<Z::FAM, 0>(fmaf((raw_get(z[n], i) - mean[Z::at(i)]) * rstd[Z::at(i)], s.w[i], s.b[i]), a.slope, &d1, &d2);
+                y[i] = activate<Z::FAM, 0>(fmaf((raw_get(x, i) - mean[Z::at(i)]) * rstd[Z::at(i)], s.w[i], s.b[i]), a.slope, &d1, &d2);
             if (a.drop.key) {
-                const uint32_t keep = keep_bits<V>(a.drop, key, words + (word + n * (uint32_t)(g.RL * g.quads)));
-#pragma unroll
-                for (int i = 0; i < V; ++i) y[i] = keep >> i & 1 ? y[i] * a.drop.scale : 0.f;
+                drop_row<V>(a.drop, keep_bits<V>(a.drop, key, words + (word + n * (uint32_t)(g.RL * g.quads))), y);
             }
             store_at<Z>(to, off + n * s.step, y, s);
         }
@@ -703,13 +841,14 @@ struct Bwd {
     // xh and g of one row
     __device__ __forceinline__ void element(const typename Z::Row& x, const typename Z::Row& d, uint32_t keep, float (&xh)[V], float (&gr)[V]) {
 #pragma unroll
+        for (int i = 0; i < V; ++i) gr[i] = raw_get(d, i);
+        drop_row<V>(a.drop, keep, gr);
+#pragma unroll
         for (int i = 0; i < V; ++i) {
             float d1, d2;
             xh[i] = (raw_get(x, i) - mean[Z::at(i)]) * rstd[Z::at(i)];
             activate<Z::FAM, 1>(fmaf(xh[i], s.w[i], s.b[i]), a.slope, &d1, &d2);
-            float dy = raw_get(d, i);
-            if (a.drop.key) dy = keep >> i & 1 ? dy * a.drop.scale : 0.f;
-            gr[i] = dy * d1;
+            gr[i] *= d1;
         }
     }
 
@@ -762,7 +901,7 @@ struct Bwd {
                     if (fresh) keep = keep_bits<V>(a.drop, key, words + (word + n * (uint32_t)(g.RL * g.quads)));
                     else keep = h.keep[HOLD ? 0 : n * V / 32] >> (n * V % 32);
                 }
-                element(h.x[n], h.d[n], keep, xh, gr);
+                element(again(h.x[n]), again(h.d[n]), keep, xh, gr);
             }
 #pragma unroll
             for (int i = 0; i < V; ++i) dx[i] = rstd[Z::at(i)] * fmaf(gr[i], s.w[i], -fmaf(xh[i], m2[Z::at(i)], m1[Z::at(i)]));
@@ -810,17 +949,23 @@ struct Bwd {
     }
 };
 
-// part [2 * NW][G][2]: sums of h and h xh over a piece; slots [U + NW][2][C]: parameter gradients of a unit (NULL: not asked for)
+// part [2 * NW][G][2]: sums of h and h xh over a piece; w.slots NULL: no parameter gradients asked for
 template <typename Z, int MODE>
 __global__ __launch_bounds__(Z::THREADS, Z::BWD_WAVES) void k_bwd(Norm a, Geo g, const typename Z::T* dY, const typename Z::T* X, const float* mean_in,
-                                                                 const float* rstd_in, typename Z::T* dX, float* part, int* found, float* slots) {
+                                                                 const float* rstd_in, typename Z::T* dX, Work w, Fold fold) {
     extern __shared__ __align__(16) float lds[];
-    if (MODE == 0) zero_rest(a, dX);
+    if (MODE == 0) {
+        zero_rest(a, dX);
+        clear_tickets(g, w);
+    } else if (blockIdx.x >= fold.first) {   // the windows' launch brings the parameter gradients along
+        fold_slots<Z::THREADS>(a, g, w, fold, blockIdx.x - fold.first, lds);
+        return;
+    }
     int unit, slab;
     if (!place(g, unit, slab)) return;
     const bool whole = MODE == 0 && unit < g.U;
     Piece p[2];
-    const int np = whole ? 0 : window_pieces<MODE == 0>(a, g, unit - (MODE == 0 ? g.U : 0), found, p);
+    const int np = whole ? 0 : window_pieces<MODE == 0>(a, g, unit - (MODE == 0 ? g.U : 0), w.found, p);
     if (!whole && np == 0) return;
     Spot<Z> s;
     locate(a, g, unit, slab, s);
@@ -846,7 +991,7 @@ __global__ __launch_bounds__(Z::THREADS, Z::BWD_WAVES) void k_bwd(Norm a, Geo g,
             }
             f.sums(r, v);
             if (!whole) {
-                put_part<2, Z>(part, i ? p[1].slot : p[0].slot, v, a, g, s);
+                put_part<2, Z>(w.part, i ? p[1].slot : p[0].slot, v, a, g, s);
             } else if (dX) {
                 f.means(v, r.r1 - r.r0);
                 f.apply(r, v[0], v[1]);
@@ -856,11 +1001,11 @@ __global__ __launch_bounds__(Z::THREADS, Z::BWD_WAVES) void k_bwd(Norm a, Geo g,
         if (i >= np) break;
         const Piece q = i ? p[1] : p[0];
         f.load_stats(q.b, mean_in, rstd_in);
-        join_parts<2, Z>(part, q.all, v, a, g, s, lds);
+        join_parts<2, Z>(w.part, q.all, v, a, g, s, lds);
         f.means(v, q.all.r1 - q.all.r0);
         f.apply(q.part, v[0], v[1]);
     }
-    if (MODE == 0 && slots) column_sums<2, Z>(f.par, a, g, s, lds, slots + (int64_t)unit * 2 * a.C);
+    if (MODE == 0 && w.slots) column_sums<2, Z>(f.par, a, g, s, lds, w.slots + (int64_t)unit * 2 * a.C);
 }
 
 // ---- second gradient ------------------------------------------------------------------------------------------------------------
@@ -883,8 +1028,11 @@ struct Bwd2 {
         typename Z::Row x[NR], d[NR], p[NR];
         uint32_t keep[KW];
     };
-    // means over the cloud of h, h xh, P, P xh, P h, q g, q g xh
-    enum { H, HX, MP, PX, PH, QG, QX, KS };
+    // Means over the cloud of h, h xh, P, P xh, P h, q g, q g xh; and, with e = w dy D phi'' and c = q xh + s, of w e {1, xh, xh xh, P, P xh}, e c,
+    // e c xh.  ub = dy D phi'' gb is linear in the means of P and P xh that gb holds, so those seven give the means of w ub and w ub xh
+    // without a second pass over the rows.
+    enum { H, HX, MP, PX, PH, QG, QX, E0, E1, E2, EP, EPX, EC, ECX };
+    static constexpr int KS = Z::FAM == DD3D_FAM_LINEAR ? 7 : 14;
 
     __device__ __forceinline__ void load_stats(int b, const float* mean_in, const float* rstd_in) {
         const int64_t at = (int64_t)b * a.G + s.slab * g.k;
@@ -908,22 +1056,28 @@ struct Bwd2 {
         }
     }
 
-    struct Elem {
-        float xh, p, dy, D, d1, d2;   // dy: after dropout
+    // one row: values after dropout, and the activation's derivatives element by element
+    struct RowOf {
+        float x[V], p[V], dy[V];
     };
-    template <int ORDER>
-    __device__ __forceinline__ Elem element(const Held& h, int n, int i) {
+    __device__ __forceinline__ RowOf row_of(const typename Z::Row& x, const typename Z::Row& d, const typename Z::Row& p, uint32_t keep) {
+        RowOf r;
+#pragma unroll
+        for (int i = 0; i < V; ++i) r.x[i] = raw_get(x, i), r.dy[i] = raw_get(d, i), r.p[i] = 0.f;
+        drop_row<V>(a.drop, keep, r.dy);
+        if (P)
+#pragma unroll
+            for (int i = 0; i < V; ++i) r.p[i] = raw_get(p, i);
+        return r;
+    }
+    struct Elem {
+        float xh, p, dy, d1, d2;
+    };
+    __device__ __forceinline__ Elem element(const RowOf& r, int i) {
         Elem e;
-        e.xh = (raw_get(h.x[n], i) - mean[Z::at(i)]) * rstd[Z::at(i)];
-        e.p = P ? raw_get(h.p[n], i) : 0.f;
-        e.D = 1.f;
-        e.dy = raw_get(h.d[n], i);
-        if (a.drop.key) {
-            const bool kept = h.keep[n * V / 32] >> (n * V % 32 + i) & 1;
-            e.D = kept ? a.drop.scale : 0.f;
-            e.dy = kept ? e.dy * a.drop.scale : 0.f;
-        }
-        activate<Z::FAM, ORDER>(fmaf(e.xh, s.w[i], s.b[i]), a.slope, &e.d1, &e.d2);
+        e.xh = (r.x[i] - mean[Z::at(i)]) * rstd[Z::at(i)];
+        e.p = r.p[i], e.dy = r.dy[i];
+        activate<Z::FAM, 2>(fmaf(e.xh, s.w[i], s.b[i]), a.slope, &e.d1, &e.d2);
         return e;
     }
 
@@ -933,10 +1087,12 @@ struct Bwd2 {
         for (int n = 0; n < NR; ++n) {
             row_border();
             if (s.rl + n * g.RL >= left) continue;
+            const RowOf row = row_of(h.x[n], h.d[n], h.p[n], h.keep[n * V / 32] >> (n * V % 32));
 #pragma unroll
             for (int i = 0; i < V; ++i) {
+                row_border();
                 const int c = Z::at(i);
-                const Elem e = element<1>(h, n, i);
+                const Elem e = element(row, i);
                 const float gr = e.dy * e.d1, hh = gr * s.w[i], qg = gr * q[i];
                 v[H][c] += hh;
                 v[HX][c] = fmaf(hh, e.xh, v[HX][c]);
@@ -945,6 +1101,16 @@ struct Bwd2 {
                 v[PH][c] = fmaf(e.p, hh, v[PH][c]);
                 v[QG][c] += qg;
                 v[QX][c] = fmaf(qg, e.xh, v[QX][c]);
+                if constexpr (KS > 7) {
+                    const float w1 = e.dy * e.d2 * s.w[i], w2 = w1 * s.w[i], wx = w2 * e.xh, wc = w1 * fmaf(q[i], e.xh, t[i]);
+                    v[E0][c] += w2;
+                    v[E1][c] += wx;
+                    v[E2][c] = fmaf(wx, e.xh, v[E2][c]);
+                    v[EP][c] = fmaf(w2, e.p, v[EP][c]);
+                    v[EPX][c] = fmaf(wx, e.p, v[EPX][c]);
+                    v[EC][c] += wc;
+                    v[ECX][c] = fmaf(wc, e.xh, v[ECX][c]);
+                }
             }
         }
     }
@@ -956,24 +1122,6 @@ struct Bwd2 {
         return fmaf(s.w[i], vv, fmaf(q[i], e.xh, t[i]));
     }
 
-    // sums of w ub and w ub xh
-    __device__ __forceinline__ void add_rows2(int all, const Held& h, const float (&m)[KS][NS], float (&v)[2][NS]) {
-        const int left = s.on ? all : 0;
-#pragma unroll
-        for (int n = 0; n < NR; ++n) {
-            row_border();
-            if (s.rl + n * g.RL >= left) continue;
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                const Elem e = element<2>(h, n, i);
-                float vv;
-                const float wub = gbar(e, m, i, vv) * e.dy * e.d2 * s.w[i];
-                v[0][Z::at(i)] += wub;
-                v[1][Z::at(i)] = fmaf(wub, e.xh, v[1][Z::at(i)]);
-            }
-        }
-    }
-
     __device__ __forceinline__ void rows_out(int base, int all, const Held& h, const float (&m)[KS][NS], const float (&u)[2][NS]) {
         const int left = s.on ? all : 0;
         T *to_y = ddY + row_at(a, base), *to_x = ddX + row_at(a, base);
@@ -983,18 +1131,23 @@ struct Bwd2 {
             row_border();
             if (s.rl + n * g.RL >= left) continue;
             float oy[V], ox[V];
+            const typename Z::Row x = again(h.x[n]), d = again(h.d[n]), p = again(h.p[n]);
+            const uint32_t keep = h.keep[n * V / 32] >> (n * V % 32);
+            const RowOf row = row_of(x, d, p, keep);
 #pragma unroll
             for (int i = 0; i < V; ++i) {
+                row_border();
                 const int c = Z::at(i);
-                const Elem e = element<2>(h, n, i);
+                const Elem e = element(row, i);
                 float vv;
                 const float gb = gbar(e, m, i, vv), gr = e.dy * e.d1, hh = gr * s.w[i], ub = Z::FAM == DD3D_FAM_LINEAR ? 0.f : gb * e.dy * e.d2;
                 const float X = fmaf(q[i], gr, s.w[i] * ub) - rstd[c] * fmaf(hh, m[PX][c], e.p * m[HX][c]);
-                oy[i] = e.D == 0.f ? 0.f : gb * e.d1 * e.D;
-                ox[i] = rstd[c] * (X - fmaf(e.xh, u[1][c], u[0][c]));
+                oy[i] = done(gb * e.d1);
+                ox[i] = done(rstd[c] * (X - fmaf(e.xh, u[1][c], u[0][c])));
                 par[0][i] += fmaf(gr, vv, ub * e.xh);
                 par[1][i] += ub;
             }
+            drop_row<V>(a.drop, keep, oy);
             if (ddY) store_at<Z>(to_y, off + n * s.step, oy, s);
             if (ddX) store_at<Z>(to_x, off + n * s.step, ox, s);
         }
@@ -1007,20 +1160,19 @@ struct Bwd2 {
 #pragma unroll
             for (int i = 0; i < NS; ++i) m[k][i] *= inv;
     }
-    // sums of w ub and w ub xh -> the mean of X, and what multiplies xh
-    __device__ __forceinline__ void finish(const float (&m)[KS][NS], float (&u)[2][NS], int rows) {
-        const float inv = 1.f / ((float)rows * (float)a.Cg);
+    // the mean of X, and what multiplies xh in d(x)
+    __device__ __forceinline__ void finish(const float (&m)[KS][NS], float (&u)[2][NS]) {
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
-            u[0][i] = fmaf(u[0][i], inv, m[QG][i]) - rstd[i] * fmaf(m[PX][i], m[H][i], m[HX][i] * m[MP][i]);
-            u[1][i] = fmaf(u[1][i], inv, m[QX][i]) + rstd[i] * (m[PH][i] - m[MP][i] * m[H][i] - 3.f * (m[PX][i] * m[HX][i]));
+            u[0][i] = m[QG][i] - rstd[i] * fmaf(m[PX][i], m[H][i], m[HX][i] * m[MP][i]);
+            u[1][i] = m[QX][i] + rstd[i] * (m[PH][i] - m[MP][i] * m[H][i] - 3.f * (m[PX][i] * m[HX][i]));
+            if constexpr (KS > 7) {   // means of w ub, w ub xh
+                u[0][i] += fmaf(rstd[i], m[EP][i] - fmaf(m[MP][i], m[E0][i], m[PX][i] * m[E1][i]), m[EC][i]);
+                u[1][i] += fmaf(rstd[i], m[EPX][i] - fmaf(m[MP][i], m[E1][i], m[PX][i] * m[E2][i]), m[ECX][i]);
+            }
         }
     }
 
-    __device__ __forceinline__ void clear(float (&u)[2][NS]) {
-#pragma unroll
-        for (int i = 0; i < NS; ++i) u[0][i] = u[1][i] = 0.f;
-    }
     __device__ __forceinline__ void clear(float (&m)[KS][NS]) {
 #pragma unroll
         for (int k = 0; k < KS; ++k)
@@ -1028,22 +1180,6 @@ struct Bwd2 {
             for (int i = 0; i < NS; ++i) m[k][i] = 0.f;
     }
 
-    __device__ __forceinline__ void short_cloud(const Range& r) {
-        const int rows = r.r1 - r.r0;
-        Held h;
-        float m[KS][NS], u[2][NS];
-        clear(m), clear(u);
-        load(r.r0, rows, h);
-        add_rows(rows, h, m);
-        group_sums<KS, Z>(m, a, g, s, lds);
-        means(m, rows);
-        if (Z::FAM != DD3D_FAM_LINEAR) {
-            add_rows2(rows, h, m, u);
-            group_sums<2, Z>(u, a, g, s, lds);
-        }
-        finish(m, u, rows);
-        rows_out(r.r0, rows, h, m, u);
-    }
     __device__ __forceinline__ void sums(const Range& r, float (&m)[KS][NS]) {
         clear(m);
         for (int base = r.r0; base < r.r1; base += NR * g.RL) {
@@ -1052,16 +1188,6 @@ struct Bwd2 {
             add_rows(r.r1 - base, h, m);
         }
         group_sums<KS, Z>(m, a, g, s, lds);
-    }
-    __device__ __forceinline__ void sums2(const Range& r, const float (&m)[KS][NS], float (&u)[2][NS]) {
-        clear(u);
-        if (Z::FAM == DD3D_FAM_LINEAR) return;
-        for (int base = r.r0; base < r.r1; base += NR * g.RL) {
-            Held h;
-            load(base, r.r1 - base, h);
-            add_rows2(r.r1 - base, h, m, u);
-        }
-        group_sums<2, Z>(u, a, g, s, lds);
     }
     __device__ __forceinline__ void apply(const Range& r, const float (&m)[KS][NS], const float (&u)[2][NS]) {
         for (int base = r.r0; base < r.r1; base += NR * g.RL) {
@@ -1072,29 +1198,29 @@ struct Bwd2 {
     }
 };
 
-// part1 [2 * NW][G][7], part2 [2 * NW][G][2]: a piece's sums of the first and second pass.  MODE 0: the clouds, and the windows' first
-// sums; MODE 1: the windows' second sums; MODE 2: the windows' rows
+// part [2 * NW][G][KS]: a piece's sums.  MODE 0: the clouds, and the windows' sums; MODE 1: the windows' rows
 template <typename Z, int MODE>
 __global__ __launch_bounds__(Z::THREADS, Z::BWD2_WAVES) void k_bwd2(Norm a, Geo g, const typename Z::T* P, const void* ggw, const void* ggb, const typename Z::T* dY,
                                                                    const typename Z::T* X, const float* mean_in, const float* rstd_in, typename Z::T* ddY,
-                                                                   typename Z::T* ddX, float* part1, float* part2, int* found, float* slots) {
+                                                                   typename Z::T* ddX, Work w) {
     extern __shared__ __align__(16) float lds[];
     if (MODE == 0) {
         zero_rest(a, ddY);
         zero_rest(a, ddX);
+        clear_tickets(g, w);
     }
     int unit, slab;
     if (!place(g, unit, slab)) return;
     const bool whole = MODE == 0 && unit < g.U;
     Piece p[2];
-    const int np = whole ? 0 : window_pieces<MODE == 0>(a, g, unit - (MODE == 0 ? g.U : 0), found, p);
+    const int np = whole ? 0 : window_pieces<MODE == 0>(a, g, unit - (MODE == 0 ? g.U : 0), w.found, p);
     if (!whole && np == 0) return;
     Spot<Z> s;
     locate(a, g, unit, slab, s);
     typedef Bwd2<Z> F;
     F f{a, g, s, P, dY, X, ddY, ddX, lds, drop_key(a.drop)};
-    load_params<Z::V>(ggw, a.pdt, s.c0, s.on ? s.lo : Z::V, s.hi, 0.f, f.q);
-    load_params<Z::V>(ggb, a.pdt, s.c0, s.on ? s.lo : Z::V, s.hi, 0.f, f.t);
+    load_params<Z::V>(ggw, a.pdt, s.c0, s.s0, s.s1, 0.f, f.q);
+    load_params<Z::V>(ggb, a.pdt, s.c0, s.s0, s.s1, 0.f, f.t);
 #pragma unroll
     for (int i = 0; i < Z::V; ++i) f.par[0][i] = f.par[1][i] = 0.f;
     float m[F::KS][Z::NS], u[2][Z::NS];
@@ -1110,42 +1236,28 @@ __global__ __launch_bounds__(Z::THREADS, Z::BWD2_WAVES) void k_bwd2(Norm a, Geo 
                 r = i ? p[1].part : p[0].part;
             }
             f.load_stats(whole ? b : i ? p[1].b : p[0].b, mean_in, rstd_in);
-            if (whole && r.r1 - r.r0 <= Z::NR * g.RL) {
-                f.short_cloud(r);
-                continue;
-            }
             f.sums(r, m);
             if (!whole) {
-                put_part<F::KS, Z>(part1, i ? p[1].slot : p[0].slot, m, a, g, s);
+                put_part<F::KS, Z>(w.part, i ? p[1].slot : p[0].slot, m, a, g, s);
                 continue;
             }
             f.means(m, r.r1 - r.r0);
-            f.sums2(r, m, u);
-            f.finish(m, u, r.r1 - r.r0);
+            f.finish(m, u);
             f.apply(r, m, u);
             continue;
         }
         if (i >= np) break;
         const Piece q = i ? p[1] : p[0];
-        const int rows = q.all.r1 - q.all.r0;
         f.load_stats(q.b, mean_in, rstd_in);
-        join_parts<F::KS, Z>(part1, q.all, m, a, g, s, lds);
-        f.means(m, rows);
-        if (MODE == 1) {
-            f.sums2(q.part, m, u);
-            put_part<2, Z>(part2, q.slot, u, a, g, s);
-            continue;
-        }
-        f.clear(u);
-        if (Z::FAM != DD3D_FAM_LINEAR) join_parts<2, Z>(part2, q.all, u, a, g, s, lds);
-        f.finish(m, u, rows);
+        join_parts<F::KS, Z>(w.part, q.all, m, a, g, s, lds);
+        f.means(m, q.all.r1 - q.all.r0);
+        f.finish(m, u);
         f.apply(q.part, m, u);
     }
     // a window's parameter gradients belong to its rows' last pass
-    if (slots && (MODE == 2 || whole)) column_sums<2, Z>(f.par, a, g, s, lds, slots + (int64_t)(MODE == 2 ? g.U + unit : unit) * 2 * a.C);
+    if (w.slots && (MODE == 1 || whole)) column_sums<2, Z>(f.par, a, g, s, lds, w.slots + (int64_t)(MODE == 1 ? g.U + unit : unit) * 2 * a.C);
 }
 
-// ---- launches (one translation unit per row type and pass) ----------------------------------------------------------------------
 struct Plan {
     Geo g;
     int V, fam, size;            // size: 0 few rows a thread, 1 many, 2 sixteen waves (slabs of more than 256 vectors)
@@ -1154,17 +1266,13 @@ struct Plan {
     size_t lds;
 };
 
-struct Work {   // the caller's workspace
-    float *part1, *part2, *slots, *folded;
-    int* found;
-};
-
 template <typename T>
 int launch_fwd(const Norm& a, const Plan& p, const void* X, void* Y, float* mean, float* rstd, const Work& w, hipStream_t st);
 template <typename T>
-int launch_bwd(const Norm& a, const Plan& p, const void* dY, const void* X, const float* mean, const float* rstd, void* dX, const Work& w, hipStream_t st);
+int launch_bwd(const Norm& a, const Plan& p, const void* dY, const void* X, const float* mean, const float* rstd, void* dX, const Work& w, Fold f, hipStream_t st);
 template <typename T>
 int launch_bwd2(const Norm& a, const Plan& p, const void* P, const void* ggw, const void* ggb, const void* dY, const void* X, const float* mean, const float* rstd,
-                void* ddY, void* ddX, const Work& w, hipStream_t st);
+                void* ddY, void* ddX, const Work& w, Fold f, hipStream_t st);
+int launch_fold(const Norm& a, const Plan& p, const Work& w, Fold f, hipStream_t st);   // (group_norm.hip)
 
 }  // namespace gn

@@ -6,8 +6,7 @@
 //   v = r (P - m(P) - xh m(P xh)),  gb = w v + q xh + s,  d(dy) = gb D phi',  ub = gb dy D phi''
 //   X = -r (h m(P xh) + P m(h xh)) + q g + w ub
 //   d(x) = r (X - m(X) - xh (m(X xh) + r (m(P h) - m(P) m(h) - m(P xh) m(h xh)))),  d(w) = sum_rows (g v + ub xh),  d(b) = sum_rows ub
-// m(X) and m(X xh) follow from the first pass's means and those of w ub and w ub xh, which take a second pass over the rows (none where
-// phi is piecewise linear and ub = 0).  The kernels: group_norm.h.  Here: argument checks, launch geometry, parameter gradients.
+// m(X) and m(X xh) follow from sums that one pass over the rows gives (group_norm.h).  The kernels: group_norm.h.  Here: argument checks, launch geometry, parameter gradients.
 #include "group_norm.h"
 
 #include <stdlib.h>
@@ -25,43 +24,9 @@ __global__ void k_zero_half(uint16_t* y, int64_t n) {
     if (threadIdx.x == 0 && n > 0) y[n - 1] = 0;   // the odd last element of a half-width matrix
 }
 
-// ---- parameter gradients: out[q][c] = sum over the units' slots [slot][2][C], slots in a fixed order ------------------------------
-// One column a thread, four row lanes a workgroup, `parts` workgroups a column block; they write their sums to `folded` for a second
-// launch of the same kernel, or with parts = 1 the result.
-__global__ __launch_bounds__(256) void k_fold(const float* slots, int n, int U, const int* found, int cols, int parts, float* folded, void* dw, void* db, int C,
-                                              int pdt) {
-    __shared__ float s_red[256];
-    const int c = blockIdx.x * 64 + (threadIdx.x & 63), part = blockIdx.y, lane = threadIdx.x >> 6;
-    float t = 0.f;
-    if (c < cols)
-#pragma unroll 8
-        for (int i = part + lane * parts; i < n; i += 4 * parts)
-            if (i < U || found[i - U]) t += slots[(int64_t)i * cols + c];   // (a window without a large cloud has written nothing)
-    s_red[threadIdx.x] = t;
-    __syncthreads();
-    if (lane || c >= cols) return;
-    t = s_red[threadIdx.x] + s_red[threadIdx.x + 64] + s_red[threadIdx.x + 128] + s_red[threadIdx.x + 192];
-    if (parts > 1) {
-        folded[(int64_t)part * cols + c] = t;
-        return;
-    }
-    void* to = c < C ? dw : db;
-    if (to) store_param(to, pdt, c < C ? c : c - C, t);
-}
-
-constexpr int FOLD = 32;
-
-inline int fold(const gn::Norm& a, const gn::Geo& g, const gn::Work& w, void* dw, void* db, hipStream_t st) {
-    const int n = g.U + g.NW, cols = 2 * a.C;
-    const unsigned blocks = (unsigned)ceil_div64(cols, 64);
-    if (n <= 128) {
-        k_fold<<<blocks, 256, 0, st>>>(w.slots, n, g.U, w.found, cols, 1, nullptr, dw, db, a.C, a.pdt);
-    } else {
-        k_fold<<<dim3(blocks, FOLD), 256, 0, st>>>(w.slots, n, g.U, w.found, cols, FOLD, w.folded, nullptr, nullptr, a.C, a.pdt);
-        k_fold<<<blocks, 256, 0, st>>>(w.folded, FOLD, FOLD, nullptr, cols, 1, nullptr, dw, db, a.C, a.pdt);
-    }
-    DD3D_CHECK_LAUNCH();
-    return 0;
+__global__ __launch_bounds__(256) void k_fold(gn::Norm a, gn::Geo g, gn::Work w, gn::Fold f) {
+    __shared__ float lds[256 + 1];
+    gn::fold_slots<256>(a, g, w, f, blockIdx.x, lds);
 }
 
 // ---- launch geometry --------------------------------------------------------------------------------------------------------------
@@ -82,6 +47,7 @@ inline gn::Div divide_by(int d) {
 inline int cloud_units(int B, bool params) { return params && B > MAX_UNITS ? (int)ceil_div64(B, ceil_div64(B, MAX_UNITS)) : B; }
 
 // sums: quantities summed at once; nr: vectors a thread holds in the variants for short and long clouds; params: column_sums is called
+constexpr int NR_STREAM[2] = {16, 16};
 inline gn::Plan plan(const gn::Norm& a, int act, int esize, bool aligned, int sums, const int (&nr)[2], bool params) {
     gn::Plan p;
     gn::Geo& g = p.g;
@@ -120,13 +86,14 @@ inline gn::Plan plan(const gn::Norm& a, int act, int esize, bool aligned, int su
     g.fast = p.uni && g.lcl >= 0 && (g.cw & (g.cw - 1)) == 0;
     g.quads = (a.C + 3) / 4;
     g.dCL = divide_by(g.CL), g.dCg = divide_by(a.Cg);
-    const int64_t cap = (int64_t)nr[p.size == 1] * g.RL;
+    const int64_t cap = (int64_t)nr[p.size == 1] * g.RL;   // rows of a chunk
     g.NW = (int)std::min<int64_t>(ceil_div64(a.M, MIN_WINDOW), max_windows(a.C));
     g.CH = g.NW ? (int)ceil_div64(a.M, g.NW) : 1;
     g.Tl = (int)std::max<int64_t>(2 * cap, g.CH);
     g.NW = a.M <= g.Tl ? 0 : (int)ceil_div64(a.M, g.CH);
     g.U = cloud_units(a.B, params);
     g.units = 0;
+    g.tickets = params ? (2 * a.C + 63) / 64 : 0;
     p.blocks0 = (unsigned)(align_up64((int64_t)g.U + g.NW, 8) * g.nslab);
     p.blocks1 = (unsigned)(align_up64(g.NW, 8) * g.nslab);
     // LDS: row partials of kb quantities (or two buffers of the waves' sums, or the columns of one parameter gradient), the columns' totals
@@ -135,38 +102,44 @@ inline gn::Plan plan(const gn::Norm& a, int act, int esize, bool aligned, int su
     g.kb = std::max(1, std::min(sums, 8192 / (g.RL * cols)));
     g.red = g.fast ? 2 * sums * (threads / 64) * g.k : g.kb * g.RL * cols;
     if (params) g.red = std::max(g.red, (g.lcl >= 0 ? threads / 64 : g.RL) * g.CL * p.V);
-    p.lds = sizeof(float) * ((size_t)g.red + g.kb * cols + sums * g.k);
+    p.lds = sizeof(float) * std::max<size_t>((size_t)g.red + g.kb * cols + sums * g.k, params ? threads + 1 : 0);
     return p;
 }
 
-// The workspace: piece sums, units' slots and their folded sums, pieces per window.  Sized by bounds that hold for every type and alignment.
+// The workspace: piece sums, units' slots and their folded sums, pieces per window, tickets.  Sized by bounds that hold for every type and
+// alignment.
 struct Layout {
-    int64_t part1, part2, slots, folded, found, bytes;
+    int64_t part, slots, folded, found, tickets, bytes;
 };
 inline Layout layout(int64_t M, int C, int B, int G, int order) {
     const int64_t windows = M > MIN_WINDOW ? std::min<int64_t>(ceil_div64(M, MIN_WINDOW), max_windows(C)) : 0;
-    const int64_t units = order ? cloud_units(B, true) + windows : 0, pieces = 2 * windows * G;
+    const int64_t units = order && B ? cloud_units(B, true) + windows : 0;
     Layout l;
     int64_t at = 0;
-    auto take = [&](int64_t floats) {
+    auto take = [&](int64_t words) {
         const int64_t here = at;
-        at = align_up64(at + floats * 4, 256);
+        at = align_up64(at + words * 4, 256);
         return here;
     };
-    l.part1 = take(pieces * (order == 2 ? 7 : 2));
-    l.part2 = take(order == 2 ? pieces * 2 : 0);
+    l.part = take(2 * windows * G * (order == 2 ? 14 : 2));
     l.slots = take(units * 2 * C);
-    l.folded = take(order && units > 128 ? (int64_t)FOLD * 2 * C : 0);
+    l.folded = take(units ? (int64_t)gn::FOLD * 2 * C : 0);
     l.found = take(windows);
+    l.tickets = take(units ? (2 * C + 63) / 64 : 0);
     l.bytes = at;
     return l;
 }
 inline gn::Work work_at(void* ws, const Layout& l, bool params) {
     char* p = (char*)ws;
     gn::Work w;
-    w.part1 = (float*)(p + l.part1), w.part2 = (float*)(p + l.part2), w.slots = params ? (float*)(p + l.slots) : nullptr;
-    w.folded = (float*)(p + l.folded), w.found = (int*)(p + l.found);
+    w.part = (float*)(p + l.part), w.slots = params ? (float*)(p + l.slots) : nullptr, w.folded = (float*)(p + l.folded);
+    w.found = (int*)(p + l.found), w.tickets = (int*)(p + l.tickets);
     return w;
+}
+// one workgroup a column block adds 128 units as fast as it starts; more are shared
+inline gn::Fold fold_for(const gn::Geo& g, void* dw, void* db) {
+    const int n = g.U + g.NW;
+    return gn::Fold{0, n <= 128 ? 1 : std::min(gn::FOLD, n / 32), dw, db};
 }
 
 inline bool aligned16(std::initializer_list<const void*> ps) {
@@ -196,14 +169,22 @@ inline int zero(void* y, const gn::Norm& a, int esize, hipStream_t st) {
     DD3D_CHECK_LAUNCH();
     return 0;
 }
+// parameter gradients of no cloud at all
 inline int zero_params(const gn::Norm& a, void* dw, void* db, hipStream_t st) {
-    if (dw || db) k_fold<<<(unsigned)ceil_div64(2 * a.C, 64), 256, 0, st>>>(nullptr, 0, 0, nullptr, 2 * a.C, 1, nullptr, dw, db, a.C, a.pdt);
+    if (!dw && !db) return 0;
+    k_fold<<<(unsigned)ceil_div64(2 * a.C, 64), 256, 0, st>>>(a, gn::Geo{}, gn::Work{}, gn::Fold{0, 1, dw, db});
     DD3D_CHECK_LAUNCH();
     return 0;
 }
 inline int esize_of(int dtype) { return dtype == DD3D_F32 ? 4 : 2; }
 
 }  // namespace
+
+int gn::launch_fold(const Norm& a, const Plan& p, const Work& w, Fold f, hipStream_t st) {
+    k_fold<<<(unsigned)(p.g.tickets * f.parts), 256, 0, st>>>(a, p.g, w, f);
+    DD3D_CHECK_LAUNCH();
+    return 0;
+}
 
 // See include/dd3d.h.
 DD3D_API int64_t dd3d_group_norm_ws_bytes(int64_t M, int C, int B, int G, int order) {
@@ -249,10 +230,10 @@ DD3D_API int dd3d_group_norm_bwd(const void* dY, const void* X, int dtype, int64
     if (!params && !dX) return 0;
     const gn::Plan q = plan(a, act, esize_of(dtype), aligned16({X, dY, dX}), 2, gn::NR_BWD, params);
     const gn::Work w = work_at(ws, l, params);
-    rc = dtype == DD3D_F32   ? gn::launch_bwd<float>(a, q, dY, X, mean, rstd, dX, w, st)
-         : dtype == DD3D_F16 ? gn::launch_bwd<half_t>(a, q, dY, X, mean, rstd, dX, w, st)
-                             : gn::launch_bwd<bf16_t>(a, q, dY, X, mean, rstd, dX, w, st);
-    return rc || !params ? rc : fold(a, q.g, w, dweight, dbias, st);
+    const gn::Fold f = fold_for(q.g, dweight, dbias);
+    return dtype == DD3D_F32   ? gn::launch_bwd<float>(a, q, dY, X, mean, rstd, dX, w, f, st)
+         : dtype == DD3D_F16 ? gn::launch_bwd<half_t>(a, q, dY, X, mean, rstd, dX, w, f, st)
+                             : gn::launch_bwd<bf16_t>(a, q, dY, X, mean, rstd, dX, w, f, st);
 }
 
 DD3D_API int dd3d_group_norm_bwd2(const void* ggX, const void* ggW, const void* ggB, const void* dY, const void* X, int dtype, int64_t M, int C,
@@ -273,10 +254,10 @@ DD3D_API int dd3d_group_norm_bwd2(const void* ggX, const void* ggW, const void* 
     }
     const bool params = ddweight || ddbias;
     if (!params && !ddY && !ddX) return 0;
-    const gn::Plan q = plan(a, act, esize_of(dtype), aligned16({X, dY, ggX, ddY, ddX}), 7, gn::NR_BWD2, params);
+    const gn::Plan q = plan(a, act, esize_of(dtype), aligned16({X, dY, ggX, ddY, ddX}), act_family(act) == DD3D_FAM_LINEAR ? 7 : 14, NR_STREAM, params);
     const gn::Work w = work_at(ws, l, params);
-    rc = dtype == DD3D_F32   ? gn::launch_bwd2<float>(a, q, ggX, ggW, ggB, dY, X, mean, rstd, ddY, ddX, w, st)
-         : dtype == DD3D_F16 ? gn::launch_bwd2<half_t>(a, q, ggX, ggW, ggB, dY, X, mean, rstd, ddY, ddX, w, st)
-                             : gn::launch_bwd2<bf16_t>(a, q, ggX, ggW, ggB, dY, X, mean, rstd, ddY, ddX, w, st);
-    return rc || !params ? rc : fold(a, q.g, w, ddweight, ddbias, st);
+    const gn::Fold f = fold_for(q.g, ddweight, ddbias);
+    return dtype == DD3D_F32   ? gn::launch_bwd2<float>(a, q, ggX, ggW, ggB, dY, X, mean, rstd, ddY, ddX, w, f, st)
+         : dtype == DD3D_F16 ? gn::launch_bwd2<half_t>(a, q, ggX, ggW, ggB, dY, X, mean, rstd, ddY, ddX, w, f, st)
+                             : gn::launch_bwd2<bf16_t>(a, q, ggX, ggW, ggB, dY, X, mean, rstd, ddY, ddX, w, f, st);
 }

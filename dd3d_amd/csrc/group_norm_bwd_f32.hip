@@ -2,5 +2,5 @@
 #include "group_norm_launch.h"
 
 namespace gn {
-template int launch_bwd<float>(const Norm&, const Plan&, const void*, const void*, const float*, const float*, void*, const Work&, hipStream_t);
+template int launch_bwd<float>(const Norm&, const Plan&, const void*, const void*, const float*, const float*, void*, const Work&, Fold, hipStream_t);
 }  // namespace gn

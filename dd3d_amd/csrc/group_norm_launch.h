@@ -49,12 +49,12 @@ int launch_fwd(const Norm& a, const Plan& p, const void* X, void* Y, float* mean
         if (rc) return rc;
         Geo g = p.g;
         g.units = g.U + g.NW;
-        k_fwd<Z, 0><<<p.blocks0, Z::THREADS, p.lds, st>>>(a, g, (const T*)X, (T*)Y, mean, rstd, w.part1, w.found);
+        k_fwd<Z, 0><<<p.blocks0, Z::THREADS, p.lds, st>>>(a, g, (const T*)X, (T*)Y, mean, rstd, w.part, w.found);
         if (g.NW) {
             rc = set_lds(k_fwd<Z, 1>, p.lds);
             if (rc) return rc;
             g.units = g.NW;
-            k_fwd<Z, 1><<<p.blocks1, Z::THREADS, p.lds, st>>>(a, g, (const T*)X, (T*)Y, mean, rstd, w.part1, w.found);
+            k_fwd<Z, 1><<<p.blocks1, Z::THREADS, p.lds, st>>>(a, g, (const T*)X, (T*)Y, mean, rstd, w.part, w.found);
         }
         DD3D_CHECK_LAUNCH();
         return 0;
@@ -62,49 +62,56 @@ int launch_fwd(const Norm& a, const Plan& p, const void* X, void* Y, float* mean
 }
 
 template <typename T>
-int launch_bwd(const Norm& a, const Plan& p, const void* dY, const void* X, const float* mean, const float* rstd, void* dX, const Work& w, hipStream_t st) {
+int launch_bwd(const Norm& a, const Plan& p, const void* dY, const void* X, const float* mean, const float* rstd, void* dX, const Work& w, Fold f, hipStream_t st) {
     return with_variant<T, NR_BWD[0], NR_BWD[1]>(p, [&](auto tag) {
         typedef typename decltype(tag)::type Z;
         int rc = set_lds(k_bwd<Z, 0>, p.lds);
         if (rc) return rc;
         Geo g = p.g;
         g.units = g.U + g.NW;
-        k_bwd<Z, 0><<<p.blocks0, Z::THREADS, p.lds, st>>>(a, g, (const T*)dY, (const T*)X, mean, rstd, (T*)dX, w.part1, w.found, w.slots);
+        k_bwd<Z, 0><<<p.blocks0, Z::THREADS, p.lds, st>>>(a, g, (const T*)dY, (const T*)X, mean, rstd, (T*)dX, w, f);
         if (g.NW && dX) {
             rc = set_lds(k_bwd<Z, 1>, p.lds);
             if (rc) return rc;
             g.units = g.NW;
-            k_bwd<Z, 1><<<p.blocks1, Z::THREADS, p.lds, st>>>(a, g, (const T*)dY, (const T*)X, mean, rstd, (T*)dX, w.part1, w.found, w.slots);
+            f.first = p.blocks1;
+            k_bwd<Z, 1><<<p.blocks1 + (w.slots ? g.tickets * f.parts : 0), Z::THREADS, p.lds, st>>>(a, g, (const T*)dY, (const T*)X, mean, rstd, (T*)dX, w, f);
+        } else if (w.slots) {
+            return launch_fold(a, p, w, f, st);
         }
         DD3D_CHECK_LAUNCH();
         return 0;
     });
 }
 
+// (the second gradient walks every cloud twice: one size, NR_BWD2[1] rows of wide vectors)
+template <typename T, typename F>
+int with_bwd2(const Plan& p, F f) {
+    if constexpr (sizeof(T) == 2) {
+        if (p.V == 8) return with_family<T, NR_BWD2[1], NR_BWD2[1], 8, true, true>(p, f);
+    }
+    if (!p.al) return with_family<T, NR_BWD2[0], NR_BWD2[0], 4, false, false>(p, f);
+    return p.uni ? with_family<T, NR_BWD2[0], NR_BWD2[0], 4, true, true>(p, f) : with_family<T, NR_BWD2[0], NR_BWD2[0], 4, true, false>(p, f);
+}
+
 template <typename T>
 int launch_bwd2(const Norm& a, const Plan& p, const void* P, const void* ggw, const void* ggb, const void* dY, const void* X, const float* mean, const float* rstd,
-                void* ddY, void* ddX, const Work& w, hipStream_t st) {
-    return with_variant<T, NR_BWD2[0], NR_BWD2[1]>(p, [&](auto tag) {
+                void* ddY, void* ddX, const Work& w, Fold f, hipStream_t st) {
+    return with_bwd2<T>(p, [&](auto tag) {
         typedef typename decltype(tag)::type Z;
-        Geo g = p.g;
-        auto go = [&](auto* kernel, unsigned blocks) {
-            const int rc = set_lds(kernel, p.lds);
-            if (rc) return rc;
-            kernel<<<blocks, Z::THREADS, p.lds, st>>>(a, g, (const T*)P, ggw, ggb, (const T*)dY, (const T*)X, mean, rstd, (T*)ddY, (T*)ddX, w.part1, w.part2, w.found,
-                                                      w.slots);
-            return 0;
-        };
-        g.units = g.U + g.NW;
-        int rc = go(k_bwd2<Z, 0>, p.blocks0);
+        int rc = set_lds(k_bwd2<Z, 0>, p.lds);
         if (rc) return rc;
+        Geo g = p.g;
+        g.units = g.U + g.NW;
+        k_bwd2<Z, 0><<<p.blocks0, Z::THREADS, p.lds, st>>>(a, g, (const T*)P, ggw, ggb, (const T*)dY, (const T*)X, mean, rstd, (T*)ddY, (T*)ddX, w);
         if (g.NW) {
-            g.units = g.NW;
-            if (Z::FAM != DD3D_FAM_LINEAR) rc = go(k_bwd2<Z, 1>, p.blocks1);
-            if (!rc) rc = go(k_bwd2<Z, 2>, p.blocks1);
+            rc = set_lds(k_bwd2<Z, 1>, p.lds);
             if (rc) return rc;
+            g.units = g.NW;
+            k_bwd2<Z, 1><<<p.blocks1, Z::THREADS, p.lds, st>>>(a, g, (const T*)P, ggw, ggb, (const T*)dY, (const T*)X, mean, rstd, (T*)ddY, (T*)ddX, w);
         }
         DD3D_CHECK_LAUNCH();
-        return 0;
+        return w.slots ? launch_fold(a, p, w, f, st) : 0;
     });
 }
 

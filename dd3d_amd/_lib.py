@@ -135,6 +135,32 @@ def stream():
     return torch.cuda.current_stream().cuda_stream
 
 
+def raw_stream(device: torch.device) -> int:
+    """The current stream of ``device`` (which need not be the current device)."""
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+if hasattr(torch._C, "_cuda_getCurrentRawStream"):   # the same number without building a Stream object around it (2 us a call)
+    def raw_stream(device: torch.device) -> int:  # noqa: F811
+        return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+class on_device:
+    """``with on_device(d):`` launches go to ``d``; nothing is done where it is the current device already."""
+
+    def __init__(self, device: torch.device):
+        self.index = device.index
+
+    def __enter__(self):
+        self.prev = torch.cuda.current_device()
+        if self.prev != self.index:
+            torch.cuda.set_device(self.index)
+
+    def __exit__(self, *exc):
+        if self.prev != self.index:
+            torch.cuda.set_device(self.prev)
+
+
 def check(rc: int, name: str):
     if rc == 0:
         return

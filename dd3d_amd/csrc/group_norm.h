@@ -558,19 +558,25 @@ template <int THREADS>
 __device__ __forceinline__ void fold_slots(const Norm& a, const Geo& g, const Work& w, const Fold& f, unsigned block, float* lds) {
     constexpr int WAVES = THREADS / 64;
     const int cols = 2 * a.C, blocks = (cols + 63) / 64, cb = block % blocks, part = block / blocks;
-    const int c = cb * 64 + (threadIdx.x & 63), lane = threadIdx.x >> 6, n = g.U + g.NW;
+    const int c = cb * 64 + (threadIdx.x & 63), lane = threadIdx.x >> 6;
     float t = 0.f;
-    if (c < cols)
+    if (c < cols) {
+        const float* from = w.slots + c;
 #pragma unroll 8
-        for (int i = part + lane * f.parts; i < n; i += WAVES * f.parts)
-            if (i < g.U || w.found[i - g.U]) t += w.slots[(int64_t)i * cols + c];   // (a window without a large cloud has written nothing)
+        for (int i = part + lane * f.parts; i < g.U; i += WAVES * f.parts) t += from[(int64_t)i * cols];
+#pragma unroll 4
+        for (int i = part + lane * f.parts; i < g.NW; i += WAVES * f.parts) {
+            const float v = from[(int64_t)(g.U + i) * cols];   // read in any case: a load behind a branch would wait for the one before it
+            t += w.found[i] ? v : 0.f;                         // (a window without a large cloud has written nothing)
+        }
+    }
     lds[threadIdx.x] = t;
     __syncthreads();
-    if (lane == 0) {
-        for (int i = 1; i < WAVES; ++i) t += lds[threadIdx.x + i * 64];
-        if (f.parts > 1 && c < cols) w.folded[(int64_t)part * cols + c] = t;
-    }
     if (f.parts > 1) {
+        if (lane == 0) {
+            for (int i = 1; i < WAVES; ++i) t += lds[threadIdx.x + i * 64];
+            if (c < cols) w.folded[(int64_t)part * cols + c] = t;
+        }
         __threadfence();
         __syncthreads();
         int* last = (int*)lds + THREADS;
@@ -579,11 +585,14 @@ __device__ __forceinline__ void fold_slots(const Norm& a, const Geo& g, const Wo
         if (!*last) return;
         __threadfence();
         t = 0.f;
-        if (lane == 0 && c < cols)
+        if (c < cols)
 #pragma unroll 8
-            for (int i = 0; i < f.parts; ++i) t += __hip_atomic_load(&w.folded[(int64_t)i * cols + c], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            for (int i = lane; i < f.parts; i += WAVES) t += __hip_atomic_load(&w.folded[(int64_t)i * cols + c], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        lds[threadIdx.x] = t;
+        __syncthreads();
     }
     if (lane || c >= cols) return;
+    for (int i = 1; i < WAVES; ++i) t += lds[threadIdx.x + i * 64];
     void* to = c < a.C ? f.dw : f.db;
     if (to) store_param(to, a.pdt, c < a.C ? c : c - a.C, t);
 }

@@ -12,6 +12,7 @@ buffers (its results carry no graph), while
 """
 from __future__ import annotations
 
+from functools import lru_cache
 from typing import NamedTuple, Optional
 
 import torch
@@ -487,9 +488,9 @@ def random_key(state: torch.Tensor) -> torch.Tensor:
     if state.dtype != torch.int64 or state.numel() != 2 or not state.is_contiguous():
         raise ValueError("the state of a key stream is a contiguous int64 tensor (seed, call)")
     _same_device(state)
-    with torch.cuda.device(state.device):
-        key = torch.empty_like(state)
-        L.call("dd3d_random_key", L.ptr(state), L.ptr(key), L.stream())
+    key = torch.empty_like(state)
+    with L.on_device(state.device):
+        L.call("dd3d_random_key", state.data_ptr(), key.data_ptr(), L.raw_stream(state.device))
     return key
 
 
@@ -498,18 +499,23 @@ class DropoutFn(Function):
 
     @staticmethod
     def forward(ctx, x, p, key):
-        x = _dense(x)
-        y = torch.empty_like(x)
-        C = x.shape[-1] if x.dim() else 1
-        with torch.cuda.device(x.device):
-            L.call("dd3d_dropout", L.ptr(x), _DTYPES[x.dtype], x.numel() // max(C, 1), C, p, L.ptr(key), L.ptr(y), L.stream())
         ctx.save_for_backward(key)
         ctx.p = p
-        return y
+        return _dropout_raw(x, p, key)
 
     @staticmethod
     def backward(ctx, g):
-        return DropoutFn.apply(g, ctx.p, ctx.saved_tensors[0]), None, None
+        key, = ctx.saved_tensors
+        return (DropoutFn.apply(g, ctx.p, key) if torch.is_grad_enabled() else _dropout_raw(g, ctx.p, key)), None, None
+
+
+def _dropout_raw(x, p, key):
+    x = _dense(x)
+    y = torch.empty_like(x)
+    C = x.shape[-1] if x.dim() else 1
+    with L.on_device(x.device):
+        L.call("dd3d_dropout", x.data_ptr(), _DTYPES[x.dtype], x.numel() // max(C, 1), C, p, key.data_ptr(), y.data_ptr(), L.raw_stream(x.device))
+    return y
 
 
 def dropout(x: torch.Tensor, p: float, key: torch.Tensor) -> torch.Tensor:
@@ -520,7 +526,14 @@ def dropout(x: torch.Tensor, p: float, key: torch.Tensor) -> torch.Tensor:
     _rows_dtype(x, "x")
     p = _check_drop(p, key)
     _same_device(x, key=key)
-    return x if p == 0.0 else DropoutFn.apply(x, p, key)
+    if p == 0.0:
+        return x
+    return DropoutFn.apply(x, p, key) if x.requires_grad and torch.is_grad_enabled() else _dropout_raw(x, p, key)
+
+
+@lru_cache(maxsize=4096)
+def _norm_workspace_bytes(M, C, B, G, order):
+    return int(L.lib.dd3d_group_norm_ws_bytes(M, C, B, G, order))
 
 
 class _NormMeta(NamedTuple):
@@ -530,15 +543,22 @@ class _NormMeta(NamedTuple):
     slope: float
     p: float
 
-    def head(self, x, seg_off, w, b):
-        """The arguments the three entry points share, in their order: rows, then the norm's shape and parameters."""
-        pdt = _DTYPES[(w if w is not None else b if b is not None else x).dtype]
-        return (_DTYPES[x.dtype], x.shape[0], x.shape[1], L.ptr(seg_off), seg_off.numel() - 1, self.G, L.ptr(w), L.ptr(b), pdt)
-
-    def workspace(self, x, seg_off, order):
-        n = int(L.lib.dd3d_group_norm_ws_bytes(x.shape[0], x.shape[1], seg_off.numel() - 1, self.G, order))
+    def call(self, name, order, x, seg_off, w, b, key, before, eps, after):
+        """One C entry point: ``before``, the rows and the norm's shape and parameters, ``eps`` (the forward's), ``after``, workspace."""
+        M, C = x.shape
+        B, dev = seg_off.numel() - 1, x.device
+        n = _norm_workspace_bytes(M, C, B, self.G, order)
         # its own block for every call: two graphs captured on one stream may be replayed side by side
-        return torch.empty(n, dtype=torch.uint8, device=x.device) if n > 0 else None
+        ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+        pdt = _DTYPES[(w if w is not None else b if b is not None else x).dtype]
+        with L.on_device(dev):
+            L.call(name, *before, x.data_ptr(), _DTYPES[x.dtype], M, C, seg_off.data_ptr(), B, self.G, _addr(w), _addr(b), pdt, *eps, self.act, self.slope,
+                   self.p, _addr(key), *after, _addr(ws), n, L.raw_stream(dev))
+
+
+def _addr(t):
+    """Device address (None -> NULL) of a tensor that group_norm or dropout has checked."""
+    return None if t is None else t.data_ptr()
 
 
 def _opt_dense(t):
@@ -547,14 +567,25 @@ def _opt_dense(t):
 
 def _norm_fwd(x, w, b, seg_off, key, meta, eps, keep):
     x, w, b = _dense(x), _opt_dense(w), _opt_dense(b)
-    with torch.cuda.device(x.device):
-        y = torch.empty_like(x)
-        stats = torch.empty((2, seg_off.numel() - 1, meta.G), dtype=_F32, device=x.device) if keep else None
-        mean, rstd = (stats[0], stats[1]) if keep else (None, None)
-        ws = meta.workspace(x, seg_off, 0)
-        L.call("dd3d_group_norm_fwd", L.ptr(x), *meta.head(x, seg_off, w, b), eps, meta.act, meta.slope, meta.p, L.ptr(key), L.ptr(y), L.ptr(mean),
-               L.ptr(rstd), L.ptr(ws), 0 if ws is None else ws.numel(), L.stream())
+    y, stats = torch.empty_like(x), None
+    if keep:   # mean and 1 / standard deviation
+        stats = torch.empty((2, seg_off.numel() - 1, meta.G), dtype=_F32, device=x.device)
+    mean = _addr(stats)
+    rstd = mean + 4 * (stats.numel() // 2) if mean else None
+    meta.call("dd3d_group_norm_fwd", 0, x, seg_off, w, b, key, (), (eps,), (y.data_ptr(), mean or None, rstd))
     return y, stats
+
+
+def _stats(stats):
+    at = stats.data_ptr()
+    return (at, at + 4 * (stats.numel() // 2)) if at else (None, None)
+
+
+def _norm_grad(dy, x, w, b, seg_off, key, stats, meta, need):
+    dy, x, w, b = _dense(dy), _dense(x), _opt_dense(w), _opt_dense(b)
+    dx, dw, db = (torch.empty_like(t) if n else None for t, n in zip((x, w, b), need))
+    meta.call("dd3d_group_norm_bwd", 1, x, seg_off, w, b, key, (dy.data_ptr(),), (), (*_stats(stats), _addr(dx), _addr(dw), _addr(db)))
+    return dx, dw, db
 
 
 class GroupNormFn(Function):
@@ -570,8 +601,8 @@ class GroupNormFn(Function):
     @staticmethod
     def backward(ctx, dy):
         x, w, b, seg_off, key, stats = ctx.saved_tensors
-        dx, dw, db = _GroupNormGradFn.apply(dy, x, w, b, seg_off, key, stats, ctx.meta, ctx.needs_input_grad[:3])
-        return dx, dw, db, None, None, None, None
+        grad = _GroupNormGradFn.apply if torch.is_grad_enabled() else _norm_grad
+        return (*grad(dy, x, w, b, seg_off, key, stats, ctx.meta, ctx.needs_input_grad[:3]), None, None, None, None)
 
 
 class _GroupNormGradFn(Function):
@@ -582,32 +613,17 @@ class _GroupNormGradFn(Function):
         ctx.save_for_backward(dy, x, w, b, seg_off, key, stats)
         ctx.meta = meta
         ctx.set_materialize_grads(False)
-        dy, x, w, b = _dense(dy), _dense(x), _opt_dense(w), _opt_dense(b)
-        with torch.cuda.device(x.device):
-            dx = torch.empty_like(x) if need[0] else None
-            dw = torch.empty_like(w) if need[1] else None
-            db = torch.empty_like(b) if need[2] else None
-            ws = meta.workspace(x, seg_off, 1)
-            L.call("dd3d_group_norm_bwd", L.ptr(dy), L.ptr(x), *meta.head(x, seg_off, w, b), meta.act, meta.slope, meta.p, L.ptr(key), L.ptr(stats[0]),
-                   L.ptr(stats[1]), L.ptr(dx), L.ptr(dw), L.ptr(db), L.ptr(ws), 0 if ws is None else ws.numel(), L.stream())
-        return dx, dw, db
+        return _norm_grad(dy, x, w, b, seg_off, key, stats, meta, need)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, ggx, ggw, ggb):
         dy, x, w, b, seg_off, key, stats = ctx.saved_tensors
-        meta, need = ctx.meta, ctx.needs_input_grad
         dy, x, w, b, ggx, ggw, ggb = _dense(dy), _dense(x), *(_opt_dense(t) for t in (w, b, ggx, ggw, ggb))
-        with torch.cuda.device(x.device):
-            ddy = torch.empty_like(dy) if need[0] else None
-            ddx = torch.empty_like(x) if need[1] else None
-            ddw = torch.empty_like(w) if need[2] else None
-            ddb = torch.empty_like(b) if need[3] else None
-            ws = meta.workspace(x, seg_off, 2)
-            L.call("dd3d_group_norm_bwd2", L.ptr(ggx), L.ptr(ggw), L.ptr(ggb), L.ptr(dy), L.ptr(x), *meta.head(x, seg_off, w, b), meta.act, meta.slope,
-                   meta.p, L.ptr(key), L.ptr(stats[0]), L.ptr(stats[1]), L.ptr(ddy), L.ptr(ddx), L.ptr(ddw), L.ptr(ddb), L.ptr(ws),
-                   0 if ws is None else ws.numel(), L.stream())
-        return ddy, ddx, ddw, ddb, None, None, None, None, None
+        out = [torch.empty_like(t) if n else None for t, n in zip((dy, x, w, b), ctx.needs_input_grad)]
+        ctx.meta.call("dd3d_group_norm_bwd2", 2, x, seg_off, w, b, key, (_addr(ggx), _addr(ggw), _addr(ggb), dy.data_ptr()), (),
+                      (*_stats(stats), *(_addr(t) for t in out)))
+        return (*out, None, None, None, None, None)
 
 
 def group_norm(x: torch.Tensor, seg_off: torch.Tensor, num_groups: int, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,

@@ -145,22 +145,6 @@ if hasattr(torch._C, "_cuda_getCurrentRawStream"):   # the same number without b
         return torch._C._cuda_getCurrentRawStream(device.index)
 
 
-class on_device:
-    """``with on_device(d):`` launches go to ``d``; nothing is done where it is the current device already."""
-
-    def __init__(self, device: torch.device):
-        self.index = device.index
-
-    def __enter__(self):
-        self.prev = torch.cuda.current_device()
-        if self.prev != self.index:
-            torch.cuda.set_device(self.index)
-
-    def __exit__(self, *exc):
-        if self.prev != self.index:
-            torch.cuda.set_device(self.prev)
-
-
 def check(rc: int, name: str):
     if rc == 0:
         return

@@ -84,8 +84,24 @@ __device__ __forceinline__ void normal_cdf_pdf(float u, float* cdf, float* pdf) 
     *pdf = e * 0.39894228f;
 }
 
+// The same Phi for results that are rounded to half width: a polynomial of degree 5 over t = 1 / (1 + 0.3 a), relative error 8.2e-6, a
+// sixtieth of fp16's half step.
+__device__ __forceinline__ float normal_cdf_short(float u) {
+    const float a = fabsf(u), t = __builtin_amdgcn_rcpf(fmaf(0.3f, a, 1.f));
+    const float e = __builtin_amdgcn_exp2f(u * u * -0.72134752f);
+    float p = -0.07709760218858719f;
+    p = fmaf(p, t, 0.21603752672672272f);
+    p = fmaf(p, t, -0.016948513686656952f);
+    p = fmaf(p, t, 0.14419656991958618f);
+    p = fmaf(p, t, 0.11374188959598541f);
+    p = fmaf(p, t, 0.12007423490285873f);
+    const float q = e * (p * t);
+    return u < 0.f ? q : 1.f - q;
+}
+
 // phi(u); with ORDER >= 1 also phi'(u) in *d1, with ORDER == 2 phi''(u) in *d2
-template <int FAM, int ORDER>
+// SHORT: the value alone, to be rounded to half width
+template <int FAM, int ORDER, bool SHORT = false>
 __device__ __forceinline__ float activate(float u, float slope, float* d1, float* d2) {
     if (FAM == DD3D_FAM_LINEAR) {
         const bool up = u > 0.f;
@@ -101,6 +117,7 @@ __device__ __forceinline__ float activate(float u, float slope, float* d1, float
         if (ORDER == 2) *d2 = ds * fmaf(u, 1.f - 2.f * s, 2.f);
         return u * s;
     }
+    if (SHORT && ORDER == 0) return u * normal_cdf_short(u);
     float cdf, pdf;
     normal_cdf_pdf(u, &cdf, &pdf);
     if (ORDER >= 1) *d1 = fmaf(u, pdf, cdf);

@@ -37,14 +37,13 @@ __device__ __forceinline__ int quot(int n, const Div& d) { return d.d == 1 ? n :
 struct Geo {
     int k, nslab;        // groups per slab, slabs
     int CL, RL, lcl;     // channel lanes (vectors per row of the slab), row lanes, log2(CL) if CL is a power of two <= 64, else -1
-    int fast;            // groups and slabs are powers of two of lanes: sums by shuffles
-    int cw;              // columns of one group: vectors where a vector lies inside one group, else channels
+    int cw;              // columns of one group (a column: the channels of a vector that share a statistic)
+    int fast;            // slabs, and groups wider than a vector, are powers of two of lanes: sums by lane exchanges
     int U, NW, CH, Tl;   // cloud units, windows, rows per window, longest cloud that one workgroup takes
     int units;           // of this launch
     int quads;           // ceil(C / 4)
     int kb;              // quantities reduced at once where the sums go through LDS
     int red;             // floats of LDS for them
-    int tickets;         // column blocks of the parameter gradients
     Div dCL, dCg;
 };
 
@@ -108,19 +107,21 @@ __device__ __forceinline__ void store_row(T* p, const float (&v)[V], int lo, int
 }
 
 // ---- where this thread stands ---------------------------------------------------------------------------------------------------
-// The compile-time side of a launch.  UNI: every vector lies inside one group (Cg % V == 0), so a thread has one set of statistics;
-// otherwise its channels may belong to up to four groups.  AL: whole, aligned vectors.
-// Vectors a thread holds in the three passes, in the variants for short (first) and long clouds, and the waves per SIMD that the
-// registers of that many rows leave.
-constexpr int NR_FWD[2] = {8, 16}, NR_BWD[2] = {8, 16}, NR_BWD2[2] = {4, 2};
+// The compile-time side of a launch.  NS: statistics a vector needs -- 1 where it lies inside one group (Cg % V == 0), 2 where it holds two
+// groups of four, else one per channel.  AL: whole, aligned vectors.
+// Vectors a thread holds in the three passes: vectors of four in the variants for short and for long clouds, vectors of eight; and the
+// waves per SIMD that the registers of that many rows leave.
+constexpr int NR_FWD[3] = {8, 16, 8}, NR_BWD[3] = {8, 16, 4}, NR_BWD2[3] = {4, 4, 2};
 
-template <typename T_, int V_, bool AL_, bool UNI_, int FAM_, int THREADS_, int NR_>
+template <typename T_, int V_, bool AL_, int NS_, int FAM_, int THREADS_, int NR_>
 struct Cfg {
     typedef T_ T;
-    static constexpr int V = V_, FAM = FAM_, THREADS = THREADS_, NR = NR_, NS = UNI_ ? 1 : V_, WAVES = THREADS_ / 64;
-    static constexpr bool AL = AL_, UNI = UNI_;
-    static constexpr int FWD_WAVES = THREADS_ > 256 || NR_ <= 8 ? 4 : 3, BWD_WAVES = THREADS_ > 256 ? 4 : NR_ > 8 ? 2 : 3, BWD2_WAVES = THREADS_ > 256 ? 4 : UNI_ ? 3 : 2;
-    static constexpr int at(int i) { return UNI_ ? 0 : i; }
+    static constexpr int V = V_, FAM = FAM_, THREADS = THREADS_, NR = NR_, NS = NS_, WAVES = THREADS_ / 64;
+    static constexpr int PER = V_ / NS_;   // channels that share a statistic
+    static constexpr bool AL = AL_;
+    static constexpr int FWD_WAVES = THREADS_ > 256 || NR_ <= 8 ? 4 : 3, BWD_WAVES = THREADS_ > 256 ? 4 : NR_ > 8 ? 2 : 3,
+                         BWD2_WAVES = THREADS_ > 256 ? 4 : NS_ == 1 ? 3 : 2;
+    static constexpr int at(int i) { return i / PER; }
     typedef Raw<T_, V_> Row;
 };
 
@@ -159,8 +160,8 @@ __device__ __forceinline__ void load_params(const void* p, int pdt, int c0, int 
 
 // consecutive workgroups go to consecutive XCDs: the slabs of one unit are eight workgroups apart, on one XCD, so lines that two slabs
 // share are fetched into one L2
-__device__ __forceinline__ bool place(const Geo& g, int& unit, int& slab) {
-    const int lo = blockIdx.x & 7, rest = blockIdx.x >> 3, hi = g.nslab == 1 ? rest : rest / g.nslab;
+__device__ __forceinline__ bool place(const Geo& g, int& unit, int& slab, unsigned first = 0) {
+    const int at = blockIdx.x - first, lo = at & 7, rest = at >> 3, hi = g.nslab == 1 ? rest : rest / g.nslab;
     slab = rest - hi * g.nslab;
     unit = hi * 8 + lo;
     return unit < g.units;
@@ -182,7 +183,7 @@ __device__ __forceinline__ void locate(const Norm& a, const Geo& g, int unit, in
     s.off = s.rl * a.C + s.cc, s.step = g.RL * a.C;
     s.word = s.rl * g.quads + s.c0 / 4;
 #pragma unroll
-    for (int i = 0; i < Z::NS; ++i) s.j[i] = min(quot(max(s.c0 + i - s.s0, 0), g.dCg), s.gs - 1);
+    for (int i = 0; i < Z::NS; ++i) s.j[i] = min(quot(max(s.c0 + i * Z::PER - s.s0, 0), g.dCg), s.gs - 1);
     load_params<Z::V>(a.W, a.pdt, s.c0, s.s0, s.s1, 1.f, s.w);
     load_params<Z::V>(a.Bi, a.pdt, s.c0, s.s0, s.s1, 0.f, s.b);
 }
@@ -340,34 +341,37 @@ __device__ __forceinline__ void add_strided(float (&v)[K], int n) {
 }
 
 // ---- sums -----------------------------------------------------------------------------------------------------------------------
-// v[q][i], per thread and (with !UNI) channel -> the sum over the rows of the workgroup and the channels of the group that thread and channel
-// belong to.  Lanes without rows bring zeros.
+// v[q][i], per thread and statistic -> the sum over the rows of the workgroup and the channels of the group that the statistic belongs to.  Lanes without rows bring zeros.
 template <int K, typename Z>
 __device__ __forceinline__ void group_sums(float (&v)[K][Z::NS], const Norm& a, const Geo& g, Spot<Z>& s, float* lds) {
-    if (Z::UNI && g.fast) {
+    constexpr int NS = Z::NS;
+    if (g.fast) {
         // the group's lanes, then the wave's row lanes; one value per wave and group through LDS.  Two buffers in turn: one barrier a call
-        float t[K];
+        float t[K * NS];
 #pragma unroll
-        for (int q = 0; q < K; ++q) t[q] = v[q][0];
-        add_block(t, g.cw);
+        for (int q = 0; q < K * NS; ++q) t[q] = v[q / NS][q % NS];
+        if (NS == 1) add_block(t, g.cw);
         add_strided(t, g.CL);
         float* red = lds + s.buf * (g.red >> 1);   // (a fixed half: calls of different K follow each other)
         s.buf ^= 1;
-        if (s.lane < g.CL && (s.lane & (g.cw - 1)) == 0 && s.hi > 0) {
+        if (s.lane < g.CL && (NS > 1 || (s.lane & (g.cw - 1)) == 0) && s.hi > 0) {
 #pragma unroll
-            for (int q = 0; q < K; ++q) red[(q * Z::WAVES + s.wave) * g.k + s.j[0]] = t[q];
+            for (int q = 0; q < K * NS; ++q)
+                if (NS == 1 || q % NS * Z::PER < s.hi) red[(q / NS * Z::WAVES + s.wave) * g.k + s.j[q % NS]] = t[q];
         }
         __syncthreads();
 #pragma unroll
-        for (int q = 0; q < K; ++q) {
-            v[q][0] = 0.f;
+        for (int q = 0; q < K; ++q)
 #pragma unroll
-            for (int p = 0; p < Z::WAVES; ++p) v[q][0] += red[(q * Z::WAVES + p) * g.k + s.j[0]];
-        }
+            for (int i = 0; i < NS; ++i) {
+                v[q][i] = 0.f;
+#pragma unroll
+                for (int p = 0; p < Z::WAVES; ++p) v[q][i] += red[(q * Z::WAVES + p) * g.k + s.j[i]];
+            }
         return;
     }
     // through LDS: [row lane][column], summed per column, then per group
-    const int cols = g.CL * Z::NS, c_first = Z::UNI ? 0 : s.s0 & 3;   // the slab's first column
+    const int cols = g.CL * NS, c_first = (s.s0 & 3) / Z::PER;   // the slab's first column
     float *tot = lds + g.red, *out = tot + g.kb * cols;
     for (int k0 = 0; k0 < K; k0 += g.kb) {
         const int kn = min(K - k0, g.kb);
@@ -440,10 +444,11 @@ __device__ __forceinline__ void column_sums(float (&acc)[K][Z::V], const Norm& a
     }
 }
 
-// part[slot][G][K]: this thread's channel that writes for its group
+// part[slot][G][K]: whether this thread's i-th statistic is the one that is written for its group
 template <typename Z>
 __device__ __forceinline__ bool writes_group(const Norm& a, const Spot<Z>& s, int i) {
-    return s.rl == 0 && s.on && i >= s.lo && i < s.hi && s.j[i] * a.Cg == s.c0 + i - s.s0;
+    const int c = i * Z::PER;
+    return s.rl == 0 && s.on && c >= s.lo && c < s.hi && s.j[i] * a.Cg == s.c0 + c - s.s0;
 }
 template <int K, typename Z>
 __device__ __forceinline__ void put_part(float* part, int slot, const float (&v)[K][Z::NS], const Norm& a, const Geo& g, const Spot<Z>& s) {
@@ -535,66 +540,39 @@ __device__ __forceinline__ void row_border() { __builtin_amdgcn_sched_barrier(0)
 
 // ---- the caller's workspace, and the parameter gradients in it --------------------------------------------------------------------
 struct Work {
-    float *part, *slots, *folded;   // pieces' sums; [units][2][C]; [FOLD][2][C]
-    int *found, *tickets;           // pieces per window; arrivals per column block
+    float *part, *slots;   // pieces' sums; [units][2][C]
+    int* found;            // pieces per window
 };
-constexpr int FOLD = 32;            // workgroups that share a block of 64 columns
-
-// where the folding workgroups of a launch begin, and what they write
 struct Fold {
-    unsigned first;
-    int parts;
+    unsigned blocks;       // workgroups (8 columns each) in front of the windows' launch
     void *dw, *db;
 };
 
-__device__ __forceinline__ void clear_tickets(const Geo& g, const Work& w) {
-    if (blockIdx.x == 0 && w.slots)
-        for (int i = threadIdx.x; i < g.tickets; i += blockDim.x) w.tickets[i] = 0;
-}
-
-// out[q][c] = the sum over units of slots[unit][q][c]: workgroup (column block, part) adds every parts-th unit, a thread a column and every
-// WAVES-th of those; the last of a column block to arrive adds the parts, in part order, so the result does not depend on who is last.
+// out[q][c] = the sum over units of slots[unit][q][c] in a fixed order: eight columns a workgroup, THREADS / 8 row lanes, sixteen loads in
+// flight a thread (latency is all there is to hide: 1300 units of 128 channels are 1.3 MB).
 template <int THREADS>
-__device__ __forceinline__ void fold_slots(const Norm& a, const Geo& g, const Work& w, const Fold& f, unsigned block, float* lds) {
-    constexpr int WAVES = THREADS / 64;
-    const int cols = 2 * a.C, blocks = (cols + 63) / 64, cb = block % blocks, part = block / blocks;
-    const int c = cb * 64 + (threadIdx.x & 63), lane = threadIdx.x >> 6;
+__device__ __forceinline__ void fold_slots(const Norm& a, const Geo& g, const Work& w, const Fold& f, float* lds) {
+    constexpr int LANES = THREADS / 8;
+    const int cols = 2 * a.C, c = blockIdx.x * 8 + (threadIdx.x & 7), lane = threadIdx.x >> 3;
     float t = 0.f;
     if (c < cols) {
         const float* from = w.slots + c;
+#pragma unroll 16
+        for (int i = lane; i < g.U; i += LANES) t += from[(int64_t)i * cols];
 #pragma unroll 8
-        for (int i = part + lane * f.parts; i < g.U; i += WAVES * f.parts) t += from[(int64_t)i * cols];
-#pragma unroll 4
-        for (int i = part + lane * f.parts; i < g.NW; i += WAVES * f.parts) {
+        for (int i = lane; i < g.NW; i += LANES) {
             const float v = from[(int64_t)(g.U + i) * cols];   // read in any case: a load behind a branch would wait for the one before it
             t += w.found[i] ? v : 0.f;                         // (a window without a large cloud has written nothing)
         }
     }
     lds[threadIdx.x] = t;
-    __syncthreads();
-    if (f.parts > 1) {
-        if (lane == 0) {
-            for (int i = 1; i < WAVES; ++i) t += lds[threadIdx.x + i * 64];
-            if (c < cols) w.folded[(int64_t)part * cols + c] = t;
-        }
-        __threadfence();
+    for (int n = LANES / 2; n > 0; n >>= 1) {
         __syncthreads();
-        int* last = (int*)lds + THREADS;
-        if (threadIdx.x == 0) *last = atomicAdd(&w.tickets[cb], 1) == f.parts - 1;
-        __syncthreads();
-        if (!*last) return;
-        __threadfence();
-        t = 0.f;
-        if (c < cols)
-#pragma unroll 8
-            for (int i = lane; i < f.parts; i += WAVES) t += __hip_atomic_load(&w.folded[(int64_t)i * cols + c], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        lds[threadIdx.x] = t;
-        __syncthreads();
+        if (lane < n) lds[threadIdx.x] += lds[threadIdx.x + n * 8];
     }
     if (lane || c >= cols) return;
-    for (int i = 1; i < WAVES; ++i) t += lds[threadIdx.x + i * 64];
     void* to = c < a.C ? f.dw : f.db;
-    if (to) store_param(to, a.pdt, c < a.C ? c : c - a.C, t);
+    if (to) store_param(to, a.pdt, c < a.C ? c : c - a.C, lds[threadIdx.x]);
 }
 
 // ---- forward --------------------------------------------------------------------------------------------------------------------
@@ -727,7 +705,7 @@ struct Fwd {
             const typename Z::Row x = again(z[n]);
 #pragma unroll
             for (int i = 0; i < V; ++i)
-                y[i] = activate<Z::FAM, 0>(fmaf((raw_get(x, i) - mean[Z::at(i)]) * rstd[Z::at(i)], s.w[i], s.b[i]), a.slope, &d1, &d2);
+                y[i] = activate<Z::FAM, 0, sizeof(T) == 2>(fmaf((raw_get(x, i) - mean[Z::at(i)]) * rstd[Z::at(i)], s.w[i], s.b[i]), a.slope, &d1, &d2);
             if (a.drop.key) {
                 drop_row<V>(a.drop, keep_bits<V>(a.drop, key, words + (word + n * (uint32_t)(g.RL * g.quads))), y);
             }
@@ -965,13 +943,12 @@ __global__ __launch_bounds__(Z::THREADS, Z::BWD_WAVES) void k_bwd(Norm a, Geo g,
     extern __shared__ __align__(16) float lds[];
     if (MODE == 0) {
         zero_rest(a, dX);
-        clear_tickets(g, w);
-    } else if (blockIdx.x >= fold.first) {   // the windows' launch brings the parameter gradients along
-        fold_slots<Z::THREADS>(a, g, w, fold, blockIdx.x - fold.first, lds);
+    } else if (blockIdx.x < fold.blocks) {   // the windows' launch brings the parameter gradients along
+        fold_slots<Z::THREADS>(a, g, w, fold, lds);
         return;
     }
     int unit, slab;
-    if (!place(g, unit, slab)) return;
+    if (!place(g, unit, slab, MODE == 0 ? 0 : fold.blocks)) return;
     const bool whole = MODE == 0 && unit < g.U;
     Piece p[2];
     const int np = whole ? 0 : window_pieces<MODE == 0>(a, g, unit - (MODE == 0 ? g.U : 0), w.found, p);
@@ -1216,7 +1193,6 @@ __global__ __launch_bounds__(Z::THREADS, Z::BWD2_WAVES) void k_bwd2(Norm a, Geo 
     if (MODE == 0) {
         zero_rest(a, ddY);
         zero_rest(a, ddX);
-        clear_tickets(g, w);
     }
     int unit, slab;
     if (!place(g, unit, slab)) return;
@@ -1270,7 +1246,8 @@ __global__ __launch_bounds__(Z::THREADS, Z::BWD2_WAVES) void k_bwd2(Norm a, Geo 
 struct Plan {
     Geo g;
     int V, fam, size;            // size: 0 few rows a thread, 1 many, 2 sixteen waves (slabs of more than 256 vectors)
-    bool al, uni;
+    bool al;
+    int ns;
     unsigned blocks0, blocks1;   // workgroups of the first launch and of the windows' launches
     size_t lds;
 };

@@ -24,9 +24,9 @@ __global__ void k_zero_half(uint16_t* y, int64_t n) {
     if (threadIdx.x == 0 && n > 0) y[n - 1] = 0;   // the odd last element of a half-width matrix
 }
 
-__global__ __launch_bounds__(256) void k_fold(gn::Norm a, gn::Geo g, gn::Work w, gn::Fold f) {
-    __shared__ float lds[256 + 1];
-    gn::fold_slots<256>(a, g, w, f, blockIdx.x, lds);
+__global__ __launch_bounds__(1024) void k_fold(gn::Norm a, gn::Geo g, gn::Work w, gn::Fold f) {
+    __shared__ float lds[1024];
+    gn::fold_slots<1024>(a, g, w, f, lds);
 }
 
 // ---- launch geometry --------------------------------------------------------------------------------------------------------------
@@ -47,15 +47,15 @@ inline gn::Div divide_by(int d) {
 inline int cloud_units(int B, bool params) { return params && B > MAX_UNITS ? (int)ceil_div64(B, ceil_div64(B, MAX_UNITS)) : B; }
 
 // sums: quantities summed at once; nr: vectors a thread holds in the variants for short and long clouds; params: column_sums is called
-constexpr int NR_STREAM[2] = {16, 16};
-inline gn::Plan plan(const gn::Norm& a, int act, int esize, bool aligned, int sums, const int (&nr)[2], bool params) {
+constexpr int NR_STREAM[3] = {16, 16, 16};   // the second gradient walks every cloud twice whatever its length: chunks do not matter
+inline gn::Plan plan(const gn::Norm& a, int act, int esize, bool aligned, int sums, const int (&nr)[3], bool params) {
     gn::Plan p;
     gn::Geo& g = p.g;
     p.fam = act_family(act);
-    p.V = esize == 2 && aligned && a.Cg % 8 == 0 && a.Cg <= 2048 ? 8 : 4;
-    const int m0 = 4 / gcd(a.Cg, 4);   // groups whose channels fill whole vectors of four
+    p.V = esize == 2 && aligned && a.C % 8 == 0 && ((a.Cg % 8 == 0 && a.Cg <= 2048) || a.Cg == 4) ? 8 : 4;
+    const int m0 = p.V / gcd(a.Cg, p.V);   // groups whose channels fill whole vectors
     p.al = aligned && a.C % p.V == 0 && m0 * a.Cg <= 4096;
-    p.uni = p.al && a.Cg % p.V == 0;
+    p.ns = p.al && a.Cg % p.V == 0 ? 1 : p.V == 8 ? 2 : 4;
     auto lanes = [&](int k) { return p.al || k >= a.G || k * a.Cg % 4 == 0 ? (k * a.Cg + p.V - 1) / p.V : (k * a.Cg + 6) / 4; };
     auto whole = [&](int k) { return k >= a.G ? a.G : p.al ? std::min(a.G, (k + m0 - 1) / m0 * m0) : k; };
     // Slab width: 64 bytes of a row at least (its neighbour reads the other half of the line into the same L2), doubled while a short
@@ -63,16 +63,16 @@ inline gn::Plan plan(const gn::Norm& a, int act, int esize, bool aligned, int su
     // bytes: 2560 clouds of 82 rows 106 / 65 / 52 / 58, 100 of 216 rows 13.7 / 15.3 / 19.8 / 28.7, 400 of 750 rows (long variant)
     // 87 / 96 / 112 / 123.
     const int kmin = whole((64 / esize + a.Cg - 1) / a.Cg);
-    const int64_t mean = a.B ? a.M / a.B : 0;
+    const int64_t mean = a.B ? a.M / a.B : 0, shorter = nr[p.V == 8 ? 2 : 0];   // rows a thread holds, short variant
     int k = kmin;
     p.size = 0;
     if (lanes(kmin) > 256) {
         p.size = 2;
     } else {
-        for (int w = whole(2 * k); k < a.G && lanes(w) <= 64 && (int64_t)nr[0] * (256 / lanes(w)) >= mean && (int64_t)a.B * ((a.G + w - 1) / w) >= 1024; w = whole(2 * k)) k = w;
-        if (p.uni && p.V == 4 && (int64_t)nr[0] * (256 / lanes(kmin)) < mean) p.size = 1;
+        for (int w = whole(2 * k); k < a.G && lanes(w) <= 64 && shorter * (256 / lanes(w)) >= mean && (int64_t)a.B * ((a.G + w - 1) / w) >= 1024; w = whole(2 * k)) k = w;
+        if (p.ns == 1 && p.V == 4 && shorter * (256 / lanes(kmin)) < mean) p.size = 1;
     }
-    if (getenv("GN_T")) p.size = p.uni && p.V == 4 ? atoi(getenv("GN_T")) : 0;
+    if (getenv("GN_T")) p.size = p.ns == 1 && p.V == 4 ? atoi(getenv("GN_T")) : 0;
     if (getenv("GN_W")) k = whole(std::max(1, atoi(getenv("GN_W")) / a.Cg));
     const int threads = p.size == 2 ? 1024 : 256;
     g.k = k;
@@ -82,34 +82,32 @@ inline gn::Plan plan(const gn::Norm& a, int act, int esize, bool aligned, int su
     g.lcl = -1;
     for (int i = 0; i <= 6; ++i)
         if (g.CL == 1 << i) g.lcl = i;
-    g.cw = p.uni ? a.Cg / p.V : a.Cg;
-    g.fast = p.uni && g.lcl >= 0 && (g.cw & (g.cw - 1)) == 0;
+    g.cw = std::max(1, a.Cg * p.ns / p.V);
+    g.fast = p.al && g.lcl >= 0 && (p.ns == 1 ? (g.cw & (g.cw - 1)) == 0 : g.cw == 1);
     g.quads = (a.C + 3) / 4;
     g.dCL = divide_by(g.CL), g.dCg = divide_by(a.Cg);
-    const int64_t cap = (int64_t)nr[p.size == 1] * g.RL;   // rows of a chunk
+    const int64_t cap = (p.size == 1 ? nr[1] : shorter) * g.RL;   // rows of a chunk
     g.NW = (int)std::min<int64_t>(ceil_div64(a.M, MIN_WINDOW), max_windows(a.C));
     g.CH = g.NW ? (int)ceil_div64(a.M, g.NW) : 1;
     g.Tl = (int)std::max<int64_t>(2 * cap, g.CH);
     g.NW = a.M <= g.Tl ? 0 : (int)ceil_div64(a.M, g.CH);
     g.U = cloud_units(a.B, params);
     g.units = 0;
-    g.tickets = params ? (2 * a.C + 63) / 64 : 0;
     p.blocks0 = (unsigned)(align_up64((int64_t)g.U + g.NW, 8) * g.nslab);
     p.blocks1 = (unsigned)(align_up64(g.NW, 8) * g.nslab);
     // LDS: row partials of kb quantities (or two buffers of the waves' sums, or the columns of one parameter gradient), the columns' totals
     // of kb quantities, the groups' sums of all
-    const int ns = p.uni ? 1 : p.V, cols = g.CL * ns;
+    const int cols = g.CL * p.ns;
     g.kb = std::max(1, std::min(sums, 8192 / (g.RL * cols)));
     g.red = g.fast ? 2 * sums * (threads / 64) * g.k : g.kb * g.RL * cols;
     if (params) g.red = std::max(g.red, (g.lcl >= 0 ? threads / 64 : g.RL) * g.CL * p.V);
-    p.lds = sizeof(float) * std::max<size_t>((size_t)g.red + g.kb * cols + sums * g.k, params ? threads + 1 : 0);
+    p.lds = sizeof(float) * std::max<size_t>((size_t)g.red + g.kb * cols + sums * g.k, params ? threads : 0);
     return p;
 }
 
-// The workspace: piece sums, units' slots and their folded sums, pieces per window, tickets.  Sized by bounds that hold for every type and
-// alignment.
+// The workspace: piece sums, units' slots, pieces per window.  Sized by bounds that hold for every type and alignment.
 struct Layout {
-    int64_t part, slots, folded, found, tickets, bytes;
+    int64_t part, slots, found, bytes;
 };
 inline Layout layout(int64_t M, int C, int B, int G, int order) {
     const int64_t windows = M > MIN_WINDOW ? std::min<int64_t>(ceil_div64(M, MIN_WINDOW), max_windows(C)) : 0;
@@ -123,24 +121,17 @@ inline Layout layout(int64_t M, int C, int B, int G, int order) {
     };
     l.part = take(2 * windows * G * (order == 2 ? 14 : 2));
     l.slots = take(units * 2 * C);
-    l.folded = take(units ? (int64_t)gn::FOLD * 2 * C : 0);
     l.found = take(windows);
-    l.tickets = take(units ? (2 * C + 63) / 64 : 0);
     l.bytes = at;
     return l;
 }
 inline gn::Work work_at(void* ws, const Layout& l, bool params) {
     char* p = (char*)ws;
     gn::Work w;
-    w.part = (float*)(p + l.part), w.slots = params ? (float*)(p + l.slots) : nullptr, w.folded = (float*)(p + l.folded);
-    w.found = (int*)(p + l.found), w.tickets = (int*)(p + l.tickets);
+    w.part = (float*)(p + l.part), w.slots = params ? (float*)(p + l.slots) : nullptr, w.found = (int*)(p + l.found);
     return w;
 }
-// one workgroup a column block adds 128 units as fast as it starts; more are shared
-inline gn::Fold fold_for(const gn::Geo& g, void* dw, void* db) {
-    const int n = g.U + g.NW;
-    return gn::Fold{0, n <= 128 ? 1 : std::min(gn::FOLD, n / 32), dw, db};
-}
+inline gn::Fold fold_for(const gn::Norm& a, void* dw, void* db) { return gn::Fold{(unsigned)ceil_div64(2 * a.C, 8), dw, db}; }
 
 inline bool aligned16(std::initializer_list<const void*> ps) {
     uintptr_t m = 0;
@@ -172,7 +163,8 @@ inline int zero(void* y, const gn::Norm& a, int esize, hipStream_t st) {
 // parameter gradients of no cloud at all
 inline int zero_params(const gn::Norm& a, void* dw, void* db, hipStream_t st) {
     if (!dw && !db) return 0;
-    k_fold<<<(unsigned)ceil_div64(2 * a.C, 64), 256, 0, st>>>(a, gn::Geo{}, gn::Work{}, gn::Fold{0, 1, dw, db});
+    const gn::Fold f = fold_for(a, dw, db);
+    k_fold<<<f.blocks, 1024, 0, st>>>(a, gn::Geo{}, gn::Work{}, f);
     DD3D_CHECK_LAUNCH();
     return 0;
 }
@@ -181,7 +173,7 @@ inline int esize_of(int dtype) { return dtype == DD3D_F32 ? 4 : 2; }
 }  // namespace
 
 int gn::launch_fold(const Norm& a, const Plan& p, const Work& w, Fold f, hipStream_t st) {
-    k_fold<<<(unsigned)(p.g.tickets * f.parts), 256, 0, st>>>(a, p.g, w, f);
+    k_fold<<<f.blocks, 1024, 0, st>>>(a, p.g, w, f);
     DD3D_CHECK_LAUNCH();
     return 0;
 }
@@ -230,7 +222,7 @@ DD3D_API int dd3d_group_norm_bwd(const void* dY, const void* X, int dtype, int64
     if (!params && !dX) return 0;
     const gn::Plan q = plan(a, act, esize_of(dtype), aligned16({X, dY, dX}), 2, gn::NR_BWD, params);
     const gn::Work w = work_at(ws, l, params);
-    const gn::Fold f = fold_for(q.g, dweight, dbias);
+    const gn::Fold f = fold_for(a, dweight, dbias);
     return dtype == DD3D_F32   ? gn::launch_bwd<float>(a, q, dY, X, mean, rstd, dX, w, f, st)
          : dtype == DD3D_F16 ? gn::launch_bwd<half_t>(a, q, dY, X, mean, rstd, dX, w, f, st)
                              : gn::launch_bwd<bf16_t>(a, q, dY, X, mean, rstd, dX, w, f, st);
@@ -256,7 +248,7 @@ DD3D_API int dd3d_group_norm_bwd2(const void* ggX, const void* ggW, const void* 
     if (!params && !ddY && !ddX) return 0;
     const gn::Plan q = plan(a, act, esize_of(dtype), aligned16({X, dY, ggX, ddY, ddX}), act_family(act) == DD3D_FAM_LINEAR ? 7 : 14, NR_STREAM, params);
     const gn::Work w = work_at(ws, l, params);
-    const gn::Fold f = fold_for(q.g, ddweight, ddbias);
+    const gn::Fold f = fold_for(a, ddweight, ddbias);
     return dtype == DD3D_F32   ? gn::launch_bwd2<float>(a, q, ggX, ggW, ggB, dY, X, mean, rstd, ddY, ddX, w, f, st)
          : dtype == DD3D_F16 ? gn::launch_bwd2<half_t>(a, q, ggX, ggW, ggB, dY, X, mean, rstd, ddY, ddX, w, f, st)
                              : gn::launch_bwd2<bf16_t>(a, q, ggX, ggW, ggB, dY, X, mean, rstd, ddY, ddX, w, f, st);

@@ -9,30 +9,30 @@ struct Tag {
     typedef Z type;
 };
 
-// NRS / NRL: vectors a thread holds in the variants for short and for long clouds
-template <typename T, int NRS, int NRL, int V, bool AL, bool UNI, int FAM, typename F>
+// NRS / NRL / NR8: vectors a thread holds (NR_* in group_norm.h)
+template <typename T, int NRS, int NRL, int V, bool AL, int NS, int FAM, typename F>
 int with_size(const Plan& p, F f) {
     if (p.size == 2) {
-        if constexpr (V == 4) return f(Tag<Cfg<T, V, AL, UNI, FAM, 1024, NRS>>());
+        if constexpr (V == 4) return f(Tag<Cfg<T, V, AL, NS, FAM, 1024, NRS>>());
     }
-    if constexpr (UNI && V == 4) {
-        if (p.size == 1) return f(Tag<Cfg<T, V, AL, UNI, FAM, 256, NRL>>());
+    if constexpr (NS == 1 && V == 4) {
+        if (p.size == 1) return f(Tag<Cfg<T, V, AL, NS, FAM, 256, NRL>>());
     }
-    return f(Tag<Cfg<T, V, AL, UNI, FAM, 256, NRS>>());
+    return f(Tag<Cfg<T, V, AL, NS, FAM, 256, NRS>>());
 }
-template <typename T, int NRS, int NRL, int V, bool AL, bool UNI, typename F>
+template <typename T, int NRS, int NRL, int V, bool AL, int NS, typename F>
 int with_family(const Plan& p, F f) {
-    return p.fam == DD3D_FAM_LINEAR ? with_size<T, NRS, NRL, V, AL, UNI, DD3D_FAM_LINEAR>(p, f)
-           : p.fam == DD3D_FAM_SILU ? with_size<T, NRS, NRL, V, AL, UNI, DD3D_FAM_SILU>(p, f)
-                                    : with_size<T, NRS, NRL, V, AL, UNI, DD3D_FAM_GELU>(p, f);
+    return p.fam == DD3D_FAM_LINEAR ? with_size<T, NRS, NRL, V, AL, NS, DD3D_FAM_LINEAR>(p, f)
+           : p.fam == DD3D_FAM_SILU ? with_size<T, NRS, NRL, V, AL, NS, DD3D_FAM_SILU>(p, f)
+                                    : with_size<T, NRS, NRL, V, AL, NS, DD3D_FAM_GELU>(p, f);
 }
-template <typename T, int NRS, int NRL, typename F>
+template <typename T, int NRS, int NRL, int NR8, typename F>
 int with_variant(const Plan& p, F f) {
     if constexpr (sizeof(T) == 2) {
-        if (p.V == 8) return with_family<T, NRS, NRL, 8, true, true>(p, f);
+        if (p.V == 8) return p.ns == 1 ? with_family<T, NR8, NR8, 8, true, 1>(p, f) : with_family<T, NR8, NR8, 8, true, 2>(p, f);
     }
-    if (!p.al) return with_family<T, NRS, NRL, 4, false, false>(p, f);
-    return p.uni ? with_family<T, NRS, NRL, 4, true, true>(p, f) : with_family<T, NRS, NRL, 4, true, false>(p, f);
+    if (!p.al) return with_family<T, NRS, NRL, 4, false, 4>(p, f);
+    return p.ns == 1 ? with_family<T, NRS, NRL, 4, true, 1>(p, f) : with_family<T, NRS, NRL, 4, true, 4>(p, f);
 }
 
 template <typename K>
@@ -43,7 +43,7 @@ int set_lds(K kernel, size_t lds) {
 
 template <typename T>
 int launch_fwd(const Norm& a, const Plan& p, const void* X, void* Y, float* mean, float* rstd, const Work& w, hipStream_t st) {
-    return with_variant<T, NR_FWD[0], NR_FWD[1]>(p, [&](auto tag) {
+    return with_variant<T, NR_FWD[0], NR_FWD[1], NR_FWD[2]>(p, [&](auto tag) {
         typedef typename decltype(tag)::type Z;
         int rc = set_lds(k_fwd<Z, 0>, p.lds);
         if (rc) return rc;
@@ -63,7 +63,7 @@ int launch_fwd(const Norm& a, const Plan& p, const void* X, void* Y, float* mean
 
 template <typename T>
 int launch_bwd(const Norm& a, const Plan& p, const void* dY, const void* X, const float* mean, const float* rstd, void* dX, const Work& w, Fold f, hipStream_t st) {
-    return with_variant<T, NR_BWD[0], NR_BWD[1]>(p, [&](auto tag) {
+    return with_variant<T, NR_BWD[0], NR_BWD[1], NR_BWD[2]>(p, [&](auto tag) {
         typedef typename decltype(tag)::type Z;
         int rc = set_lds(k_bwd<Z, 0>, p.lds);
         if (rc) return rc;
@@ -74,8 +74,8 @@ int launch_bwd(const Norm& a, const Plan& p, const void* dY, const void* X, cons
             rc = set_lds(k_bwd<Z, 1>, p.lds);
             if (rc) return rc;
             g.units = g.NW;
-            f.first = p.blocks1;
-            k_bwd<Z, 1><<<p.blocks1 + (w.slots ? g.tickets * f.parts : 0), Z::THREADS, p.lds, st>>>(a, g, (const T*)dY, (const T*)X, mean, rstd, (T*)dX, w, f);
+            if (!w.slots) f.blocks = 0;
+            k_bwd<Z, 1><<<f.blocks + p.blocks1, Z::THREADS, p.lds, st>>>(a, g, (const T*)dY, (const T*)X, mean, rstd, (T*)dX, w, f);
         } else if (w.slots) {
             return launch_fold(a, p, w, f, st);
         }
@@ -84,20 +84,10 @@ int launch_bwd(const Norm& a, const Plan& p, const void* dY, const void* X, cons
     });
 }
 
-// (the second gradient walks every cloud twice: one size, NR_BWD2[1] rows of wide vectors)
-template <typename T, typename F>
-int with_bwd2(const Plan& p, F f) {
-    if constexpr (sizeof(T) == 2) {
-        if (p.V == 8) return with_family<T, NR_BWD2[1], NR_BWD2[1], 8, true, true>(p, f);
-    }
-    if (!p.al) return with_family<T, NR_BWD2[0], NR_BWD2[0], 4, false, false>(p, f);
-    return p.uni ? with_family<T, NR_BWD2[0], NR_BWD2[0], 4, true, true>(p, f) : with_family<T, NR_BWD2[0], NR_BWD2[0], 4, true, false>(p, f);
-}
-
 template <typename T>
 int launch_bwd2(const Norm& a, const Plan& p, const void* P, const void* ggw, const void* ggb, const void* dY, const void* X, const float* mean, const float* rstd,
                 void* ddY, void* ddX, const Work& w, Fold f, hipStream_t st) {
-    return with_bwd2<T>(p, [&](auto tag) {
+    return with_variant<T, NR_BWD2[0], NR_BWD2[1], NR_BWD2[2]>(p, [&](auto tag) {
         typedef typename decltype(tag)::type Z;
         int rc = set_lds(k_bwd2<Z, 0>, p.lds);
         if (rc) return rc;

@@ -448,9 +448,9 @@ def _rows_dtype(t: torch.Tensor, name: str) -> int:
     return _DTYPES[t.dtype]
 
 
-def _dense(t: torch.Tensor) -> torch.Tensor:
-    t = t.detach()
-    return t if t.is_contiguous() else t.contiguous()
+def _dense(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    """For raw use where no graph is recorded (inside a Function, or with nothing that requires one)."""
+    return t if t is None or t.is_contiguous() else t.contiguous()
 
 
 def _same_device(x: torch.Tensor, **others):
@@ -489,8 +489,7 @@ def random_key(state: torch.Tensor) -> torch.Tensor:
         raise ValueError("the state of a key stream is a contiguous int64 tensor (seed, call)")
     _same_device(state)
     key = torch.empty_like(state)
-    with L.on_device(state.device):
-        L.call("dd3d_random_key", state.data_ptr(), key.data_ptr(), L.raw_stream(state.device))
+    _launch(state.device, "dd3d_random_key", state.data_ptr(), key.data_ptr(), L.raw_stream(state.device))
     return key
 
 
@@ -513,8 +512,7 @@ def _dropout_raw(x, p, key):
     x = _dense(x)
     y = torch.empty_like(x)
     C = x.shape[-1] if x.dim() else 1
-    with L.on_device(x.device):
-        L.call("dd3d_dropout", x.data_ptr(), _DTYPES[x.dtype], x.numel() // max(C, 1), C, p, key.data_ptr(), y.data_ptr(), L.raw_stream(x.device))
+    _launch(x.device, "dd3d_dropout", x.data_ptr(), _DTYPES[x.dtype], x.numel() // max(C, 1), C, p, key.data_ptr(), y.data_ptr(), L.raw_stream(x.device))
     return y
 
 
@@ -551,9 +549,17 @@ class _NormMeta(NamedTuple):
         # its own block for every call: two graphs captured on one stream may be replayed side by side
         ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
         pdt = _DTYPES[(w if w is not None else b if b is not None else x).dtype]
-        with L.on_device(dev):
-            L.call(name, *before, x.data_ptr(), _DTYPES[x.dtype], M, C, seg_off.data_ptr(), B, self.G, _addr(w), _addr(b), pdt, *eps, self.act, self.slope,
-                   self.p, _addr(key), *after, _addr(ws), n, L.raw_stream(dev))
+        _launch(dev, name, *before, x.data_ptr(), _DTYPES[x.dtype], M, C, seg_off.data_ptr(), B, self.G, _addr(w), _addr(b), pdt, *eps, self.act, self.slope,
+                self.p, _addr(key), *after, _addr(ws), n, L.raw_stream(dev))
+
+
+def _launch(dev, name, *args):
+    """L.call with the rows' device current."""
+    if torch.cuda.current_device() == dev.index:
+        L.call(name, *args)
+    else:
+        with torch.cuda.device(dev):
+            L.call(name, *args)
 
 
 def _addr(t):
@@ -561,12 +567,8 @@ def _addr(t):
     return None if t is None else t.data_ptr()
 
 
-def _opt_dense(t):
-    return None if t is None else _dense(t)
-
-
 def _norm_fwd(x, w, b, seg_off, key, meta, eps, keep):
-    x, w, b = _dense(x), _opt_dense(w), _opt_dense(b)
+    x, w, b = _dense(x), _dense(w), _dense(b)
     y, stats = torch.empty_like(x), None
     if keep:   # mean and 1 / standard deviation
         stats = torch.empty((2, seg_off.numel() - 1, meta.G), dtype=_F32, device=x.device)
@@ -582,8 +584,10 @@ def _stats(stats):
 
 
 def _norm_grad(dy, x, w, b, seg_off, key, stats, meta, need):
-    dy, x, w, b = _dense(dy), _dense(x), _opt_dense(w), _opt_dense(b)
-    dx, dw, db = (torch.empty_like(t) if n else None for t, n in zip((x, w, b), need))
+    dy, x, w, b = _dense(dy), _dense(x), _dense(w), _dense(b)
+    dx = torch.empty_like(x) if need[0] else None
+    dw = torch.empty_like(w) if need[1] else None
+    db = torch.empty_like(b) if need[2] else None
     meta.call("dd3d_group_norm_bwd", 1, x, seg_off, w, b, key, (dy.data_ptr(),), (), (*_stats(stats), _addr(dx), _addr(dw), _addr(db)))
     return dx, dw, db
 
@@ -619,7 +623,7 @@ class _GroupNormGradFn(Function):
     @once_differentiable
     def backward(ctx, ggx, ggw, ggb):
         dy, x, w, b, seg_off, key, stats = ctx.saved_tensors
-        dy, x, w, b, ggx, ggw, ggb = _dense(dy), _dense(x), *(_opt_dense(t) for t in (w, b, ggx, ggw, ggb))
+        dy, x, w, b, ggx, ggw, ggb = (_dense(t) for t in (dy, x, w, b, ggx, ggw, ggb))
         out = [torch.empty_like(t) if n else None for t, n in zip((dy, x, w, b), ctx.needs_input_grad)]
         ctx.meta.call("dd3d_group_norm_bwd2", 2, x, seg_off, w, b, key, (_addr(ggx), _addr(ggw), _addr(ggb), dy.data_ptr()), (),
                       (*_stats(stats), *(_addr(t) for t in out)))

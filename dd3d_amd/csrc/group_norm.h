@@ -78,34 +78,6 @@ __device__ __forceinline__ R again(R r) {
     return r;
 }
 
-// AL: the vector is whole, aligned and loaded at once; otherwise channels [lo, hi) of it exist and are moved one by one
-template <typename T, int V, bool AL>
-__device__ __forceinline__ Raw<T, V> load_row(const T* p, int lo, int hi) {
-    Raw<T, V> r;
-    if (AL) {
-        __builtin_memcpy(&r, __builtin_assume_aligned(p, V * sizeof(T)), sizeof(r));
-    } else {
-        T e[V];
-#pragma unroll
-        for (int i = 0; i < V; ++i) e[i] = (i >= lo && i < hi) ? p[i] : narrow<T>(0.f);
-        __builtin_memcpy(&r, e, sizeof(r));
-    }
-    return r;
-}
-template <typename T, int V, bool AL>
-__device__ __forceinline__ void store_row(T* p, const float (&v)[V], int lo, int hi) {
-    T e[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) e[i] = narrow<T>(v[i]);
-    if (AL) {
-        __builtin_memcpy(__builtin_assume_aligned(p, V * sizeof(T)), e, sizeof(e));
-    } else {
-#pragma unroll
-        for (int i = 0; i < V; ++i)
-            if (i >= lo && i < hi) p[i] = e[i];
-    }
-}
-
 // ---- where this thread stands ---------------------------------------------------------------------------------------------------
 // The compile-time side of a launch.  NS: statistics a vector needs -- 1 where it lies inside one group (Cg % V == 0), 2 where it holds two
 // groups of four, else one per channel.  AL: whole, aligned vectors.
@@ -133,9 +105,8 @@ struct Spot {
     int c0, lo, hi;       // first channel of this thread, which of its V exist in the slab
     bool on;              // this thread has rows at all
     int buf;              // which half of the sums' LDS is next
-    uint32_t off, step;   // elements from a chunk's first row to this thread's first vector, and from one of its rows to the next
+    uint32_t off, step;   // bytes from a chunk's first row to this thread's first vector, and from one of its rows to the next
     uint32_t word;        // the same in blocks of random words
-    uint32_t cc;          // c0, or for a thread without channels some vector that exists
     int j[Z::NS];         // group (within the slab) of its channels
     float w[Z::V], b[Z::V];
 };
@@ -179,8 +150,8 @@ __device__ __forceinline__ void locate(const Norm& a, const Geo& g, int unit, in
     s.lo = s.s0 - s.c0, s.hi = s.s1 - s.c0;
     s.on = s.rl < g.RL && s.hi > 0;
     s.buf = 0;
-    s.cc = Z::AL ? min(s.c0, s.s1 - Z::V) : s.c0;
-    s.off = s.rl * a.C + s.cc, s.step = g.RL * a.C;
+    s.step = g.RL * a.C * (int)sizeof(typename Z::T);
+    s.off = Z::AL && !s.on ? 0x40000000u : (uint32_t)(s.rl * a.C + s.c0) * (uint32_t)sizeof(typename Z::T);   // (a chunk is far below 2^30 bytes)
     s.word = s.rl * g.quads + s.c0 / 4;
 #pragma unroll
     for (int i = 0; i < Z::NS; ++i) s.j[i] = min(quot(max(s.c0 + i * Z::PER - s.s0, 0), g.dCg), s.gs - 1);
@@ -515,22 +486,61 @@ __device__ __forceinline__ PhiloxKey drop_key(const Drop& d) {
     return k;
 }
 
-// the thread's rows of the chunk that begins at `from` with `left` rows before the end.  No load waits behind a branch of its own: threads
-// past the end (and threads without channels) read the last row again.
+// The chunk of rows that begins at `from`, `left` rows before the end, as a buffer: an access past its last row, or by a thread without
+// channels (whose offset lies past any chunk), reads zeros and writes nothing, so no access waits behind a branch and none needs its
+// bounds computed.  Unaligned rows are moved element by element, under the thread's own bounds.
 template <typename Z>
-__device__ __forceinline__ void load_chunk(const typename Z::T* from, int C, int left, const Geo& g, const Spot<Z>& s, typename Z::Row (&x)[Z::NR]) {
-    const uint32_t last = (uint32_t)(left - 1) * (uint32_t)C + s.cc, off = here(s.off);
-#pragma unroll
-    for (int n = 0; n < Z::NR; ++n) {
-        if (n * g.RL < left)
-            x[n] = load_row<typename Z::T, Z::V, Z::AL>(
-                (const typename Z::T*)((const char*)from + min(off + n * s.step, last) * (uint32_t)sizeof(typename Z::T)), s.on ? s.lo : Z::V, s.hi);
+struct Chunk {
+    typedef typename Z::T T;
+    __amdgpu_buffer_rsrc_t buf;
+    T* at;
+    int left;
+
+    __device__ __forceinline__ Chunk(const T* from, int C, int left_, const Geo& g) : at(const_cast<T*>(from)), left(left_) {
+        if (Z::AL) buf = __builtin_amdgcn_make_buffer_rsrc(at, 0, min(left, Z::NR * g.RL) * C * (int)sizeof(T), 0x00020000);
     }
-}
-template <typename Z>
-__device__ __forceinline__ void store_at(typename Z::T* to, uint32_t off, const float (&v)[Z::V], const Spot<Z>& s) {
-    store_row<typename Z::T, Z::V, Z::AL>((typename Z::T*)((char*)to + off * (uint32_t)sizeof(typename Z::T)), v, s.lo, s.hi);
-}
+    __device__ __forceinline__ bool has(const Geo& g, const Spot<Z>& s, int n) const { return s.on && s.rl + n * g.RL < left; }
+
+    // row n of the thread; off = here(s.off)
+    __device__ __forceinline__ typename Z::Row load(const Geo& g, const Spot<Z>& s, uint32_t off, int n) const {
+        typename Z::Row r;
+        const uint32_t o = off + n * s.step;
+        if constexpr (Z::AL && sizeof(r) == 16) {
+            r.u = __builtin_amdgcn_raw_buffer_load_b128(buf, (int)o, 0, 0);
+        } else if constexpr (Z::AL) {
+            r.u = __builtin_amdgcn_raw_buffer_load_b64(buf, (int)o, 0, 0);
+        } else {
+            T e[Z::V];
+#pragma unroll
+            for (int i = 0; i < Z::V; ++i) e[i] = has(g, s, n) && i >= s.lo && i < s.hi ? ((const T*)((const char*)at + o))[i] : narrow<T>(0.f);
+            __builtin_memcpy(&r, e, sizeof(r));
+        }
+        return r;
+    }
+    __device__ __forceinline__ void store(const Geo& g, const Spot<Z>& s, uint32_t off, int n, const float (&v)[Z::V]) const {
+        typename Z::Row r;
+        T e[Z::V];
+        const uint32_t o = off + n * s.step;
+#pragma unroll
+        for (int i = 0; i < Z::V; ++i) e[i] = narrow<T>(v[i]);
+        if constexpr (Z::AL) {
+            __builtin_memcpy(&r, e, sizeof(r));
+            if constexpr (sizeof(r) == 16) __builtin_amdgcn_raw_buffer_store_b128(r.u, buf, (int)o, 0, 0);
+            else __builtin_amdgcn_raw_buffer_store_b64(r.u, buf, (int)o, 0, 0);
+        } else {
+#pragma unroll
+            for (int i = 0; i < Z::V; ++i)
+                if (has(g, s, n) && i >= s.lo && i < s.hi) ((T*)((char*)at + o))[i] = e[i];
+        }
+    }
+    // all rows of the thread
+    __device__ __forceinline__ void load_all(const Geo& g, const Spot<Z>& s, typename Z::Row (&x)[Z::NR]) const {
+        const uint32_t off = here(s.off);
+#pragma unroll
+        for (int n = 0; n < Z::NR; ++n)
+            if (n * g.RL < left) x[n] = load(g, s, off, n);
+    }
+};
 // element offset of row `base`, and its first block of random words
 __device__ __forceinline__ int64_t row_at(const Norm& a, int base) { return (int64_t)base * a.C; }
 __device__ __forceinline__ uint64_t words_at(const Geo& g, int base) { return (uint64_t)(uint32_t)base * (uint32_t)g.quads; }
@@ -595,12 +605,12 @@ struct Fwd {
 #pragma unroll
         for (int i = 0; i < NS; ++i) sx[i] = q[i] = 0.f;
 #pragma unroll
-        for (int n = 0; n < NR; ++n)
-            if (s.rl + n * g.RL < left) {
-                n1 += (float)(V / NS);
+        for (int n = 0; n < NR; ++n) {
+            if (n * g.RL >= all) break;
+            n1 += s.rl + n * g.RL < left ? (float)(V / NS) : 0.f;
 #pragma unroll
-                for (int i = 0; i < V; ++i) sx[Z::at(i)] += raw_get(z[n], i);
-            }
+            for (int i = 0; i < V; ++i) sx[Z::at(i)] += raw_get(z[n], i);   // (zeros past the end)
+        }
         if (n1 == 0.f) return;
         // (reciprocals to a step: any shift near the mean serves the sum of squares)
         const float inv = __builtin_amdgcn_rcpf(n1), sum = cnt + n1, part = n1 * __builtin_amdgcn_rcpf(sum), cross = cnt * part;
@@ -650,7 +660,7 @@ struct Fwd {
         for (int i = 0; i < NS; ++i) mu[i] = m2[0][i] = 0.f;
         for (int base = r.r0; base < r.r1; base += NR * g.RL) {
             typename Z::Row z[NR];
-            load_chunk<Z>(X + row_at(a, base), a.C, r.r1 - base, g, s, z);
+            Chunk<Z>(X + row_at(a, base), a.C, r.r1 - base, g).load_all(g, s, z);
             add_rows(r.r1 - base, z, cnt, mu, m2);
         }
         join(r.r1 - r.r0, cnt, mu, m2, v);
@@ -673,7 +683,7 @@ struct Fwd {
     __device__ __forceinline__ void apply(const Range& r, const float (&mean)[NS], const float (&rstd)[NS]) {
         for (int base = r.r0; base < r.r1; base += NR * g.RL) {
             typename Z::Row z[NR];
-            load_chunk<Z>(X + row_at(a, base), a.C, r.r1 - base, g, s, z);
+            Chunk<Z>(X + row_at(a, base), a.C, r.r1 - base, g).load_all(g, s, z);
             rows_out(base, r.r1 - base, mean, rstd, z);
         }
     }
@@ -682,7 +692,7 @@ struct Fwd {
     __device__ __forceinline__ void short_cloud(const Range& r, int b, float* mean_out, float* rstd_out) {
         const int rows = r.r1 - r.r0;
         typename Z::Row z[NR];
-        load_chunk<Z>(X + row_at(a, r.r0), a.C, rows, g, s, z);
+        Chunk<Z>(X + row_at(a, r.r0), a.C, rows, g).load_all(g, s, z);
         float cnt = 0.f, mu[NS], m2[1][NS], v[2][NS], rstd[NS];
 #pragma unroll
         for (int i = 0; i < NS; ++i) mu[i] = m2[0][i] = 0.f;
@@ -693,23 +703,25 @@ struct Fwd {
     }
 
     __device__ __forceinline__ void rows_out(int base, int all, const float (&mean)[NS], const float (&rstd)[NS], const typename Z::Row (&z)[NR]) {
-        const int left = s.on ? all : 0;
-        T* to = Y + row_at(a, base);
+        const Chunk<Z> to(Y + row_at(a, base), a.C, all, g);
         const uint64_t words = words_at(g, base);
         const uint32_t off = here(s.off), word = here(s.word);
+        float scale[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) scale[i] = rstd[Z::at(i)] * s.w[i];
 #pragma unroll
         for (int n = 0; n < NR; ++n) {
             row_border();
-            if (s.rl + n * g.RL >= left) continue;
+            if (n * g.RL >= all) break;
             float y[V], d1, d2;
             const typename Z::Row x = again(z[n]);
 #pragma unroll
             for (int i = 0; i < V; ++i)
-                y[i] = activate<Z::FAM, 0, sizeof(T) == 2>(fmaf((raw_get(x, i) - mean[Z::at(i)]) * rstd[Z::at(i)], s.w[i], s.b[i]), a.slope, &d1, &d2);
+                y[i] = activate<Z::FAM, 0, sizeof(T) == 2>(fmaf(raw_get(x, i) - mean[Z::at(i)], scale[i], s.b[i]), a.slope, &d1, &d2);
             if (a.drop.key) {
                 drop_row<V>(a.drop, keep_bits<V>(a.drop, key, words + (word + n * (uint32_t)(g.RL * g.quads))), y);
             }
-            store_at<Z>(to, off + n * s.step, y, s);
+            to.store(g, s, off, n, y);
         }
     }
 };
@@ -821,8 +833,8 @@ struct Bwd {
     }
 
     __device__ __forceinline__ void load(int base, int all, Held& h) {
-        load_chunk<Z>(X + row_at(a, base), a.C, all, g, s, h.x);
-        load_chunk<Z>(dY + row_at(a, base), a.C, all, g, s, h.d);
+        Chunk<Z>(X + row_at(a, base), a.C, all, g).load_all(g, s, h.x);
+        Chunk<Z>(dY + row_at(a, base), a.C, all, g).load_all(g, s, h.d);
     }
 
     // xh and g of one row
@@ -841,15 +853,14 @@ struct Bwd {
 
     // the chunk's part of v = sums of h and h xh per group, and of the parameter gradients
     __device__ __forceinline__ void add_rows(int base, int all, Held& h, float (&v)[2][NS]) {
-        const int left = s.on ? all : 0;
         const uint64_t words = words_at(g, base);
         const uint32_t word = here(s.word);
 #pragma unroll
         for (int i = 0; i < (HOLD ? 1 : (NR * V + 31) / 32); ++i) h.keep[i] = 0;
 #pragma unroll
-        for (int n = 0; n < NR; ++n) {
+        for (int n = 0; n < NR; ++n) {   // (a row past the end has dy = 0 and adds nothing)
             row_border();
-            if (s.rl + n * g.RL >= left) continue;
+            if (n * g.RL >= all) break;
             uint32_t keep = 0;
             if (a.drop.key) {
                 keep = keep_bits<V>(a.drop, key, words + (word + n * (uint32_t)(g.RL * g.quads)));
@@ -870,14 +881,13 @@ struct Bwd {
     }
 
     __device__ __forceinline__ void rows_out(int base, int all, const Held& h, bool fresh, const float (&m1)[NS], const float (&m2)[NS]) {
-        const int left = s.on ? all : 0;
-        T* to = dX + row_at(a, base);
+        const Chunk<Z> to(dX + row_at(a, base), a.C, all, g);
         const uint64_t words = words_at(g, base);
         const uint32_t off = here(s.off), word = here(s.word);
 #pragma unroll
         for (int n = 0; n < NR; ++n) {
             row_border();
-            if (s.rl + n * g.RL >= left) continue;
+            if (n * g.RL >= all) break;
             float xh[V], gr[V], dx[V];
             if (HOLD && !fresh) {
 #pragma unroll
@@ -892,7 +902,7 @@ struct Bwd {
             }
 #pragma unroll
             for (int i = 0; i < V; ++i) dx[i] = rstd[Z::at(i)] * fmaf(gr[i], s.w[i], -fmaf(xh[i], m2[Z::at(i)], m1[Z::at(i)]));
-            store_at<Z>(to, off + n * s.step, dx, s);
+            to.store(g, s, off, n, dx);
         }
     }
 
@@ -1027,9 +1037,9 @@ struct Bwd2 {
     }
 
     __device__ __forceinline__ void load(int base, int all, Held& h) {
-        load_chunk<Z>(X + row_at(a, base), a.C, all, g, s, h.x);
-        load_chunk<Z>(dY + row_at(a, base), a.C, all, g, s, h.d);
-        if (P) load_chunk<Z>(P + row_at(a, base), a.C, all, g, s, h.p);
+        Chunk<Z>(X + row_at(a, base), a.C, all, g).load_all(g, s, h.x);
+        Chunk<Z>(dY + row_at(a, base), a.C, all, g).load_all(g, s, h.d);
+        if (P) Chunk<Z>(P + row_at(a, base), a.C, all, g).load_all(g, s, h.p);
 #pragma unroll
         for (int i = 0; i < KW; ++i) h.keep[i] = 0;
         if (!a.drop.key) return;
@@ -1068,11 +1078,10 @@ struct Bwd2 {
     }
 
     __device__ __forceinline__ void add_rows(int all, const Held& h, float (&v)[KS][NS]) {
-        const int left = s.on ? all : 0;
 #pragma unroll
-        for (int n = 0; n < NR; ++n) {
+        for (int n = 0; n < NR; ++n) {   // (a row past the end has dy = P = 0 and adds nothing)
             row_border();
-            if (s.rl + n * g.RL >= left) continue;
+            if (n * g.RL >= all) break;
             const RowOf row = row_of(h.x[n], h.d[n], h.p[n], h.keep[n * V / 32] >> (n * V % 32));
 #pragma unroll
             for (int i = 0; i < V; ++i) {
@@ -1109,13 +1118,12 @@ struct Bwd2 {
     }
 
     __device__ __forceinline__ void rows_out(int base, int all, const Held& h, const float (&m)[KS][NS], const float (&u)[2][NS]) {
-        const int left = s.on ? all : 0;
-        T *to_y = ddY + row_at(a, base), *to_x = ddX + row_at(a, base);
+        const Chunk<Z> to_y(ddY + row_at(a, base), a.C, all, g), to_x(ddX + row_at(a, base), a.C, all, g);
         const uint32_t off = here(s.off);
 #pragma unroll
         for (int n = 0; n < NR; ++n) {
             row_border();
-            if (s.rl + n * g.RL >= left) continue;
+            if (n * g.RL >= all) break;
             float oy[V], ox[V];
             const typename Z::Row x = again(h.x[n]), d = again(h.d[n]), p = again(h.p[n]);
             const uint32_t keep = h.keep[n * V / 32] >> (n * V % 32);
@@ -1134,8 +1142,8 @@ struct Bwd2 {
                 par[1][i] += ub;
             }
             drop_row<V>(a.drop, keep, oy);
-            if (ddY) store_at<Z>(to_y, off + n * s.step, oy, s);
-            if (ddX) store_at<Z>(to_x, off + n * s.step, ox, s);
+            if (ddY) to_y.store(g, s, off, n, oy);
+            if (ddX) to_x.store(g, s, off, n, ox);
         }
     }
 

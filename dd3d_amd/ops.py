@@ -509,10 +509,12 @@ class DropoutFn(Function):
 
 
 def _dropout_raw(x, p, key):
-    x = _dense(x)
+    if not x.is_contiguous():
+        x = x.contiguous()
     y = torch.empty_like(x)
+    dev = x.device
     C = x.shape[-1] if x.dim() else 1
-    _launch(x.device, "dd3d_dropout", x.data_ptr(), _DTYPES[x.dtype], x.numel() // max(C, 1), C, p, key.data_ptr(), y.data_ptr(), L.raw_stream(x.device))
+    _launch(dev, "dd3d_dropout", x.data_ptr(), _DTYPES[x.dtype], x.numel() // (C or 1), C, p, key.data_ptr(), y.data_ptr(), L.raw_stream(dev))
     return y
 
 
@@ -521,11 +523,13 @@ def dropout(x: torch.Tensor, p: float, key: torch.Tensor) -> torch.Tensor:
     ``x.view(-1, x.shape[-1])`` is dropped iff its word of a counter-based generator under ``key`` = int64 (seed, call) is below
     round(p * 2^32): the mask is never stored, a call with the same key drops the same elements, and a dropped element is zero even
     where ``x`` is not finite.  p = 0 returns ``x``."""
-    _rows_dtype(x, "x")
-    p = _check_drop(p, key)
-    _same_device(x, key=key)
-    if p == 0.0:
-        return x
+    if not (x.is_cuda and x.dtype in _DTYPES and p.__class__ is float and 0.0 < p <= 1.0 and key is not None and key.dtype is torch.int64
+            and key.numel() == 2 and key.is_contiguous() and key.device == x.device):   # (the ordinary call takes one test)
+        _rows_dtype(x, "x")
+        p = _check_drop(p, key)
+        _same_device(x, key=key)
+        if p == 0.0:
+            return x
     return DropoutFn.apply(x, p, key) if x.requires_grad and torch.is_grad_enabled() else _dropout_raw(x, p, key)
 
 
@@ -541,16 +545,16 @@ class _NormMeta(NamedTuple):
     slope: float
     p: float
 
-    def call(self, name, order, x, seg_off, w, b, key, before, eps, after):
-        """One C entry point: ``before``, the rows and the norm's shape and parameters, ``eps`` (the forward's), ``after``, workspace."""
+    def shape(self, x, seg_off, w, b):
+        """The arguments that the three C entry points share: the rows' type and size, the clouds, the parameters and their type."""
         M, C = x.shape
-        B, dev = seg_off.numel() - 1, x.device
-        n = _norm_workspace_bytes(M, C, B, self.G, order)
-        # its own block for every call: two graphs captured on one stream may be replayed side by side
-        ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
-        pdt = _DTYPES[(w if w is not None else b if b is not None else x).dtype]
-        _launch(dev, name, *before, x.data_ptr(), _DTYPES[x.dtype], M, C, seg_off.data_ptr(), B, self.G, _addr(w), _addr(b), pdt, *eps, self.act, self.slope,
-                self.p, _addr(key), *after, _addr(ws), n, L.raw_stream(dev))
+        pdt = _DTYPES[(x if w is None and b is None else b if w is None else w).dtype]
+        return (_DTYPES[x.dtype], M, C, seg_off.data_ptr(), seg_off.numel() - 1, self.G, _addr(w), _addr(b), pdt)
+
+    def workspace(self, x, seg_off, order):
+        """Its own block for every call: two graphs captured on one stream may be replayed side by side."""
+        n = _norm_workspace_bytes(x.shape[0], x.shape[1], seg_off.numel() - 1, self.G, order)
+        return (torch.empty(n, dtype=torch.uint8, device=x.device) if n else None), n
 
 
 def _launch(dev, name, *args):
@@ -569,26 +573,29 @@ def _addr(t):
 
 def _norm_fwd(x, w, b, seg_off, key, meta, eps, keep):
     x, w, b = _dense(x), _dense(w), _dense(b)
-    y, stats = torch.empty_like(x), None
-    if keep:   # mean and 1 / standard deviation
-        stats = torch.empty((2, seg_off.numel() - 1, meta.G), dtype=_F32, device=x.device)
-    mean = _addr(stats)
-    rstd = mean + 4 * (stats.numel() // 2) if mean else None
-    meta.call("dd3d_group_norm_fwd", 0, x, seg_off, w, b, key, (), (eps,), (y.data_ptr(), mean or None, rstd))
+    dev = x.device
+    y = torch.empty_like(x)
+    stats = torch.empty((2, seg_off.numel() - 1, meta.G), dtype=_F32, device=dev) if keep else None   # mean and 1 / standard deviation
+    ws, n = meta.workspace(x, seg_off, 0)
+    _launch(dev, "dd3d_group_norm_fwd", x.data_ptr(), *meta.shape(x, seg_off, w, b), eps, meta.act, meta.slope, meta.p, _addr(key), y.data_ptr(), *_stats(stats),
+            _addr(ws), n, L.raw_stream(dev))
     return y, stats
 
 
 def _stats(stats):
-    at = stats.data_ptr()
-    return (at, at + 4 * (stats.numel() // 2)) if at else (None, None)
+    at = stats.data_ptr() if stats is not None else 0
+    return (at, at + 2 * stats.numel()) if at else (None, None)   # the second half of 4-byte values
 
 
 def _norm_grad(dy, x, w, b, seg_off, key, stats, meta, need):
     dy, x, w, b = _dense(dy), _dense(x), _dense(w), _dense(b)
+    dev = x.device
     dx = torch.empty_like(x) if need[0] else None
     dw = torch.empty_like(w) if need[1] else None
     db = torch.empty_like(b) if need[2] else None
-    meta.call("dd3d_group_norm_bwd", 1, x, seg_off, w, b, key, (dy.data_ptr(),), (), (*_stats(stats), _addr(dx), _addr(dw), _addr(db)))
+    ws, n = meta.workspace(x, seg_off, 1)
+    _launch(dev, "dd3d_group_norm_bwd", dy.data_ptr(), x.data_ptr(), *meta.shape(x, seg_off, w, b), meta.act, meta.slope, meta.p, _addr(key), *_stats(stats),
+            _addr(dx), _addr(dw), _addr(db), _addr(ws), n, L.raw_stream(dev))
     return dx, dw, db
 
 
@@ -623,11 +630,17 @@ class _GroupNormGradFn(Function):
     @once_differentiable
     def backward(ctx, ggx, ggw, ggb):
         dy, x, w, b, seg_off, key, stats = ctx.saved_tensors
-        dy, x, w, b, ggx, ggw, ggb = (_dense(t) for t in (dy, x, w, b, ggx, ggw, ggb))
-        out = [torch.empty_like(t) if n else None for t, n in zip((dy, x, w, b), ctx.needs_input_grad)]
-        ctx.meta.call("dd3d_group_norm_bwd2", 2, x, seg_off, w, b, key, (_addr(ggx), _addr(ggw), _addr(ggb), dy.data_ptr()), (),
-                      (*_stats(stats), *(_addr(t) for t in out)))
-        return (*out, None, None, None, None, None)
+        meta, need = ctx.meta, ctx.needs_input_grad
+        dy, x, w, b, ggx, ggw, ggb = _dense(dy), _dense(x), _dense(w), _dense(b), _dense(ggx), _dense(ggw), _dense(ggb)
+        dev = x.device
+        ddy = torch.empty_like(dy) if need[0] else None
+        ddx = torch.empty_like(x) if need[1] else None
+        ddw = torch.empty_like(w) if need[2] else None
+        ddb = torch.empty_like(b) if need[3] else None
+        ws, n = meta.workspace(x, seg_off, 2)
+        _launch(dev, "dd3d_group_norm_bwd2", _addr(ggx), _addr(ggw), _addr(ggb), dy.data_ptr(), x.data_ptr(), *meta.shape(x, seg_off, w, b), meta.act,
+                meta.slope, meta.p, _addr(key), *_stats(stats), _addr(ddy), _addr(ddx), _addr(ddw), _addr(ddb), _addr(ws), n, L.raw_stream(dev))
+        return ddy, ddx, ddw, ddb, None, None, None, None, None
 
 
 def group_norm(x: torch.Tensor, seg_off: torch.Tensor, num_groups: int, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
@@ -649,10 +662,10 @@ def group_norm(x: torch.Tensor, seg_off: torch.Tensor, num_groups: int, weight: 
         raise ValueError(f"group_norm takes up to {_MAX_NORM_CHANNELS} channels and 2^31 - 1 rows, got [{M}, {C}]")
     if seg_off.dtype != torch.int32 or seg_off.dim() != 1 or seg_off.numel() < 1 or not seg_off.is_contiguous():
         raise ValueError("seg_off has to be a contiguous int32 tensor [B + 1]")
-    for name, t in (("weight", weight), ("bias", bias)):
-        if t is not None and (t.numel() != C or t.dtype not in (_F32, x.dtype)):
-            raise ValueError(f"{name} has to hold {C} values in float32 or {x.dtype}")
-    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+    for t in (weight, bias):
+        if t is not None and (t.numel() != C or (t.dtype is not _F32 and t.dtype is not x.dtype)):
+            raise ValueError(f"weight and bias have to hold {C} values in float32 or {x.dtype}")
+    if weight is not None and bias is not None and weight.dtype is not bias.dtype:
         raise ValueError("weight and bias have to be of one type")
     if activation not in _ACTIVATIONS:
         raise ValueError(f"unknown activation {activation!r}: none, relu, leaky_relu, silu or gelu")
@@ -660,8 +673,11 @@ def group_norm(x: torch.Tensor, seg_off: torch.Tensor, num_groups: int, weight: 
         raise ValueError(f"eps has to be positive, got {eps}")
     if negative_slope != negative_slope:
         raise ValueError("negative_slope is not a number")
-    p = _check_drop(dropout, key)
-    _same_device(x, seg_off=seg_off, weight=weight, bias=bias, key=key)
+    p = _check_drop(dropout, key) if dropout != 0.0 else 0.0
+    dev = x.device
+    if not x.is_cuda or seg_off.device != dev or (weight is not None and weight.device != dev) or (bias is not None and bias.device != dev) or (
+            key is not None and key.device != dev):
+        _same_device(x, seg_off=seg_off, weight=weight, bias=bias, key=key)
     meta = _NormMeta(int(num_groups), _ACTIVATIONS[activation], float(negative_slope), p)
     key = key if p > 0.0 else None
     if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or (bias is not None and bias.requires_grad)):

@@ -64,39 +64,34 @@ __device__ __forceinline__ void store_param(void* p, int pdt, int64_t i, float v
 
 __host__ __device__ __forceinline__ int act_family(int act) { return act <= DD3D_ACT_LEAKY ? DD3D_FAM_LINEAR : act == DD3D_ACT_SILU ? DD3D_FAM_SILU : DD3D_FAM_GELU; }
 
-// Phi(u) and the density n(u).  The upper tail is n-shaped: Q(a) = exp(-a^2 / 2) t P(t) for a = |u|, t = 1 / (1 + 0.35 a), P a degree-8
-// polynomial fitted for least relative error over a in [0, 14] (3.2e-8), so the far tail keeps its relative accuracy and no
-// cancellation occurs on either side; one exponential serves Phi and n alike.
-__device__ __forceinline__ void normal_cdf_pdf(float u, float* cdf, float* pdf) {
-    const float a = fabsf(u), t = __builtin_amdgcn_rcpf(fmaf(0.35f, a, 1.f));
-    const float e = __builtin_amdgcn_exp2f(u * u * -0.72134752f);
-    float p = -0.029146108776330948f;
-    p = fmaf(p, t, 0.14397257566452026f);
-    p = fmaf(p, t, -0.25571608543395996f);
-    p = fmaf(p, t, 0.15917624533176422f);
-    p = fmaf(p, t, -0.02311127260327339f);
-    p = fmaf(p, t, 0.10550861060619354f);
-    p = fmaf(p, t, 0.11983271688222885f);
-    p = fmaf(p, t, 0.13986189663410187f);
-    p = fmaf(p, t, 0.13962140679359436f);
-    const float q = e * (p * t);
-    *cdf = u < 0.f ? q : 1.f - q;
-    *pdf = e * 0.39894228f;
-}
-
-// The same Phi for results that are rounded to half width: a polynomial of degree 5 over t = 1 / (1 + 0.3 a), relative error 8.2e-6, a
-// sixtieth of fp16's half step.
-__device__ __forceinline__ float normal_cdf_short(float u) {
-    const float a = fabsf(u), t = __builtin_amdgcn_rcpf(fmaf(0.3f, a, 1.f));
-    const float e = __builtin_amdgcn_exp2f(u * u * -0.72134752f);
-    float p = -0.07709760218858719f;
-    p = fmaf(p, t, 0.21603752672672272f);
-    p = fmaf(p, t, -0.016948513686656952f);
-    p = fmaf(p, t, 0.14419656991958618f);
-    p = fmaf(p, t, 0.11374188959598541f);
-    p = fmaf(p, t, 0.12007423490285873f);
-    const float q = e * (p * t);
-    return u < 0.f ? q : 1.f - q;
+// The upper tail Q(a) = 1 - Phi(a) of the normal distribution, a = |u|, is n-shaped: Q(a) = exp(-a^2 / 2) t P(t) with t = 1 / (1 + 0.35 a) and P a
+// degree-8 polynomial fitted for least relative error over a in [0, 14] (3.2e-8).  So the far tail keeps its relative accuracy, one
+// exponential serves Phi and the density alike, and on either side only one subtraction is left:
+//   u Phi(u) = max(u, 0) - a Q(a),   Phi(u) + u n(u) = u > 0 ? 1 + r : -r,  r = a n(a) - Q(a),   2 n - u^2 n = n (2 - u^2).
+// SHORT: results that are rounded to half width take degree 5 over t = 1 / (1 + 0.3 a), relative error 8.2e-6, a sixtieth of fp16's half step.
+template <bool SHORT>
+__device__ __forceinline__ void normal_tail(float a, float* e, float* pt) {
+    const float s = a * 0.84932180f;   // sqrt(log2(e) / 2)
+    const float t = __builtin_amdgcn_rcpf(fmaf(SHORT ? 0.3f : 0.35f, a, 1.f));
+    float p;
+    if (SHORT) {
+        p = fmaf(-0.07709760218858719f, t, 0.21603752672672272f);
+        p = fmaf(p, t, -0.016948513686656952f);
+        p = fmaf(p, t, 0.14419656991958618f);
+        p = fmaf(p, t, 0.11374188959598541f);
+        p = fmaf(p, t, 0.12007423490285873f);
+    } else {
+        p = fmaf(-0.029146108776330948f, t, 0.14397257566452026f);
+        p = fmaf(p, t, -0.25571608543395996f);
+        p = fmaf(p, t, 0.15917624533176422f);
+        p = fmaf(p, t, -0.02311127260327339f);
+        p = fmaf(p, t, 0.10550861060619354f);
+        p = fmaf(p, t, 0.11983271688222885f);
+        p = fmaf(p, t, 0.13986189663410187f);
+        p = fmaf(p, t, 0.13962140679359436f);
+    }
+    *e = __builtin_amdgcn_exp2f(-s * s);
+    *pt = p * t;   // Q = e pt
 }
 
 // phi(u); with ORDER >= 1 also phi'(u) in *d1, with ORDER == 2 phi''(u) in *d2
@@ -117,12 +112,16 @@ __device__ __forceinline__ float activate(float u, float slope, float* d1, float
         if (ORDER == 2) *d2 = ds * fmaf(u, 1.f - 2.f * s, 2.f);
         return u * s;
     }
-    if (SHORT && ORDER == 0) return u * normal_cdf_short(u);
-    float cdf, pdf;
-    normal_cdf_pdf(u, &cdf, &pdf);
-    if (ORDER >= 1) *d1 = fmaf(u, pdf, cdf);
-    if (ORDER == 2) *d2 = pdf * fmaf(-u, u, 2.f);
-    return u * cdf;
+    const float a = fabsf(u);
+    float e, pt;
+    normal_tail<SHORT && ORDER == 0>(a, &e, &pt);
+    if (ORDER >= 1) {
+        const float r = e * fmaf(a, 0.39894228f, -pt);
+        *d1 = u > 0.f ? 1.f + r : -r;
+    }
+    if (ORDER == 2) *d2 = 0.39894228f * e * fmaf(-u, u, 2.f);
+    const float up = u < 0.f ? 0.f : u;   // (NaN stays)
+    return fmaf(-a, e * pt, up);
 }
 
 // ---- random words ---------------------------------------------------------------------------------------------------------------
@@ -148,14 +147,16 @@ __device__ __forceinline__ PhiloxKey philox_key(const int64_t* key) {
     return k;
 }
 
+__device__ __forceinline__ uint32_t xor3(uint32_t a, uint32_t b, uint32_t c) { return __builtin_amdgcn_bitop3_b32(a, b, c, 0x96); }
+
 __device__ __forceinline__ uint4 philox_block(const PhiloxKey k, uint64_t block) {
     uint32_t c0 = (uint32_t)block, c1 = (uint32_t)(block >> 32), c2 = k.c2, c3 = k.c3, k0 = k.k0, k1 = k.k1;
 #pragma unroll
     for (int r = 0; r < 10; ++r) {
         const uint64_t a = (uint64_t)c0 * 0xD2511F53u, b = (uint64_t)c2 * 0xCD9E8D57u;
-        c0 = (uint32_t)(b >> 32) ^ c1 ^ k0;
+        c0 = xor3((uint32_t)(b >> 32), c1, k0);
         c1 = (uint32_t)b;
-        c2 = (uint32_t)(a >> 32) ^ c3 ^ k1;
+        c2 = xor3((uint32_t)(a >> 32), c3, k1);
         c3 = (uint32_t)a;
         k0 += 0x9E3779B9u;
         k1 += 0xBB67AE85u;

@@ -460,25 +460,36 @@ __device__ __forceinline__ void join_parts(const float* part, const Range& r, fl
         for (int i = 0; i < Z::NS; ++i) v[q][i] = out[q * g.k + s.j[i]];
 }
 
-// the elements of this thread's vector that dropout keeps, as bits
+// the random words of a thread's vector
 template <int V>
-__device__ __forceinline__ uint32_t keep_bits(const Drop& d, const PhiloxKey& k, uint64_t block) {
-    uint32_t m = 0;
-    if (d.all) return 0;
+struct Words {
+    uint32_t w[V];
+
+    __device__ __forceinline__ Words(const PhiloxKey& k, uint64_t block) {
 #pragma unroll
-    for (int h = 0; h < V / 4; ++h) {
-        const uint4 w = philox_block(k, block + h);
-        m |= (uint32_t)(w.x >= d.thr) << (4 * h) | (uint32_t)(w.y >= d.thr) << (4 * h + 1) | (uint32_t)(w.z >= d.thr) << (4 * h + 2) |
-             (uint32_t)(w.w >= d.thr) << (4 * h + 3);
+        for (int h = 0; h < V / 4; ++h) {
+            const uint4 r = philox_block(k, block + h);
+            w[4 * h] = r.x, w[4 * h + 1] = r.y, w[4 * h + 2] = r.z, w[4 * h + 3] = r.w;
+        }
     }
-    return m;
-}
-// dropout of one row's values, behind one uniform branch
+    __device__ __forceinline__ void drop(const Drop& d, float (&v)[V]) const {
+        // (with p = 1 thr is the largest word, which is kept, and the scale is 0: infinite values are told apart by `all`)
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] = w[i] >= d.thr && !d.all ? v[i] * d.scale : 0.f;
+    }
+    __device__ __forceinline__ uint32_t bits(const Drop& d) const {
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < V; ++i) m |= w[i] >= d.thr && !d.all ? 1u << i : 0u;
+        return m;
+    }
+};
+// dropout of one row's values by kept bits, behind one uniform branch
 template <int V>
 __device__ __forceinline__ void drop_row(const Drop& d, uint32_t keep, float (&v)[V]) {
     if (!d.key) return;
 #pragma unroll
-    for (int i = 0; i < V; ++i) v[i] = keep >> i & 1 ? v[i] * d.scale : 0.f;
+    for (int i = 0; i < V; ++i) v[i] = keep & (1u << i) ? v[i] * d.scale : 0.f;
 }
 __device__ __forceinline__ PhiloxKey drop_key(const Drop& d) {
     PhiloxKey k = {0, 0, 0, 0};
@@ -719,7 +730,7 @@ struct Fwd {
             for (int i = 0; i < V; ++i)
                 y[i] = activate<Z::FAM, 0, sizeof(T) == 2>(fmaf(raw_get(x, i) - mean[Z::at(i)], scale[i], s.b[i]), a.slope, &d1, &d2);
             if (a.drop.key) {
-                drop_row<V>(a.drop, keep_bits<V>(a.drop, key, words + (word + n * (uint32_t)(g.RL * g.quads))), y);
+                Words<V>(key, words + (word + n * (uint32_t)(g.RL * g.quads))).drop(a.drop, y);
             }
             to.store(g, s, off, n, y);
         }
@@ -838,10 +849,7 @@ struct Bwd {
     }
 
     // xh and g of one row
-    __device__ __forceinline__ void element(const typename Z::Row& x, const typename Z::Row& d, uint32_t keep, float (&xh)[V], float (&gr)[V]) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) gr[i] = raw_get(d, i);
-        drop_row<V>(a.drop, keep, gr);
+    __device__ __forceinline__ void element(const typename Z::Row& x, float (&xh)[V], float (&gr)[V]) {   // gr: dy after dropout -> g
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             float d1, d2;
@@ -861,13 +869,15 @@ struct Bwd {
         for (int n = 0; n < NR; ++n) {   // (a row past the end has dy = 0 and adds nothing)
             row_border();
             if (n * g.RL >= all) break;
-            uint32_t keep = 0;
-            if (a.drop.key) {
-                keep = keep_bits<V>(a.drop, key, words + (word + n * (uint32_t)(g.RL * g.quads)));
-                if (!HOLD) h.keep[n * V / 32] |= keep << (n * V % 32);
-            }
             float xh[V], gr[V];
-            element(h.x[n], h.d[n], keep, xh, gr);
+#pragma unroll
+            for (int i = 0; i < V; ++i) gr[i] = raw_get(h.d[n], i);
+            if (a.drop.key) {
+                const Words<V> rnd(key, words + (word + n * (uint32_t)(g.RL * g.quads)));
+                rnd.drop(a.drop, gr);
+                if (!HOLD) h.keep[n * V / 32] |= rnd.bits(a.drop) << (n * V % 32);
+            }
+            element(h.x[n], xh, gr);
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 const float t = gr[i] * s.w[i];
@@ -893,12 +903,12 @@ struct Bwd {
 #pragma unroll
                 for (int i = 0; i < V; ++i) xh[i] = h.xh[n][i], gr[i] = h.gr[n][i];
             } else {
-                uint32_t keep = 0;
-                if (a.drop.key) {
-                    if (fresh) keep = keep_bits<V>(a.drop, key, words + (word + n * (uint32_t)(g.RL * g.quads)));
-                    else keep = h.keep[HOLD ? 0 : n * V / 32] >> (n * V % 32);
-                }
-                element(again(h.x[n]), again(h.d[n]), keep, xh, gr);
+                const typename Z::Row x = again(h.x[n]), d = again(h.d[n]);
+#pragma unroll
+                for (int i = 0; i < V; ++i) gr[i] = raw_get(d, i);
+                if (!fresh) drop_row<V>(a.drop, h.keep[HOLD ? 0 : n * V / 32] >> (n * V % 32), gr);
+                else if (a.drop.key) Words<V>(key, words + (word + n * (uint32_t)(g.RL * g.quads))).drop(a.drop, gr);
+                element(x, xh, gr);
             }
 #pragma unroll
             for (int i = 0; i < V; ++i) dx[i] = rstd[Z::at(i)] * fmaf(gr[i], s.w[i], -fmaf(xh[i], m2[Z::at(i)], m1[Z::at(i)]));
@@ -1048,7 +1058,7 @@ struct Bwd2 {
 #pragma unroll
         for (int n = 0; n < NR; ++n) {
             row_border();
-            if (n * g.RL < all) h.keep[n * V / 32] |= keep_bits<V>(a.drop, key, words + (word + n * (uint32_t)(g.RL * g.quads))) << (n * V % 32);
+            if (n * g.RL < all) h.keep[n * V / 32] |= Words<V>(key, words + (word + n * (uint32_t)(g.RL * g.quads))).bits(a.drop) << (n * V % 32);
         }
     }
 

@@ -87,7 +87,7 @@ inline gn::Plan plan(const gn::Norm& a, int act, int esize, bool aligned, int su
     g.quads = (a.C + 3) / 4;
     g.dCL = divide_by(g.CL), g.dCg = divide_by(a.Cg);
     const int64_t cap = (p.size == 1 ? nr[1] : shorter) * g.RL;   // rows of a chunk
-    g.NW = (int)std::min<int64_t>(ceil_div64(a.M, MIN_WINDOW), max_windows(a.C));
+    g.NW = (int)std::min<int64_t>(std::min<int64_t>(ceil_div64(a.M, MIN_WINDOW), max_windows(a.C)), std::max(64, atoi(getenv("GN_NW") ? getenv("GN_NW") : "1024") / g.nslab));
     g.CH = g.NW ? (int)ceil_div64(a.M, g.NW) : 1;
     g.Tl = (int)std::max<int64_t>(2 * cap, g.CH);
     g.NW = a.M <= g.Tl ? 0 : (int)ceil_div64(a.M, g.CH);

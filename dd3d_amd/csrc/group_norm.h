@@ -473,7 +473,6 @@ struct Words {
         }
     }
     __device__ __forceinline__ void drop(const Drop& d, float (&v)[V]) const {
-        // (with p = 1 thr is the largest word, which is kept, and the scale is 0: infinite values are told apart by `all`)
 #pragma unroll
         for (int i = 0; i < V; ++i) v[i] = w[i] >= d.thr && !d.all ? v[i] * d.scale : 0.f;
     }

@@ -9,8 +9,6 @@
 // m(X) and m(X xh) follow from sums that one pass over the rows gives (group_norm.h).  The kernels: group_norm.h.  Here: argument checks, launch geometry, parameter gradients.
 #include "group_norm.h"
 
-#include <stdlib.h>
-
 #include <algorithm>
 #include <initializer_list>
 
@@ -33,6 +31,9 @@ __global__ __launch_bounds__(1024) void k_fold(gn::Norm a, gn::Geo g, gn::Work w
 // windows of the whole batch: enough to fill the chip with the slabs of a row, never so many that joining them shows
 inline int max_windows(int C) { return C >= 1024 ? 64 : C <= 64 ? 1024 : 65536 / C; }
 constexpr int MIN_WINDOW = 512, MAX_UNITS = 2048;
+// Workgroups of a windows' launch: three a compute unit, all at once.  Seven clouds of 57 000 rows of 96 bf16 channels, forward / backward:
+// 59 / 104 us, with 512 workgroups 70 / 124, with 2048 68 / 110 (a second round starts as the first ends).
+constexpr int WINDOW_GROUPS = 768;
 
 inline int gcd(int a, int b) { return b ? gcd(b, a % b) : a; }
 
@@ -60,20 +61,21 @@ inline gn::Plan plan(const gn::Norm& a, int act, int esize, bool aligned, int su
     auto whole = [&](int k) { return k >= a.G ? a.G : p.al ? std::min(a.G, (k + m0 - 1) / m0 * m0) : k; };
     // Slab width: 64 bytes of a row at least (its neighbour reads the other half of the line into the same L2), doubled while a short
     // cloud still fits one chunk and 1024 workgroups remain to fill the chip.  fp32 forward, 128 channels, us at 64 / 128 / 256 / 512
-    // bytes: 2560 clouds of 82 rows 106 / 65 / 52 / 58, 100 of 216 rows 13.7 / 15.3 / 19.8 / 28.7, 400 of 750 rows (long variant)
-    // 87 / 96 / 112 / 123.
+    // bytes: 2560 clouds of 82 rows 105 / 66 / 53 / 59, 100 of 216 rows 13.7 / 16.0 / 20.3 / 29.6, 400 of 750 rows (long variant)
+    // 88 / 98 / 120 / 138.  Less than 64 bytes where that leaves less than 512 workgroups (97 clouds of 309 rows, 100 channels in groups of
+    // 20, fp16: 31 us at 40 bytes, 44 at 80; backward 39 and 58).
     const int kmin = whole((64 / esize + a.Cg - 1) / a.Cg);
     const int64_t mean = a.B ? a.M / a.B : 0, shorter = nr[p.V == 8 ? 2 : 0];   // rows a thread holds, short variant
     int k = kmin;
+    const int64_t pieces = a.B + std::min<int64_t>(a.M / MIN_WINDOW, WINDOW_GROUPS);   // clouds and windows
+    while (k > 1 && pieces * ((a.G + k - 1) / k) < 512 && whole(k / 2) < k) k = whole(k / 2);
     p.size = 0;
-    if (lanes(kmin) > 256) {
+    if (lanes(k) > 256) {
         p.size = 2;
     } else {
         for (int w = whole(2 * k); k < a.G && lanes(w) <= 64 && shorter * (256 / lanes(w)) >= mean && (int64_t)a.B * ((a.G + w - 1) / w) >= 1024; w = whole(2 * k)) k = w;
-        if (p.ns == 1 && p.V == 4 && shorter * (256 / lanes(kmin)) < mean) p.size = 1;
+        if (p.ns == 1 && p.V == 4 && shorter * (256 / lanes(k)) < mean) p.size = 1;
     }
-    if (getenv("GN_T")) p.size = p.ns == 1 && p.V == 4 ? atoi(getenv("GN_T")) : 0;
-    if (getenv("GN_W")) k = whole(std::max(1, atoi(getenv("GN_W")) / a.Cg));
     const int threads = p.size == 2 ? 1024 : 256;
     g.k = k;
     g.nslab = (a.G + k - 1) / k;
@@ -87,7 +89,7 @@ inline gn::Plan plan(const gn::Norm& a, int act, int esize, bool aligned, int su
     g.quads = (a.C + 3) / 4;
     g.dCL = divide_by(g.CL), g.dCg = divide_by(a.Cg);
     const int64_t cap = (p.size == 1 ? nr[1] : shorter) * g.RL;   // rows of a chunk
-    g.NW = (int)std::min<int64_t>(std::min<int64_t>(ceil_div64(a.M, MIN_WINDOW), max_windows(a.C)), std::max(64, atoi(getenv("GN_NW") ? getenv("GN_NW") : "1024") / g.nslab));
+    g.NW = (int)std::min<int64_t>(std::min<int64_t>(ceil_div64(a.M, MIN_WINDOW), max_windows(a.C)), std::max(64, WINDOW_GROUPS / g.nslab));
     g.CH = g.NW ? (int)ceil_div64(a.M, g.NW) : 1;
     g.Tl = (int)std::max<int64_t>(2 * cap, g.CH);
     g.NW = a.M <= g.Tl ? 0 : (int)ceil_div64(a.M, g.CH);
@@ -191,7 +193,7 @@ DD3D_API int dd3d_group_norm_fwd(const void* X, int dtype, int64_t M, int C, con
     gn::Norm a;
     const int rc = check(dtype, M, C, seg_off, B, G, weight, bias, pdtype, act, slope, p, key, &a);
     if (rc) return rc;
-    if (!(eps > 0.f) || (!mean != !rstd) || (M > 0 && (!X || !Y))) return DD3D_EARG;
+    if (!(eps >= 1.17549435e-38f && eps <= 3.4e38f) || (!mean != !rstd) || (M > 0 && (!X || !Y))) return DD3D_EARG;
     a.eps = eps;
     const Layout l = layout(M, C, B, G, 0);
     if (ws_bytes < l.bytes || (l.bytes > 0 && !ws)) return DD3D_EWS;

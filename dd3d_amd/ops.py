@@ -669,8 +669,8 @@ def group_norm(x: torch.Tensor, seg_off: torch.Tensor, num_groups: int, weight: 
         raise ValueError("weight and bias have to be of one type")
     if activation not in _ACTIVATIONS:
         raise ValueError(f"unknown activation {activation!r}: none, relu, leaky_relu, silu or gelu")
-    if not eps > 0.0:
-        raise ValueError(f"eps has to be positive, got {eps}")
+    if not 2.0 ** -126 <= eps <= 3.4e38:
+        raise ValueError(f"eps has to be positive (a normal fp32 number), got {eps}")
     if negative_slope != negative_slope:
         raise ValueError("negative_slope is not a number")
     p = _check_drop(dropout, key) if dropout != 0.0 else 0.0

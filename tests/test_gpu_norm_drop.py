@@ -110,6 +110,51 @@ def test_long_clouds(lens, C, G, dtype):
     check(through_autograd(t, so, G, 2, 0.0, activation="relu"), seg, t, G, "relu", 0.0)
 
 
+@pytest.mark.parametrize("lens,C,G,dtype", [([2] * 2500, 8, 1, F32), ([1, 4, 2] * 900, 12, 3, BF16), ([90] * 40, 128, 8, F16), ([82] * 300, 64, 4, F32)])
+def test_many_short_clouds(lens, C, G, dtype):
+    """More clouds than workgroups leave parts of the parameter gradients for: one workgroup takes several."""
+    seg, t = batch(lens, C, dtype, seed=21)
+    so = torch.tensor(seg, dtype=torch.int32, device=dev())
+    check(through_autograd(t, so, G, 2, 0.2, activation="silu", eps=1e-2), seg, t, G, "silu", 0.2, eps=1e-2)
+
+
+@pytest.mark.parametrize("rows", [1, 31, 32, 33, 63, 64, 65, 255, 256, 257, 511, 512, 513, 1023, 1024, 1025, 2047, 2049, 4097])
+def test_lengths_about_the_chunk_and_window_sizes(rows):
+    lens = [rows, 2, rows + 1]
+    for C, G, dtype in ((16, 2, F32), (32, 1, BF16), (128, 32, F16)):
+        seg, t = batch(lens, C, dtype, seed=rows)
+        so = torch.tensor(seg, dtype=torch.int32, device=dev())
+        check(through_autograd(t, so, G, 2, 0.1, activation="silu", eps=1e-2), seg, t, G, "silu", 0.1, eps=1e-2)
+
+
+def test_everything_dropped_and_next_to_it():
+    seg, t = batch(MIXED, 16, F32, seed=22)
+    so = torch.tensor(seg, dtype=torch.int32, device=dev())
+    got = through_autograd(t, so, 4, 2, 1.0, activation="silu")
+    assert not any(bool(v.any()) for k, v in got.items()), "p = 1 leaves nothing"
+    check(through_autograd(t, so, 4, 2, 0.999, activation="silu"), seg, t, 4, "silu", 0.999)
+
+
+def test_two_calls_at_once():
+    """Two streams, one pair of parameters: neither call sees the other's workspace."""
+    from dd3d_amd import ops
+    so = torch.tensor(offsets([6000, 40, 9000] + [70] * 50), dtype=torch.int32, device=dev())
+    xs = [torch.randn(18540, 64, device=dev(), generator=torch.Generator(dev()).manual_seed(i)).requires_grad_() for i in range(2)]
+    w, b = torch.rand(64, device=dev()).requires_grad_(), torch.rand(64, device=dev()).requires_grad_()
+    run = lambda x: torch.autograd.grad(ops.group_norm(x, so, 8, w, b, activation="gelu", dropout=0.1, key=key()).square().sum(), (x, w, b))  # noqa: E731
+    want = [[g.clone() for g in run(x)] for x in xs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in xs]
+    for _ in range(3):
+        got = []
+        for x, s in zip(xs, streams):
+            with torch.cuda.stream(s):
+                got.append(run(x))
+        torch.cuda.synchronize()
+        for o, r in zip(got, want):
+            assert all(torch.equal(a, c) for a, c in zip(o[1:], r[1:])) and torch.equal(o[0], r[0])
+
+
 @pytest.mark.parametrize("affine", [(False, False), (True, False), (False, True)])
 def test_without_weight_or_bias(affine):
     seg, t = batch(MIXED, 16, F32, seed=3)

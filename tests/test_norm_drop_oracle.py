@@ -89,7 +89,7 @@ def test_c_entry_points_refuse_bad_arguments_before_any_launch():
     def fwd(dtype=0, M=10, C=8, seg=one, B=1, G=2, w=one, b=one, pdt=0, eps=1e-5, act=0, slope=0.1, p=0.0, key=None, x=one, y=one, mean=None, rstd=None):
         return lib.dd3d_group_norm_fwd(x, dtype, M, C, seg, B, G, w, b, pdt, eps, act, slope, p, key, y, mean, rstd, None, 0, None)
     for bad in (dict(dtype=3), dict(dtype=-1), dict(M=-1), dict(C=0), dict(C=9), dict(G=0), dict(B=-1), dict(seg=None), dict(pdt=1), dict(eps=0.0),
-                dict(eps=float("nan")), dict(act=5), dict(act=-1), dict(slope=float("nan")), dict(p=-0.1), dict(p=1.5), dict(p=float("nan")), dict(p=0.5),
+                dict(eps=float("nan")), dict(eps=1e-40), dict(eps=float("inf")), dict(act=5), dict(act=-1), dict(slope=float("nan")), dict(p=-0.1), dict(p=1.5), dict(p=float("nan")), dict(p=0.5),
                 dict(x=None), dict(y=None), dict(mean=one), dict(rstd=one)):
         assert fwd(**bad) == -1, bad
     for bad in (dict(M=2 ** 31), dict(C=4098, G=2), dict(B=2 ** 30, G=8)):
@@ -125,7 +125,7 @@ def test_python_entry_points_refuse_bad_arguments():
         ops.dropout(x.long(), 0.5, key)
     for bad in (dict(x=x[0]), dict(G=3), dict(G=0), dict(G=16), dict(seg=seg.long()), dict(seg=seg[None]), dict(seg=seg[:0]), dict(w=torch.ones(7)),
                 dict(w=torch.ones(8, dtype=torch.float64)), dict(w=torch.ones(8, dtype=torch.bfloat16)), dict(activation="tanh"), dict(eps=0.0),
-                dict(eps=float("nan")), dict(negative_slope=float("nan")), dict(dropout=1.2, key=key), dict(dropout=-0.1, key=key), dict(dropout=0.3),
+                dict(eps=float("nan")), dict(eps=1e-40), dict(eps=float("inf")), dict(negative_slope=float("nan")), dict(dropout=1.2, key=key), dict(dropout=-0.1, key=key), dict(dropout=0.3),
                 dict(dropout=0.3, key=key.int()), dict(dropout=0.3, key=key[:1]), dict(x=torch.zeros(2, 4100), G=1)):
         with pytest.raises(ValueError):
             gn(**bad)

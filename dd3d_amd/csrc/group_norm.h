@@ -843,8 +843,11 @@ struct Bwd {
     }
 
     __device__ __forceinline__ void load(int base, int all, Held& h) {
-        Chunk<Z>(X + row_at(a, base), a.C, all, g).load_all(g, s, h.x);
-        Chunk<Z>(dY + row_at(a, base), a.C, all, g).load_all(g, s, h.d);
+        const Chunk<Z> cx(X + row_at(a, base), a.C, all, g), cd(dY + row_at(a, base), a.C, all, g);
+        const uint32_t off = here(s.off);
+#pragma unroll
+        for (int n = 0; n < NR; ++n)   // row by row: the first can be worked on while the others are on their way
+            if (n * g.RL < all) h.x[n] = cx.load(g, s, off, n), h.d[n] = cd.load(g, s, off, n);
     }
 
     // xh and g of one row
@@ -1046,9 +1049,12 @@ struct Bwd2 {
     }
 
     __device__ __forceinline__ void load(int base, int all, Held& h) {
-        Chunk<Z>(X + row_at(a, base), a.C, all, g).load_all(g, s, h.x);
-        Chunk<Z>(dY + row_at(a, base), a.C, all, g).load_all(g, s, h.d);
-        if (P) Chunk<Z>(P + row_at(a, base), a.C, all, g).load_all(g, s, h.p);
+        const Chunk<Z> cx(X + row_at(a, base), a.C, all, g), cd(dY + row_at(a, base), a.C, all, g);
+        const Chunk<Z> cp(P ? P + row_at(a, base) : X, a.C, P ? all : 0, g);   // (without P: an empty buffer, whose rows read as zeros)
+        const uint32_t off = here(s.off);
+#pragma unroll
+        for (int n = 0; n < NR; ++n)   // row by row: the first can be worked on while the others are on their way
+            if (n * g.RL < all) h.x[n] = cx.load(g, s, off, n), h.d[n] = cd.load(g, s, off, n), h.p[n] = cp.load(g, s, off, n);
 #pragma unroll
         for (int i = 0; i < KW; ++i) h.keep[i] = 0;
         if (!a.drop.key) return;
@@ -1068,11 +1074,8 @@ struct Bwd2 {
     __device__ __forceinline__ RowOf row_of(const typename Z::Row& x, const typename Z::Row& d, const typename Z::Row& p, uint32_t keep) {
         RowOf r;
 #pragma unroll
-        for (int i = 0; i < V; ++i) r.x[i] = raw_get(x, i), r.dy[i] = raw_get(d, i), r.p[i] = 0.f;
+        for (int i = 0; i < V; ++i) r.x[i] = raw_get(x, i), r.dy[i] = raw_get(d, i), r.p[i] = raw_get(p, i);
         drop_row<V>(a.drop, keep, r.dy);
-        if (P)
-#pragma unroll
-            for (int i = 0; i < V; ++i) r.p[i] = raw_get(p, i);
         return r;
     }
     struct Elem {

@@ -18,6 +18,7 @@ from typing import NamedTuple, Optional
 import torch
 from torch.autograd import Function
 from torch.autograd.function import once_differentiable
+from torch.autograd.graph import increment_version
 
 from . import _lib as L
 from .sparse import CoordinateManager
@@ -490,6 +491,8 @@ def random_key(state: torch.Tensor) -> torch.Tensor:
     _same_device(state)
     key = torch.empty_like(state)
     _launch(state.device, "dd3d_random_key", state.data_ptr(), key.data_ptr(), L.raw_stream(state.device))
+    if not state.is_inference():
+        increment_version(state)   # a graph that saved the state itself as a key must not draw its mask from the changed one
     return key
 
 

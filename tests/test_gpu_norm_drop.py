@@ -75,6 +75,14 @@ def check(got, seg, t, G, act, p=0.0, eps=1e-5, slope=0.01, order=2, affine=(Tru
         assert far <= 1, f"{n}: {far:.3g} times what its roundings allow"
 
 
+def check_some(got, lens, every, seg, t, G, act, order):
+    """The matrices' rows of the last four clouds and of one cloud in ``every``."""
+    some = [i + i // every % 4 for i in range(0, len(lens) - 4, every)] + list(range(len(lens) - 4, len(lens)))
+    rows = torch.tensor([r for i in some for r in range(seg[i], seg[i + 1])])
+    part = {k: v[rows] if v.shape[0] == seg[-1] else v for k, v in t.items()}
+    check({n: got[n].cpu()[rows] for n in ("y", "dx", "ddy", "ddx")[:2 * order]}, offsets([lens[i] for i in some]), part, G, act, order=order)
+
+
 MIXED = [5, 0, 1, 37, 2, 0, 82, 250, 3]
 
 
@@ -397,6 +405,35 @@ def test_key_stream():
     state = ops.random_state(42, dev())
     keys = [ops.random_key(state).tolist() for _ in range(3)]
     assert keys == [[42, 0], [42, 1], [42, 2]] and state.tolist() == [42, 3]
+
+
+def test_a_state_used_as_a_key_is_not_read_after_it_changed():
+    from dd3d_amd import ops
+    state = ops.random_state(42, dev())
+    x = torch.randn(40, 32, device=dev(), requires_grad=True)
+    so = torch.tensor([0, 40], dtype=torch.int32, device=dev())
+    for call in (lambda: ops.dropout(x, 0.4, state), lambda: ops.group_norm(x, so, 4, dropout=0.4, key=state)):
+        y = call()
+        torch.autograd.grad(y.sum(), x, retain_graph=True)
+        ops.random_key(state)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(y.sum(), x)
+
+
+def test_more_clouds_than_workgroups():
+    """70 000 clouds of a row or two, on at most 32 768 forward and 2048 backward workgroups; every 500th cloud is compared."""
+    lens = [1, 2, 0, 2] * 17500
+    seg, t = batch(lens, 16, F32, seed=17)
+    got = through_autograd(t, torch.tensor(seg, dtype=torch.int32, device=dev()), 4, 1, activation="silu")
+    check_some(got, lens, 500, seg, t, 4, "silu", 1)
+
+
+@pytest.mark.parametrize("C,G,dtype", [(256, 256, F32), (256, 256, BF16), (256, 64, F16)])
+def test_as_many_groups_as_channels_and_many_clouds(C, G, dtype):
+    lens = [30, 45, 0, 1] * 300
+    seg, t = batch(lens, C, dtype, seed=18)
+    got = through_autograd(t, torch.tensor(seg, dtype=torch.int32, device=dev()), G, 2, activation="silu")
+    check_some(got, lens, 100, seg, t, G, "silu", 2)
 
 
 def test_a_captured_step_draws_a_new_mask_at_every_replay():

@@ -44,6 +44,7 @@ struct Geo {
     int quads;           // ceil(C / 4)
     int kb;              // quantities reduced at once where the sums go through LDS
     int red;             // floats of LDS for them
+    int hold;            // where in LDS (floats) the second gradient keeps a cloud's first chunk, 0: nowhere
     Div dCL, dCg;
 };
 
@@ -1029,6 +1030,7 @@ struct Bwd2 {
     T *ddY, *ddX;
     float* lds;
     PhiloxKey key;
+    typename Z::Row* mine;                 // this thread's rows in LDS: [NR][x, dy, P], a workgroup's width apart; NULL: none
     float q[V], t[V];                      // cotangents of dw and db
     float mean[NS], rstd[NS], par[2][V];   // d(w), d(b)
 
@@ -1048,13 +1050,8 @@ struct Bwd2 {
         for (int i = 0; i < NS; ++i) mean[i] = mean_in[at + s.j[i]], rstd[i] = rstd_in[at + s.j[i]];
     }
 
-    __device__ __forceinline__ void load(int base, int all, Held& h) {
-        const Chunk<Z> cx(X + row_at(a, base), a.C, all, g), cd(dY + row_at(a, base), a.C, all, g);
-        const Chunk<Z> cp(P ? P + row_at(a, base) : X, a.C, P ? all : 0, g);   // (without P: an empty buffer, whose rows read as zeros)
-        const uint32_t off = here(s.off);
-#pragma unroll
-        for (int n = 0; n < NR; ++n)   // row by row: the first can be worked on while the others are on their way
-            if (n * g.RL < all) h.x[n] = cx.load(g, s, off, n), h.d[n] = cd.load(g, s, off, n), h.p[n] = cp.load(g, s, off, n);
+    __device__ __forceinline__ void load(int base, int all, Held& h, bool from_lds) {
+        if (!from_lds) load_rows(base, all, h);
 #pragma unroll
         for (int i = 0; i < KW; ++i) h.keep[i] = 0;
         if (!a.drop.key) return;
@@ -1065,6 +1062,14 @@ struct Bwd2 {
             row_border();
             if (n * g.RL < all) h.keep[n * V / 32] |= Words<V>(key, words + (word + n * (uint32_t)(g.RL * g.quads))).bits(a.drop) << (n * V % 32);
         }
+    }
+    __device__ __forceinline__ void load_rows(int base, int all, Held& h) {
+        const Chunk<Z> cx(X + row_at(a, base), a.C, all, g), cd(dY + row_at(a, base), a.C, all, g);
+        const Chunk<Z> cp(P ? P + row_at(a, base) : X, a.C, P ? all : 0, g);   // (without P: an empty buffer, whose rows read as zeros)
+        const uint32_t off = here(s.off);
+#pragma unroll
+        for (int n = 0; n < NR; ++n)   // row by row: the first can be worked on while the others are on their way
+            if (n * g.RL < all) h.x[n] = cx.load(g, s, off, n), h.d[n] = cd.load(g, s, off, n), h.p[n] = cp.load(g, s, off, n);
     }
 
     // one row: values after dropout, and the activation's derivatives element by element
@@ -1089,11 +1094,12 @@ struct Bwd2 {
         return e;
     }
 
-    __device__ __forceinline__ void add_rows(int all, const Held& h, float (&v)[KS][NS]) {
+    __device__ __forceinline__ void add_rows(int all, const Held& h, float (&v)[KS][NS], bool to_lds) {
 #pragma unroll
         for (int n = 0; n < NR; ++n) {   // (a row past the end has dy = P = 0 and adds nothing)
             row_border();
             if (n * g.RL >= all) break;
+            if (to_lds) mine[3 * n * Z::THREADS] = h.x[n], mine[(3 * n + 1) * Z::THREADS] = h.d[n], mine[(3 * n + 2) * Z::THREADS] = h.p[n];
             const RowOf row = row_of(h.x[n], h.d[n], h.p[n], h.keep[n * V / 32] >> (n * V % 32));
 #pragma unroll
             for (int i = 0; i < V; ++i) {
@@ -1129,7 +1135,7 @@ struct Bwd2 {
         return fmaf(s.w[i], vv, fmaf(q[i], e.xh, t[i]));
     }
 
-    __device__ __forceinline__ void rows_out(int base, int all, const Held& h, const float (&m)[KS][NS], const float (&u)[2][NS]) {
+    __device__ __forceinline__ void rows_out(int base, int all, const Held& h, const float (&m)[KS][NS], const float (&u)[2][NS], bool from_lds) {
         const Chunk<Z> to_y(ddY + row_at(a, base), a.C, all, g), to_x(ddX + row_at(a, base), a.C, all, g);
         const uint32_t off = here(s.off);
 #pragma unroll
@@ -1137,7 +1143,8 @@ struct Bwd2 {
             row_border();
             if (n * g.RL >= all) break;
             float oy[V], ox[V];
-            const typename Z::Row x = again(h.x[n]), d = again(h.d[n]), p = again(h.p[n]);
+            typename Z::Row x = h.x[n], d = h.d[n], p = h.p[n];
+            if (from_lds) x = mine[3 * n * Z::THREADS], d = mine[(3 * n + 1) * Z::THREADS], p = mine[(3 * n + 2) * Z::THREADS];
             const uint32_t keep = h.keep[n * V / 32] >> (n * V % 32);
             const RowOf row = row_of(x, d, p, keep);
 #pragma unroll
@@ -1186,20 +1193,22 @@ struct Bwd2 {
             for (int i = 0; i < NS; ++i) m[k][i] = 0.f;
     }
 
-    __device__ __forceinline__ void sums(const Range& r, float (&m)[KS][NS]) {
+    // sums from the first chunk to the last, results from the last to the first: what was read last is nearest
+    __device__ __forceinline__ void sums(const Range& r, float (&m)[KS][NS], bool keep_first) {
         clear(m);
         for (int base = r.r0; base < r.r1; base += NR * g.RL) {
             Held h;
-            load(base, r.r1 - base, h);
-            add_rows(r.r1 - base, h, m);
+            load(base, r.r1 - base, h, false);
+            add_rows(r.r1 - base, h, m, keep_first && base == r.r0);
         }
         group_sums<KS, Z>(m, a, g, s, lds);
     }
-    __device__ __forceinline__ void apply(const Range& r, const float (&m)[KS][NS], const float (&u)[2][NS]) {
-        for (int base = r.r0; base < r.r1; base += NR * g.RL) {
+    __device__ __forceinline__ void apply(const Range& r, const float (&m)[KS][NS], const float (&u)[2][NS], bool kept_first) {
+        const int chunk = NR * g.RL;
+        for (int base = r.r0 + (r.r1 - r.r0 - 1) / chunk * chunk; base >= r.r0; base -= chunk) {
             Held h;
-            load(base, r.r1 - base, h);
-            rows_out(base, r.r1 - base, h, m, u);
+            load(base, r.r1 - base, h, kept_first && base == r.r0);
+            rows_out(base, r.r1 - base, h, m, u, kept_first && base == r.r0);
         }
     }
 };
@@ -1223,7 +1232,8 @@ __global__ __launch_bounds__(Z::THREADS, Z::BWD2_WAVES) void k_bwd2(Norm a, Geo 
     Spot<Z> s;
     locate(a, g, unit, slab, s);
     typedef Bwd2<Z> F;
-    F f{a, g, s, P, dY, X, ddY, ddX, lds, drop_key(a.drop)};
+    F f{a, g, s, P, dY, X, ddY, ddX, lds, drop_key(a.drop), (typename Z::Row*)(lds + g.hold) + threadIdx.x};
+    const bool held = MODE == 0 && whole && g.hold;
     load_params<Z::V>(ggw, a.pdt, s.c0, s.s0, s.s1, 0.f, f.q);
     load_params<Z::V>(ggb, a.pdt, s.c0, s.s0, s.s1, 0.f, f.t);
 #pragma unroll
@@ -1241,14 +1251,14 @@ __global__ __launch_bounds__(Z::THREADS, Z::BWD2_WAVES) void k_bwd2(Norm a, Geo 
                 r = i ? p[1].part : p[0].part;
             }
             f.load_stats(whole ? b : i ? p[1].b : p[0].b, mean_in, rstd_in);
-            f.sums(r, m);
+            f.sums(r, m, held);
             if (!whole) {
                 put_part<F::KS, Z>(w.part, i ? p[1].slot : p[0].slot, m, a, g, s);
                 continue;
             }
             f.means(m, r.r1 - r.r0);
             f.finish(m, u);
-            f.apply(r, m, u);
+            f.apply(r, m, u, held);
             continue;
         }
         if (i >= np) break;
@@ -1257,7 +1267,7 @@ __global__ __launch_bounds__(Z::THREADS, Z::BWD2_WAVES) void k_bwd2(Norm a, Geo 
         join_parts<F::KS, Z>(w.part, q.all, m, a, g, s, lds);
         f.means(m, q.all.r1 - q.all.r0);
         f.finish(m, u);
-        f.apply(q.part, m, u);
+        f.apply(q.part, m, u, false);
     }
     // a window's parameter gradients belong to its rows' last pass
     if (w.slots && (MODE == 1 || whole)) column_sums<2, Z>(f.par, a, g, s, lds, w.slots + (int64_t)(MODE == 1 ? g.U + unit : unit) * 2 * a.C);

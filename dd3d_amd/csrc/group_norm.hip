@@ -98,7 +98,7 @@ inline gn::Plan plan(const gn::Norm& a, int act, int esize, bool aligned, int su
     g.Tl = (int)std::max<int64_t>(2 * cap, g.CH);
     g.NW = a.M <= g.Tl ? 0 : (int)ceil_div64(a.M, g.CH);
     g.U = cloud_units(a.B, params);
-    g.units = 0;
+    g.units = g.hold = 0;
     p.blocks0 = (unsigned)(align_up64((int64_t)g.U + g.NW, 8) * g.nslab);
     p.blocks1 = (unsigned)(align_up64(g.NW, 8) * g.nslab);
     // LDS: row partials of kb quantities (or two buffers of the waves' sums, or the columns of one parameter gradient), the columns' totals

@@ -35,6 +35,9 @@ int with_variant(const Plan& p, F f) {
     return p.ns == 1 ? with_family<T, NRS, NRL, 4, true, 1>(p, f) : with_family<T, NRS, NRL, 4, true, 4>(p, f);
 }
 
+// LDS of a workgroup of the second gradient that keeps a chunk in it: a third of a compute unit's 160 KB, as its registers allow three
+constexpr size_t HOLD_LDS = 53 * 1024;
+
 template <typename K>
 int set_lds(K kernel, size_t lds) {
     if (lds > 64 * 1024) DD3D_HIP(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
@@ -89,11 +92,15 @@ int launch_bwd2(const Norm& a, const Plan& p, const void* P, const void* ggw, co
                 void* ddY, void* ddX, const Work& w, Fold f, hipStream_t st) {
     return with_variant<T, NR_BWD2[0], NR_BWD2[1], NR_BWD2[2]>(p, [&](auto tag) {
         typedef typename decltype(tag)::type Z;
-        int rc = set_lds(k_bwd2<Z, 0>, p.lds);
-        if (rc) return rc;
         Geo g = p.g;
+        const size_t chunk = 3 * Z::NR * sizeof(typename Z::Row) * Z::THREADS, with = align_up64(p.lds, 16) + chunk;
+        const bool hold = with <= HOLD_LDS;
+        g.hold = hold ? (int)((with - chunk) / 4) : 0;
+        const size_t lds = hold ? with : p.lds;
+        int rc = set_lds(k_bwd2<Z, 0>, lds);
+        if (rc) return rc;
         g.units = g.U + g.NW;
-        k_bwd2<Z, 0><<<p.blocks0, Z::THREADS, p.lds, st>>>(a, g, (const T*)P, ggw, ggb, (const T*)dY, (const T*)X, mean, rstd, (T*)ddY, (T*)ddX, w);
+        k_bwd2<Z, 0><<<p.blocks0, Z::THREADS, lds, st>>>(a, g, (const T*)P, ggw, ggb, (const T*)dY, (const T*)X, mean, rstd, (T*)ddY, (T*)ddX, w);
         if (g.NW) {
             rc = set_lds(k_bwd2<Z, 1>, p.lds);
             if (rc) return rc;

@@ -1043,6 +1043,10 @@ struct Bwd2 {
     // without a second pass over the rows.
     enum { H, HX, MP, PX, PH, QG, QX, E0, E1, E2, EP, EPX, EC, ECX };
     static constexpr int KS = Z::FAM == DD3D_FAM_LINEAR ? 7 : 14;
+    // A cloud's rows are needed twice, and what lies between has more of them in flight than the L2 holds (400 clouds of 750 rows of 128 fp32
+    // channels: 972 MB read instead of 461).  So LDS keeps the first chunk of a cloud and the registers its last: 242 us without, 227 with
+    // the LDS alone, 221 with both.  Variants whose registers are full already would spill, and walk all rows twice.
+    static constexpr bool HOLD = V == 4 && NS == 1 && Z::THREADS == 256;
 
     __device__ __forceinline__ void load_stats(int b, const float* mean_in, const float* rstd_in) {
         const int64_t at = (int64_t)b * a.G + s.slab * g.k;
@@ -1099,7 +1103,7 @@ struct Bwd2 {
         for (int n = 0; n < NR; ++n) {   // (a row past the end has dy = P = 0 and adds nothing)
             row_border();
             if (n * g.RL >= all) break;
-            if (to_lds) mine[3 * n * Z::THREADS] = h.x[n], mine[(3 * n + 1) * Z::THREADS] = h.d[n], mine[(3 * n + 2) * Z::THREADS] = h.p[n];
+            if (HOLD && to_lds) mine[3 * n * Z::THREADS] = h.x[n], mine[(3 * n + 1) * Z::THREADS] = h.d[n], mine[(3 * n + 2) * Z::THREADS] = h.p[n];
             const RowOf row = row_of(h.x[n], h.d[n], h.p[n], h.keep[n * V / 32] >> (n * V % 32));
 #pragma unroll
             for (int i = 0; i < V; ++i) {
@@ -1143,8 +1147,8 @@ struct Bwd2 {
             row_border();
             if (n * g.RL >= all) break;
             float oy[V], ox[V];
-            typename Z::Row x = h.x[n], d = h.d[n], p = h.p[n];
-            if (from_lds) x = mine[3 * n * Z::THREADS], d = mine[(3 * n + 1) * Z::THREADS], p = mine[(3 * n + 2) * Z::THREADS];
+            typename Z::Row x = again(h.x[n]), d = again(h.d[n]), p = again(h.p[n]);
+            if (HOLD && from_lds) x = mine[3 * n * Z::THREADS], d = mine[(3 * n + 1) * Z::THREADS], p = mine[(3 * n + 2) * Z::THREADS];
             const uint32_t keep = h.keep[n * V / 32] >> (n * V % 32);
             const RowOf row = row_of(x, d, p, keep);
 #pragma unroll
@@ -1193,22 +1197,30 @@ struct Bwd2 {
             for (int i = 0; i < NS; ++i) m[k][i] = 0.f;
     }
 
-    // sums from the first chunk to the last, results from the last to the first: what was read last is nearest
-    __device__ __forceinline__ void sums(const Range& r, float (&m)[KS][NS], bool keep_first) {
+    // Sums from the first chunk to the last, results from the last to the first.  HOLD: LDS keeps the first chunk's rows, h the last one's.
+    __device__ __forceinline__ void sums(const Range& r, float (&m)[KS][NS], bool first_to_lds, Held& h) {
         clear(m);
         for (int base = r.r0; base < r.r1; base += NR * g.RL) {
-            Held h;
-            load(base, r.r1 - base, h, false);
-            add_rows(r.r1 - base, h, m, keep_first && base == r.r0);
+            Held fresh;
+            Held& rows = HOLD ? h : fresh;
+            load(base, r.r1 - base, rows, false);
+            add_rows(r.r1 - base, rows, m, first_to_lds && base == r.r0);
         }
         group_sums<KS, Z>(m, a, g, s, lds);
     }
-    __device__ __forceinline__ void apply(const Range& r, const float (&m)[KS][NS], const float (&u)[2][NS], bool kept_first) {
-        const int chunk = NR * g.RL;
-        for (int base = r.r0 + (r.r1 - r.r0 - 1) / chunk * chunk; base >= r.r0; base -= chunk) {
+    __device__ __forceinline__ void apply_held(const Range& r, const float (&m)[KS][NS], const float (&u)[2][NS], bool first_in_lds, Held& h) {
+        const int chunk = NR * g.RL, last = r.r0 + (r.r1 - r.r0 - 1) / chunk * chunk;
+        for (int base = last; base >= r.r0; base -= chunk) {
+            const bool in_lds = first_in_lds && base == r.r0 && base != last;
+            if (base != last) load(base, r.r1 - base, h, in_lds);
+            rows_out(base, r.r1 - base, h, m, u, in_lds);
+        }
+    }
+    __device__ __forceinline__ void apply(const Range& r, const float (&m)[KS][NS], const float (&u)[2][NS]) {
+        for (int base = r.r0; base < r.r1; base += NR * g.RL) {
             Held h;
-            load(base, r.r1 - base, h, kept_first && base == r.r0);
-            rows_out(base, r.r1 - base, h, m, u, kept_first && base == r.r0);
+            load(base, r.r1 - base, h, false);
+            rows_out(base, r.r1 - base, h, m, u, false);
         }
     }
 };
@@ -1233,7 +1245,7 @@ __global__ __launch_bounds__(Z::THREADS, Z::BWD2_WAVES) void k_bwd2(Norm a, Geo 
     locate(a, g, unit, slab, s);
     typedef Bwd2<Z> F;
     F f{a, g, s, P, dY, X, ddY, ddX, lds, drop_key(a.drop), (typename Z::Row*)(lds + g.hold) + threadIdx.x};
-    const bool held = MODE == 0 && whole && g.hold;
+    const bool held = F::HOLD && MODE == 0 && whole && g.hold;
     load_params<Z::V>(ggw, a.pdt, s.c0, s.s0, s.s1, 0.f, f.q);
     load_params<Z::V>(ggb, a.pdt, s.c0, s.s0, s.s1, 0.f, f.t);
 #pragma unroll
@@ -1251,14 +1263,16 @@ __global__ __launch_bounds__(Z::THREADS, Z::BWD2_WAVES) void k_bwd2(Norm a, Geo 
                 r = i ? p[1].part : p[0].part;
             }
             f.load_stats(whole ? b : i ? p[1].b : p[0].b, mean_in, rstd_in);
-            f.sums(r, m, held);
+            typename F::Held rows;
+            f.sums(r, m, held, rows);
             if (!whole) {
                 put_part<F::KS, Z>(w.part, i ? p[1].slot : p[0].slot, m, a, g, s);
                 continue;
             }
             f.means(m, r.r1 - r.r0);
             f.finish(m, u);
-            f.apply(r, m, u, held);
+            if constexpr (F::HOLD) f.apply_held(r, m, u, held, rows);
+            else f.apply(r, m, u);
             continue;
         }
         if (i >= np) break;
@@ -1267,7 +1281,7 @@ __global__ __launch_bounds__(Z::THREADS, Z::BWD2_WAVES) void k_bwd2(Norm a, Geo 
         join_parts<F::KS, Z>(w.part, q.all, m, a, g, s, lds);
         f.means(m, q.all.r1 - q.all.r0);
         f.finish(m, u);
-        f.apply(q.part, m, u, false);
+        f.apply(q.part, m, u);
     }
     // a window's parameter gradients belong to its rows' last pass
     if (w.slots && (MODE == 1 || whole)) column_sums<2, Z>(f.par, a, g, s, lds, w.slots + (int64_t)(MODE == 1 ? g.U + unit : unit) * 2 * a.C);

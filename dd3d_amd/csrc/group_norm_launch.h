@@ -94,7 +94,7 @@ int launch_bwd2(const Norm& a, const Plan& p, const void* P, const void* ggw, co
         typedef typename decltype(tag)::type Z;
         Geo g = p.g;
         const size_t chunk = 3 * Z::NR * sizeof(typename Z::Row) * Z::THREADS, with = align_up64(p.lds, 16) + chunk;
-        const bool hold = with <= HOLD_LDS;
+        const bool hold = Bwd2<Z>::HOLD && with <= HOLD_LDS;
         g.hold = hold ? (int)((with - chunk) / 4) : 0;
         const size_t lds = hold ? with : p.lds;
         int rc = set_lds(k_bwd2<Z, 0>, lds);

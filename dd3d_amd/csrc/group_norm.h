@@ -1,12 +1,14 @@
 // Device code of the group norm (formulas: group_norm.hip), shared by its three passes and instantiated per row type and pass in group_norm_*.hip.
 //
-// All three passes are bound by HBM: the arithmetic is a few dozen fp32 operations an element.  What they need is sums over (cloud, group)
-// before anything can be written, so a row has to be read twice unless it stays on chip in between.  Layout of the work:
-//   * a SLAB is a run of whole groups, at least one 128-byte line of a row wide; a workgroup owns one slab of one cloud after another.
-//     Thread t holds V channels (one 16-byte vector) of the rows rl, rl + RL, ...: the rows of a chunk of NR * RL are loaded at once into
-//     registers, so up to that many loads are in flight per thread, and stay there while the workgroup forms the sums -- HBM sees every
-//     row once.  Four waves a workgroup: with sixteen the instructions that every wave spends on the sums outweighed the rows
-//     (82-row clouds of 128 channels, fp32 forward: 97 us against 64).
+// The passes need sums over (cloud, group) before anything can be written, so a row has to be read twice unless it stays on chip in between.
+// Large batches of fp32 rows are bound by HBM: 210 000 x 128 in 2560 clouds, SiLU, forward 51 us (4.2 TB/s), backward 82 (3.9); second
+// gradient of 300 000 x 128 in 400 clouds, GELU, 221 (3.5, and 4.9 with what it reads twice).  GELU, dropout and half-width rows are bound
+// by vector instructions (400 000 x 128 fp32 with GELU and dropout: forward 117 us, backward 179).  Layout of the work:
+//   * a SLAB is a run of whole groups, 64 bytes of a row at least; a workgroup owns one slab of one cloud after another.  Thread t holds V
+//     channels (one 16-byte vector) of the rows rl, rl + RL, ...: the rows of a chunk of NR * RL are loaded at once into registers, so up to
+//     that many loads are in flight per thread, and stay there while the workgroup forms the sums -- HBM sees every row once.  Four waves
+//     a workgroup: with sixteen the instructions that every wave spends on the sums outweighed the rows (2560 clouds of 82 rows of 128
+//     channels, fp32 forward, before the sums went by lane exchanges: 97 us against 64).  Sixteen only where a slab has more than 256 vectors.
 //   * a cloud longer than one chunk and up to `Tl` rows is walked again by the same workgroup (its slab mostly comes out of the caches).
 //   * a longer cloud ("large") is cut by WINDOWS of CH rows of the whole batch; Tl >= CH, so a window meets at most two large clouds: the
 //     one it begins in (slot 2w) and one that begins inside it (slot 2w + 1).  Windows write partial sums, a second launch joins them
@@ -83,7 +85,9 @@ __device__ __forceinline__ R again(R r) {
 // The compile-time side of a launch.  NS: statistics a vector needs -- 1 where it lies inside one group (Cg % V == 0), 2 where it holds two
 // groups of four, else one per channel.  AL: whole, aligned vectors.
 // Vectors a thread holds in the three passes: vectors of four in the variants for short and for long clouds, vectors of eight; and the
-// waves per SIMD that the registers of that many rows leave.
+// waves per SIMD that the registers of that many rows leave.  More rows spare a long cloud its second reading until registers run out
+// (400 clouds of 750 rows of 128 fp32 channels, 8 against 16: forward 99 and 74 us, backward 152 and 126); clouds that fit 8 gain from the
+// waves that 8 leave.
 constexpr int NR_FWD[3] = {8, 16, 8}, NR_BWD[3] = {8, 16, 4}, NR_BWD2[3] = {4, 4, 2};
 
 template <typename T_, int V_, bool AL_, int NS_, int FAM_, int THREADS_, int NR_>
@@ -815,7 +819,8 @@ __global__ __launch_bounds__(Z::THREADS, Z::FWD_WAVES) void k_fwd(Norm a, Geo g,
 }
 
 // ---- first gradient -------------------------------------------------------------------------------------------------------------
-// What a thread keeps of a row between the sums and the result: the normalised values and g (fp32 rows: in the registers the loaded rows
+// Bound by HBM and, at two to three waves per SIMD, by the latency of its loads; with dropout by vector instructions (30% of the cycles of
+// all waves).  What a thread keeps of a row between the sums and the result: the normalised values and g (fp32 rows: in the registers the loaded rows
 // had), or the rows as loaded and the bits dropout kept (half-width rows: half the registers, the derivative is computed again).
 template <typename Z>
 struct Bwd {
@@ -1018,7 +1023,8 @@ __global__ __launch_bounds__(Z::THREADS, Z::BWD_WAVES) void k_bwd(Norm a, Geo g,
 }
 
 // ---- second gradient ------------------------------------------------------------------------------------------------------------
-// The three matrices stay as loaded; the activation's derivatives are computed again in every pass over them.
+// Three matrices in, two out, and 14 sums an element: bound by HBM where rows are read twice, 27% of the waves' cycles are vector
+// instructions.  The three matrices stay as loaded; the activation's derivatives are computed again in every pass over them.
 template <typename Z>
 struct Bwd2 {
     typedef typename Z::T T;

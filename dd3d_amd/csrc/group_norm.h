@@ -2,7 +2,7 @@
 //
 // The passes need sums over (cloud, group) before anything can be written, so a row has to be read twice unless it stays on chip in between.
 // Large batches of fp32 rows are bound by HBM: 210 000 x 128 in 2560 clouds, SiLU, forward 51 us (4.2 TB/s), backward 82 (3.9); second
-// gradient of 300 000 x 128 in 400 clouds, GELU, 221 (3.5, and 4.9 with what it reads twice).  GELU, dropout and half-width rows are bound
+// gradient of 300 000 x 128 in 400 clouds, GELU, 221 (3.5, and 4.8 with what it reads twice).  GELU, dropout and half-width rows are bound
 // by vector instructions (400 000 x 128 fp32 with GELU and dropout: forward 117 us, backward 179).  Layout of the work:
 //   * a SLAB is a run of whole groups, 64 bytes of a row at least; a workgroup owns one slab of one cloud after another.  Thread t holds V
 //     channels (one 16-byte vector) of the rows rl, rl + RL, ...: the rows of a chunk of NR * RL are loaded at once into registers, so up to
@@ -1050,8 +1050,8 @@ struct Bwd2 {
     enum { H, HX, MP, PX, PH, QG, QX, E0, E1, E2, EP, EPX, EC, ECX };
     static constexpr int KS = Z::FAM == DD3D_FAM_LINEAR ? 7 : 14;
     // A cloud's rows are needed twice, and what lies between has more of them in flight than the L2 holds (400 clouds of 750 rows of 128 fp32
-    // channels: 972 MB read instead of 461).  So LDS keeps the first chunk of a cloud and the registers its last: 242 us without, 227 with
-    // the LDS alone, 221 with both.  Variants whose registers are full already would spill, and walk all rows twice.
+    // channels: 972 MiB read instead of 439).  So LDS keeps the first chunk of a cloud and the registers its last: 242 us without, 227 with
+    // the LDS alone, 221 and 703 MiB with both.  Variants whose registers are full already would spill, and walk all rows twice.
     static constexpr bool HOLD = V == 4 && NS == 1 && Z::THREADS == 256;
 
     __device__ __forceinline__ void load_stats(int b, const float* mean_in, const float* rstd_in) {

@@ -52,7 +52,7 @@ inline int cloud_units(int B, bool params) {
 }
 
 // sums: quantities summed at once; nr: vectors a thread holds in the variants for short and long clouds; params: column_sums is called
-constexpr int NR_STREAM[3] = {16, 16, 16};   // the second gradient walks every cloud twice whatever its length: chunks do not matter
+constexpr int NR_STREAM[3] = {16, 16, 16};   // the second gradient walks long clouds twice: its slabs and windows are cut as if 16 rows were held
 inline gn::Plan plan(const gn::Norm& a, int act, int esize, bool aligned, int sums, const int (&nr)[3], bool params) {
     gn::Plan p;
     gn::Geo& g = p.g;

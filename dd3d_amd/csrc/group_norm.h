@@ -20,8 +20,12 @@
 
 namespace gn {
 
+// Rows, clouds, and clouds times groups of one call: 65536 below 2^31, so that a counter which a loop has moved past its end by one step (a chunk of
+// 4096 rows at most, or the 32768 clouds that lie between two of one workgroup) is still a positive 32-bit number.
+constexpr int64_t MOST = (1ll << 31) - 65536;
+
 struct Norm {
-    int M, C, B, G, Cg, pdt;   // M < 2^31: row numbers fit 32 bits, element offsets do not
+    int M, C, B, G, Cg, pdt;   // M, B <= MOST: row and cloud numbers fit 32 bits, element offsets do not
     const int* seg;
     const void *W, *Bi;
     float eps, slope;

@@ -149,7 +149,7 @@ inline bool aligned16(std::initializer_list<const void*> ps) {
 inline int check(int dtype, int64_t M, int C, const int32_t* seg, int B, int G, const void* W, const void* Bi, int pdt, int act, float slope, double p,
                  const int64_t* key, gn::Norm* a) {
     if (M < 0 || B < 0 || C <= 0 || G <= 0 || C % G != 0) return DD3D_EARG;
-    if (M >= (1ll << 31) || C > 4096 || (int64_t)B * G >= (1ll << 31)) return DD3D_ESIZE;
+    if (M > gn::MOST || C > 4096 || (int64_t)B * G > gn::MOST) return DD3D_ESIZE;
     if (dtype < DD3D_F32 || dtype > DD3D_BF16 || (pdt != DD3D_F32 && pdt != dtype) || act < DD3D_ACT_NONE || act > DD3D_ACT_GELU) return DD3D_EARG;
     if (slope != slope || (B > 0 && !seg) || !make_drop(p, key, &a->drop)) return DD3D_EARG;
     a->M = (int)M, a->C = C, a->B = B, a->G = G, a->Cg = C / G, a->pdt = pdt, a->seg = seg, a->W = W, a->Bi = Bi;
@@ -187,7 +187,7 @@ int gn::launch_fold(const Norm& a, const Plan& p, const Work& w, Fold f, hipStre
 // See include/dd3d.h.
 DD3D_API int64_t dd3d_group_norm_ws_bytes(int64_t M, int C, int B, int G, int order) {
     if (M < 0 || B < 0 || C <= 0 || G <= 0 || C % G != 0 || order < 0 || order > 2) return DD3D_EARG;
-    if (M >= (1ll << 31) || C > 4096 || (int64_t)B * G >= (1ll << 31)) return DD3D_ESIZE;
+    if (M > gn::MOST || C > 4096 || (int64_t)B * G > gn::MOST) return DD3D_ESIZE;
     return layout(M, C, B, G, order).bytes;
 }
 

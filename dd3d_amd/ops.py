@@ -441,6 +441,7 @@ class NormActPoolFn(Function):
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "leaky_relu": 2, "silu": 3, "gelu": 4}
 _MAX_NORM_CHANNELS = 4096
+_MAX_NORM_ROWS = 2 ** 31 - 65536   # the kernels count rows and clouds in 32 bits and step past the end
 
 
 def _rows_dtype(t: torch.Tensor, name: str) -> int:
@@ -661,10 +662,12 @@ def group_norm(x: torch.Tensor, seg_off: torch.Tensor, num_groups: int, weight: 
     M, C = x.shape
     if not 0 < num_groups <= C or C % num_groups:
         raise ValueError(f"{C} channels do not divide into {num_groups} groups")
-    if C > _MAX_NORM_CHANNELS or M >= 2 ** 31:
-        raise ValueError(f"group_norm takes up to {_MAX_NORM_CHANNELS} channels and 2^31 - 1 rows, got [{M}, {C}]")
+    if C > _MAX_NORM_CHANNELS or M > _MAX_NORM_ROWS:
+        raise ValueError(f"group_norm takes up to {_MAX_NORM_CHANNELS} channels and 2^31 - 65536 rows, got [{M}, {C}]")
     if seg_off.dtype != torch.int32 or seg_off.dim() != 1 or seg_off.numel() < 1 or not seg_off.is_contiguous():
         raise ValueError("seg_off has to be a contiguous int32 tensor [B + 1]")
+    if (seg_off.numel() - 1) * num_groups > _MAX_NORM_ROWS:
+        raise ValueError(f"group_norm takes up to 2^31 - 65536 clouds times groups, got {seg_off.numel() - 1} x {num_groups}")
     for t in (weight, bias):
         if t is not None and (t.numel() != C or (t.dtype is not _F32 and t.dtype is not x.dtype)):
             raise ValueError(f"weight and bias have to hold {C} values in float32 or {x.dtype}")

@@ -266,7 +266,8 @@ int dd3d_global_avg_pool_bwd(const float* g, int64_t M, const int32_t* seg_off, 
  * [j*C/G, (j+1)*C/G).  Biased variance over the rows of a cloud and the channels of a group; statistics, sums and the activation in fp32,
  * one rounding to dtype at the end.  weight / bias: [C], nullable, both of type pdtype (0, or dtype).  act: 0 none, 1 ReLU, 2 leaky ReLU
  * (slope below zero), 3 SiLU, 4 GELU (the normal distribution's).  p, key: as in dd3d_dropout (key nullable with p = 0).
- * Rows of [0, M) that belong to no cloud come out as zeros; rows from M on are not touched.  C <= 4096, M < 2^31, eps >= 2^-126.
+ * Rows of [0, M) that belong to no cloud come out as zeros; rows from M on are not touched.  C <= 4096, M and B*G <= 2^31 - 65536,
+ * eps >= 2^-126.
  *   fwd : Y = dropout(act(xhat*weight + bias)); mean / rstd [B,G] fp32 are kept for the gradients (nullable pair; zeros for an empty cloud)
  *   bwd : dX (nullable), dweight / dbias [C] in pdtype (each nullable) from dY
  *   bwd2: the gradient of bwd: from the cotangents ggX[M,C], ggW[C], ggB[C] of its three results (each nullable) the cotangents of its

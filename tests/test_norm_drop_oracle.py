@@ -111,6 +111,30 @@ def test_c_entry_points_refuse_bad_arguments_before_any_launch():
     assert lib.dd3d_random_key(None, one, None) == -1
 
 
+def test_rows_and_clouds_whose_counters_would_leave_32_bits_are_refused():
+    """A walk over rows steps by up to 4096 (a chunk), one over clouds by up to 32 768 (a launch's workgroups), and tests for the end after the step."""
+    from dd3d_amd import _lib as L, ops
+    lib, one, most = L.lib, 256, 2 ** 31 - 65536
+    assert most - 1 + 32768 < 2 ** 31
+    ws = lib.dd3d_group_norm_ws_bytes
+    for order in (0, 1, 2):
+        assert ws(most, 1, 1, 1, order) >= 0 and ws(1000, 1, most, 1, order) >= 0 and ws(1000, 8, most // 8, 8, order) >= 0
+        for bad in ((most + 1, 1, 1, 1), (2 ** 31 - 1, 1, 1, 1), (1000, 1, most + 1, 1), (1000, 1, 2 ** 31 - 1, 1), (1000, 8, most // 8 + 1, 8)):
+            assert ws(*bad, order) == -2, bad
+    for M, B in ((most + 1, 1), (2 ** 31 - 1, 1), (10, most + 1), (10, 2 ** 31 - 1)):
+        head = (0, M, 1, one, B, 1, one, one, 0)
+        assert lib.dd3d_group_norm_fwd(one, *head, 1e-5, 0, 0.0, 0.0, None, one, None, None, None, 0, None) == -2
+        assert lib.dd3d_group_norm_bwd(one, one, *head, 0, 0.0, 0.0, None, one, one, one, one, one, None, 0, None) == -2
+        assert lib.dd3d_group_norm_bwd2(None, None, None, one, one, *head, 0, 0.0, 0.0, None, one, one, one, one, one, one, None, 0, None) == -2
+    rows, seg = torch.empty(most + 1, 1, device="meta"), torch.empty(2, dtype=torch.int32, device="meta")
+    with pytest.raises(ValueError, match="rows"):
+        ops.group_norm(rows, seg, 1)
+    with pytest.raises(ValueError, match="clouds times groups"):
+        ops.group_norm(rows[:10], torch.empty(most + 2, dtype=torch.int32, device="meta"), 1)
+    with pytest.raises(ValueError, match="clouds times groups"):
+        ops.group_norm(torch.empty(10, 8, device="meta"), torch.empty(most // 8 + 2, dtype=torch.int32, device="meta"), 8)
+
+
 def test_python_entry_points_refuse_bad_arguments():
     from dd3d_amd import nn as ME, ops
     x, seg, key = torch.zeros(6, 8), torch.tensor([0, 6], dtype=torch.int32), torch.zeros(2, dtype=torch.int64)

@@ -112,18 +112,17 @@ __device__ __forceinline__ float activate(float u, float slope, float* d1, float
         if (ORDER == 2) *d2 = ds * fmaf(u, 1.f - 2.f * s, 2.f);
         return u * s;
     }
-    // From 14 on the exponential is zero, and at 64 it multiplies numbers that are still finite: u = inf gives inf (-inf, as SiLU's, inf * 0), and u^2
-    // of a huge u does not leave fp32.  NaN stays NaN in both bounds.
-    const float a = __builtin_elementwise_minimum(fabsf(u), 64.f);
+    // From 14 on e is zero, so what it multiplies may be bounded there: infinite u give their limits (inf and 0), and u^2 of a huge u does not
+    // leave fp32.  (A NaN that a bound swallows is still in e.)
+    const float a = fabsf(u), near = fminf(a, 64.f);
     float e, pt;
     normal_tail<SHORT && ORDER == 0>(a, &e, &pt);
     if (ORDER >= 1) {
         const float r = e * fmaf(a, 0.39894228f, -pt);
         *d1 = u > 0.f ? 1.f + r : -r;
     }
-    if (ORDER == 2) *d2 = 0.39894228f * e * fmaf(-a, a, 2.f);
-    const float up = u - __builtin_elementwise_minimum(u, 0.f);
-    return fmaf(-a, e * pt, up);
+    if (ORDER == 2) *d2 = 0.39894228f * e * fmaf(-near, near, 2.f);
+    return fmaf(-near, e * pt, fmaxf(u, 0.f));
 }
 
 // ---- random words ---------------------------------------------------------------------------------------------------------------

@@ -37,3 +37,11 @@ def test_huge_finite_preactivations_twice_differentiated(act, dtype):
     seg, t = batch(MIXED, 8, dtype, seed=32)
     t["b"] = torch.tensor([1e20, -1e20, 3e38, -3e38, 2e19, -2e19, 0.5, -0.5])
     check(through_autograd(t, seg_on_device(seg), 8, 2, activation=act, eps=1e-2), seg, t, 8, act, eps=1e-2)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_gelu_at_minus_infinity_is_its_limit(dtype):
+    from dd3d_amd import ops
+    seg, t = batch(MIXED, 8, dtype, seed=36)
+    y = ops.group_norm(t["x"].to(dev()), seg_on_device(seg), 2, None, torch.full((8,), -math.inf, device=dev()), activation="gelu")
+    assert not y.any()

@@ -14,7 +14,8 @@
 //     one it begins in (slot 2w) and one that begins inside it (slot 2w + 1).  Windows write partial sums, a second launch joins them
 //     (every workgroup for itself, in window order) and walks the rows again.  Which clouds are large is read from seg_off on the device.
 // Sums are fp32: per thread over its rows, then lanes, waves, windows in a fixed order.  Variances come from differences to a mean
-// at every level (thread, workgroup, windows), never from a mean of squares.
+// at every level (thread, workgroup, windows), never from a mean of squares; and the mean of those differences is added to the mean they were
+// taken to, so that neither the sum's roundings nor a reciprocal's stay in it: a constant cloud is centred to zeros.
 #pragma once
 #include "feature_math.h"
 
@@ -605,6 +606,13 @@ __device__ __forceinline__ void fold_slots(const Norm& a, const Geo& g, const Wo
 }
 
 // ---- forward --------------------------------------------------------------------------------------------------------------------
+// The sum of squares about the mean, from the sums `e` of differences and `q` of their squares about a shift that lies shift = e / n below the mean.
+// What is left below the roundings of q (2^-18: some sixty half steps) is nothing: of equal values only those are left.
+__device__ __forceinline__ float about_mean(float q, float e, float shift) {
+    const float r = fmaf(-e, shift, q);
+    return r < q * 0x1p-18f ? 0.f : r;
+}
+
 template <typename Z>
 struct Fwd {
     typedef typename Z::T T;
@@ -618,11 +626,11 @@ struct Fwd {
     PhiloxKey key;
 
     // per-thread count, mean and centred sum of squares, joined with those of one more chunk
-    __device__ __forceinline__ void add_rows(int all, const typename Z::Row (&z)[NR], float& cnt, float (&mu)[NS], float (&m2)[1][NS]) {
+    __device__ __forceinline__ void add_rows(int all, const typename Z::Row (&z)[NR], float& cnt, float (&mu)[NS], float (&m2)[NS]) {
         const int left = s.on ? all : 0;
-        float n1 = 0.f, sx[NS], q[NS];
+        float n1 = 0.f, sx[NS], e[NS], q[NS];
 #pragma unroll
-        for (int i = 0; i < NS; ++i) sx[i] = q[i] = 0.f;
+        for (int i = 0; i < NS; ++i) sx[i] = e[i] = q[i] = 0.f;
 #pragma unroll
         for (int n = 0; n < NR; ++n) {
             if (n * g.RL >= all) break;
@@ -631,8 +639,8 @@ struct Fwd {
             for (int i = 0; i < V; ++i) sx[Z::at(i)] += raw_get(z[n], i);   // (zeros past the end)
         }
         if (n1 == 0.f) return;
-        // (reciprocals to a step: any shift near the mean serves the sum of squares)
-        const float inv = __builtin_amdgcn_rcpf(n1), sum = cnt + n1, part = n1 * __builtin_amdgcn_rcpf(sum), cross = cnt * part;
+        // (reciprocals to a step: sx need only be near the chunk's mean; the first chunk's is taken as it is)
+        const float inv = __builtin_amdgcn_rcpf(n1), sum = cnt + n1, part = cnt > 0.f ? n1 * __builtin_amdgcn_rcpf(sum) : 1.f, cross = cnt * part;
 #pragma unroll
         for (int i = 0; i < NS; ++i) sx[i] *= inv;
 #pragma unroll
@@ -642,47 +650,62 @@ struct Fwd {
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
                     const float d = raw_get(x, i) - sx[Z::at(i)];
+                    e[Z::at(i)] += d;
                     q[Z::at(i)] = fmaf(d, d, q[Z::at(i)]);
                 }
             }
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
-            const float d = sx[i] - mu[i];
+            const float shift = e[i] * inv, d = sx[i] + shift - mu[i];
             mu[i] = fmaf(d, part, mu[i]);
-            m2[0][i] += fmaf(d * d, cross, q[i]);
+            m2[i] += fmaf(d * cross, d, about_mean(q[i], e[i], shift));
         }
         cnt = sum;
     }
 
-    // the thread's part -> v[0] = mean, v[1] = centred sum of squares of its groups over `rows` rows
-    __device__ __forceinline__ void join(int rows, float cnt, const float (&mu)[NS], float (&m2)[1][NS], float (&v)[2][NS]) {
-        const float inv = 1.f / ((float)rows * (float)a.Cg);
-        float sum[1][NS];
+    // A value next to the mean that all threads of a group know: its first channel in the first row.  Sums over threads are of differences to it, so
+    // that equal means add up to exactly that mean.
+    __device__ __forceinline__ void reference(int row, float (&k)[NS]) {
+        const T* at = X + row_at(a, row) + s.s0;
 #pragma unroll
-        for (int i = 0; i < NS; ++i) sum[0][i] = cnt * mu[i];
+        for (int i = 0; i < NS; ++i) k[i] = widen(at[s.j[i] * a.Cg]);
+    }
+
+    // the thread's part -> v[0] = mean, v[1] = centred sum of squares of its groups over `rows` rows
+    __device__ __forceinline__ void join(int rows, const float (&k)[NS], float cnt, const float (&mu)[NS], const float (&m2)[NS], float (&v)[2][NS]) {
+        const float inv = 1.f / ((float)rows * (float)a.Cg);
+        float sum[1][NS], eq[2][NS];
+#pragma unroll
+        for (int i = 0; i < NS; ++i) sum[0][i] = cnt * (mu[i] - k[i]);
         group_sums<1, Z>(sum, a, g, s, lds);
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
-            v[0][i] = sum[0][i] * inv;
+            v[0][i] = fmaf(sum[0][i], inv, k[i]);
             const float d = mu[i] - v[0][i];
-            m2[0][i] = cnt > 0.f ? fmaf(d * cnt, d, m2[0][i]) : 0.f;
+            eq[0][i] = d * cnt;
+            eq[1][i] = cnt > 0.f ? fmaf(eq[0][i], d, m2[i]) : 0.f;
         }
-        group_sums<1, Z>(m2, a, g, s, lds);
+        group_sums<2, Z>(eq, a, g, s, lds);
 #pragma unroll
-        for (int i = 0; i < NS; ++i) v[1][i] = m2[0][i];
+        for (int i = 0; i < NS; ++i) {
+            const float shift = eq[0][i] * inv;
+            v[0][i] += shift;
+            v[1][i] = about_mean(eq[1][i], eq[0][i], shift);
+        }
     }
 
     // statistics of rows that take several chunks
     __device__ __forceinline__ void stats(const Range& r, float (&v)[2][NS]) {
-        float cnt = 0.f, mu[NS], m2[1][NS];
+        float cnt = 0.f, k[NS], mu[NS], m2[NS];
+        reference(r.r0, k);
 #pragma unroll
-        for (int i = 0; i < NS; ++i) mu[i] = m2[0][i] = 0.f;
+        for (int i = 0; i < NS; ++i) mu[i] = m2[i] = 0.f;
         for (int base = r.r0; base < r.r1; base += NR * g.RL) {
             typename Z::Row z[NR];
             Chunk<Z>(X + row_at(a, base), a.C, r.r1 - base, g).load_all(g, s, z);
             add_rows(r.r1 - base, z, cnt, mu, m2);
         }
-        join(r.r1 - r.r0, cnt, mu, m2, v);
+        join(r.r1 - r.r0, k, cnt, mu, m2, v);
     }
 
     // 1 / standard deviation from v of a whole cloud of `rows` rows; `keep`: this workgroup writes the statistics
@@ -712,11 +735,12 @@ struct Fwd {
         const int rows = r.r1 - r.r0;
         typename Z::Row z[NR];
         Chunk<Z>(X + row_at(a, r.r0), a.C, rows, g).load_all(g, s, z);
-        float cnt = 0.f, mu[NS], m2[1][NS], v[2][NS], rstd[NS];
+        float cnt = 0.f, k[NS], mu[NS], m2[NS], v[2][NS], rstd[NS];
+        reference(r.r0, k);
 #pragma unroll
-        for (int i = 0; i < NS; ++i) mu[i] = m2[0][i] = 0.f;
+        for (int i = 0; i < NS; ++i) mu[i] = m2[i] = 0.f;
         add_rows(rows, z, cnt, mu, m2);
-        join(rows, cnt, mu, m2, v);
+        join(rows, k, cnt, mu, m2, v);
         finish(v, b, rows, true, mean_out, rstd_out, rstd);
         rows_out(r.r0, rows, v[0], rstd, z);
     }
@@ -803,9 +827,11 @@ __global__ __launch_bounds__(Z::THREADS, Z::FWD_WAVES) void k_fwd(Norm a, Geo g,
         for (int j = s.wave; j < s.gs; j += Z::WAVES) {
             const float* from = part + (s.slab * g.k + j) * 2;
             const float inv = 1.f / (float)rows;
-            float m = 0.f, m2 = 0.f;
+            float m = 0.f, e = 0.f, m2 = 0.f;
             for (int o = s.lane; o < n; o += 64) m = fmaf(from[(int64_t)piece_slot(g, q.all, o) * a.G * 2], (float)piece_rows(g, q.all, o) * inv, m);
             m = wave_sum(m);
+            for (int o = s.lane; o < n; o += 64) e = fmaf(from[(int64_t)piece_slot(g, q.all, o) * a.G * 2] - m, (float)piece_rows(g, q.all, o) * inv, e);
+            m += wave_sum(e);
             for (int o = s.lane; o < n; o += 64) {
                 const float* z = from + (int64_t)piece_slot(g, q.all, o) * a.G * 2;
                 const float d = z[0] - m;

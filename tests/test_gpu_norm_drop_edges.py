@@ -45,3 +45,61 @@ def test_gelu_at_minus_infinity_is_its_limit(dtype):
     seg, t = batch(MIXED, 8, dtype, seed=36)
     y = ops.group_norm(t["x"].to(dev()), seg_on_device(seg), 2, None, torch.full((8,), -math.inf, device=dev()), activation="gelu")
     assert not y.any()
+
+
+# ------------------------------------------------------------------------------------------------------------ clouds without spread
+LENGTHS = [32, 5, 1, 82, 700, 3001, 9000, 20011]
+
+
+@pytest.mark.parametrize("C,G", [(16, 4), (16, 1), (7, 7), (24, 2), (12, 3), (128, 8), (128, 32), (2048, 1)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("value", [100.3, 3.1, -1e17])
+def test_a_constant_cloud_is_a_cloud_of_zeros(C, G, dtype, value):
+    """x - mean is zero whatever the constant, also where neither it nor 1 / count is a sum of few powers of two: value and gradients
+    are those of a cloud of zeros, bit for bit."""
+    lens = LENGTHS if C <= 128 else [82, 5, 1500]
+    seg, t = batch(lens, C, dtype, seed=33)
+    so = seg_on_device(seg)
+    t["x"] = torch.zeros_like(t["x"])
+    want = through_autograd(t, so, G, 2, activation="silu")
+    t["x"] = torch.full_like(t["x"], value)
+    got = through_autograd(t, so, G, 2, activation="silu")
+    for k in want:
+        assert torch.equal(got[k], want[k]), k
+
+
+@pytest.mark.parametrize("lens,C,G", [([32, 45, 7, 1, 60], 16, 4), ([82] * 50, 128, 8), ([30, 9], 10, 5)])
+@pytest.mark.parametrize("shift", [3000.0, 1e6])
+def test_the_mean_is_off_by_its_own_rounding(lens, C, G, shift):
+    """A thread's mean is corrected by the mean of its differences and rounded once, and so is the cloud's: two half steps, and the
+    differences' own roundings (at most 2^10 additions of numbers below 2^4: less than an eighth of the half step at 3000)."""
+    from dd3d_amd import _lib as L
+    seg, t = batch(lens, C, F32, seed=34)
+    x, so, B, M = (t["x"].clamp(-7, 7) + shift).to(dev()), seg_on_device(seg), len(lens), seg[-1]
+    y, mean, rstd = torch.empty_like(x), torch.empty(B, G, device=dev()), torch.empty(B, G, device=dev())
+    n = L.lib.dd3d_group_norm_ws_bytes(M, C, B, G, 0)
+    ws = torch.empty(max(1, n), dtype=torch.uint8, device=dev())
+    L.call("dd3d_group_norm_fwd", L.ptr(x), 0, M, C, L.ptr(so), B, G, None, None, 0, 1e-5, 0, 0.0, 0.0, None, L.ptr(y), L.ptr(mean), L.ptr(rstd), L.ptr(ws),
+           ws.numel(), L.stream())
+    half = 2.0 ** (math.floor(math.log2(shift)) - 24)
+    for b, (r0, r1) in enumerate(zip(seg[:-1], seg[1:])):
+        want = x[r0:r1].double().reshape(r1 - r0, G, -1).mean((0, 2))
+        assert float((mean[b].double() - want).abs().max()) <= 2.125 * half
+
+
+def test_a_spike_in_a_clouds_first_element_costs_no_accuracy():
+    """The first element serves as a reference for the sums; every element but that one lies next to the mean in units of the spread, and its
+    value comes out to the roundings of the mean (two half steps of |mean|) and of its own three operations."""
+    from dd3d_amd import ops
+    seg, t = batch([82, 700, 9000], 16, F32, seed=37)
+    for r in seg[:-1]:
+        t["x"][r, ::4] = 1e6
+    y = ops.group_norm(t["x"].to(dev()), seg_on_device(seg), 4).cpu().double()
+    for r0, r1 in zip(seg[:-1], seg[1:]):
+        x = t["x"][r0:r1].double().reshape(r1 - r0, 4, 4)
+        mean = x.mean((0, 2), keepdim=True)
+        sd = torch.sqrt(((x - mean) ** 2).mean((0, 2), keepdim=True) + 1e-5)
+        want = (x - mean) / sd
+        # (the spread is a sum of squares of at most 2^18 elements, some 30 half steps in partial sums)
+        allow = (4 * mean.abs() / sd + 40 * want.abs()) * 2.0 ** -24
+        assert bool(((y[r0:r1].reshape(r1 - r0, 4, 4) - want).abs() <= allow).all())

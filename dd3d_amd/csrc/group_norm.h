@@ -848,6 +848,14 @@ __global__ __launch_bounds__(Z::THREADS, Z::FWD_WAVES) void k_fwd(Norm a, Geo g,
     }
 }
 
+// 1 / standard deviation for one row; zero for a row that is not there: what stands in for its values is read as zeros, which may lie as far from the
+// mean as fp32 goes in units of the spread, and only times a finite number do its dy = 0 and P = 0 add nothing.
+template <int NS>
+__device__ __forceinline__ void row_rstd(const float (&rstd)[NS], bool there, float (&rs)[NS]) {
+#pragma unroll
+    for (int i = 0; i < NS; ++i) rs[i] = there ? rstd[i] : 0.f;
+}
+
 // ---- first gradient -------------------------------------------------------------------------------------------------------------
 // Bound by HBM and, at two to three waves per SIMD, by the latency of its loads; with dropout by vector instructions (30% of the cycles of
 // all waves).  What a thread keeps of a row between the sums and the result: the normalised values and g (fp32 rows: in the registers the loaded rows
@@ -887,11 +895,11 @@ struct Bwd {
     }
 
     // xh and g of one row
-    __device__ __forceinline__ void element(const typename Z::Row& x, float (&xh)[V], float (&gr)[V]) {   // gr: dy after dropout -> g
+    __device__ __forceinline__ void element(const typename Z::Row& x, const float (&rs)[NS], float (&xh)[V], float (&gr)[V]) {   // gr: dy after dropout -> g
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             float d1, d2;
-            xh[i] = (raw_get(x, i) - mean[Z::at(i)]) * rstd[Z::at(i)];
+            xh[i] = (raw_get(x, i) - mean[Z::at(i)]) * rs[Z::at(i)];
             activate<Z::FAM, 1>(fmaf(xh[i], s.w[i], s.b[i]), a.slope, &d1, &d2);
             gr[i] *= d1;
         }
@@ -904,10 +912,11 @@ struct Bwd {
 #pragma unroll
         for (int i = 0; i < (HOLD ? 1 : (NR * V + 31) / 32); ++i) h.keep[i] = 0;
 #pragma unroll
-        for (int n = 0; n < NR; ++n) {   // (a row past the end has dy = 0 and adds nothing)
+        for (int n = 0; n < NR; ++n) {   // (a row past the end has dy = 0 and xh = 0, and adds nothing)
             row_border();
             if (n * g.RL >= all) break;
-            float xh[V], gr[V];
+            float xh[V], gr[V], rs[NS];
+            row_rstd(rstd, s.rl < all - n * g.RL, rs);
 #pragma unroll
             for (int i = 0; i < V; ++i) gr[i] = raw_get(h.d[n], i);
             if (a.drop.key) {
@@ -915,7 +924,7 @@ struct Bwd {
                 rnd.drop(a.drop, gr);
                 if (!HOLD) h.keep[n * V / 32] |= rnd.bits(a.drop) << (n * V % 32);
             }
-            element(h.x[n], xh, gr);
+            element(h.x[n], rs, xh, gr);
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 const float t = gr[i] * s.w[i];
@@ -946,7 +955,7 @@ struct Bwd {
                 for (int i = 0; i < V; ++i) gr[i] = raw_get(d, i);
                 if (!fresh) drop_row<V>(a.drop, h.keep[HOLD ? 0 : n * V / 32] >> (n * V % 32), gr);
                 else if (a.drop.key) Words<V>(key, words + (word + n * (uint32_t)(g.RL * g.quads))).drop(a.drop, gr);
-                element(x, xh, gr);
+                element(x, rstd, xh, gr);   // (a row past the end is not stored)
             }
 #pragma unroll
             for (int i = 0; i < V; ++i) dx[i] = rstd[Z::at(i)] * fmaf(gr[i], s.w[i], -fmaf(xh[i], m2[Z::at(i)], m1[Z::at(i)]));
@@ -1114,10 +1123,11 @@ struct Bwd2 {
 
     // one row: values after dropout, and the activation's derivatives element by element
     struct RowOf {
-        float x[V], p[V], dy[V];
+        float x[V], p[V], dy[V], rs[NS];
     };
-    __device__ __forceinline__ RowOf row_of(const typename Z::Row& x, const typename Z::Row& d, const typename Z::Row& p, uint32_t keep) {
+    __device__ __forceinline__ RowOf row_of(const typename Z::Row& x, const typename Z::Row& d, const typename Z::Row& p, uint32_t keep, bool there) {
         RowOf r;
+        row_rstd(rstd, there, r.rs);
 #pragma unroll
         for (int i = 0; i < V; ++i) r.x[i] = raw_get(x, i), r.dy[i] = raw_get(d, i), r.p[i] = raw_get(p, i);
         drop_row<V>(a.drop, keep, r.dy);
@@ -1128,7 +1138,7 @@ struct Bwd2 {
     };
     __device__ __forceinline__ Elem element(const RowOf& r, int i) {
         Elem e;
-        e.xh = (r.x[i] - mean[Z::at(i)]) * rstd[Z::at(i)];
+        e.xh = (r.x[i] - mean[Z::at(i)]) * r.rs[Z::at(i)];
         e.p = r.p[i], e.dy = r.dy[i];
         activate<Z::FAM, 2>(fmaf(e.xh, s.w[i], s.b[i]), a.slope, &e.d1, &e.d2);
         return e;
@@ -1136,11 +1146,11 @@ struct Bwd2 {
 
     __device__ __forceinline__ void add_rows(int all, const Held& h, float (&v)[KS][NS], bool to_lds) {
 #pragma unroll
-        for (int n = 0; n < NR; ++n) {   // (a row past the end has dy = P = 0 and adds nothing)
+        for (int n = 0; n < NR; ++n) {   // (a row past the end has dy = P = xh = 0 and adds nothing)
             row_border();
             if (n * g.RL >= all) break;
             if (HOLD && to_lds) mine[3 * n * Z::THREADS] = h.x[n], mine[(3 * n + 1) * Z::THREADS] = h.d[n], mine[(3 * n + 2) * Z::THREADS] = h.p[n];
-            const RowOf row = row_of(h.x[n], h.d[n], h.p[n], h.keep[n * V / 32] >> (n * V % 32));
+            const RowOf row = row_of(h.x[n], h.d[n], h.p[n], h.keep[n * V / 32] >> (n * V % 32), s.rl < all - n * g.RL);
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 row_border();
@@ -1186,7 +1196,7 @@ struct Bwd2 {
             typename Z::Row x = again(h.x[n]), d = again(h.d[n]), p = again(h.p[n]);
             if (HOLD && from_lds) x = mine[3 * n * Z::THREADS], d = mine[(3 * n + 1) * Z::THREADS], p = mine[(3 * n + 2) * Z::THREADS];
             const uint32_t keep = h.keep[n * V / 32] >> (n * V % 32);
-            const RowOf row = row_of(x, d, p, keep);
+            const RowOf row = row_of(x, d, p, keep, s.rl < all - n * g.RL);
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 row_border();

@@ -103,3 +103,20 @@ def test_a_spike_in_a_clouds_first_element_costs_no_accuracy():
         # (the spread is a sum of squares of at most 2^18 elements, some 30 half steps in partial sums)
         allow = (4 * mean.abs() / sd + 40 * want.abs()) * 2.0 ** -24
         assert bool(((y[r0:r1].reshape(r1 - r0, 4, 4) - want).abs() <= allow).all())
+
+
+@pytest.mark.parametrize("act", ["none", "silu", "gelu"])
+@pytest.mark.parametrize("value,eps", [(2.0 ** 57, 1e-5), (2.0 ** 20, 1e-30), (2.0 ** 70, 1e-36)])
+@pytest.mark.parametrize("C,G,dtype", [(16, 4, F32), (9, 3, F32), (32, 2, BF16)])
+def test_rows_that_are_not_there_add_nothing_to_a_constant_cloud(act, value, eps, C, G, dtype):
+    """Zeros stand in for rows behind a chunk's last one.  They lie far from a constant cloud's mean in units of its spread, and what is
+    computed from them may leave fp32; the gradients stay those of a cloud of zeros."""
+    seg, t = batch([32, 5, 700, 9000], C, dtype, seed=35)
+    so = seg_on_device(seg)
+    t["x"] = torch.zeros_like(t["x"])
+    want = through_autograd(t, so, G, 2, 0.2, activation=act, eps=eps)
+    assert all(bool(torch.isfinite(v).all()) for v in want.values())
+    t["x"] = torch.full_like(t["x"], value)
+    got = through_autograd(t, so, G, 2, 0.2, activation=act, eps=eps)
+    for k in want:
+        assert torch.equal(got[k], want[k]), k

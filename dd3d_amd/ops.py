@@ -16,7 +16,7 @@ from functools import lru_cache
 from typing import NamedTuple, Optional
 
 import torch
-from torch.autograd import Function
+from torch.autograd import Function, forward_ad
 from torch.autograd.function import once_differentiable
 from torch.autograd.graph import increment_version
 
@@ -463,6 +463,12 @@ def _same_device(x: torch.Tensor, **others):
             raise ValueError(f"{name} is on {t.device}, the rows are on {x.device}")
 
 
+def _no_tangents(*ts):
+    """A kernel's result has no tangent: an input that has one is refused, inside a Function or where the Function is passed by."""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in ts):
+        raise NotImplementedError("group_norm and dropout have no forward-mode derivative")
+
+
 def _check_p(p) -> float:
     if not 0.0 <= float(p) <= 1.0:
         raise ValueError(f"dropout probability has to be between 0 and 1, got {p}")
@@ -513,6 +519,7 @@ class DropoutFn(Function):
 
 
 def _dropout_raw(x, p, key):
+    _no_tangents(x)
     if not x.is_contiguous():
         x = x.contiguous()
     y = torch.empty_like(x)
@@ -576,6 +583,7 @@ def _addr(t):
 
 
 def _norm_fwd(x, w, b, seg_off, key, meta, eps, keep):
+    _no_tangents(x, w, b)
     x, w, b = _dense(x), _dense(w), _dense(b)
     dev = x.device
     y = torch.empty_like(x)
@@ -592,6 +600,7 @@ def _stats(stats):
 
 
 def _norm_grad(dy, x, w, b, seg_off, key, stats, meta, need):
+    _no_tangents(dy, x, w, b)
     dy, x, w, b = _dense(dy), _dense(x), _dense(w), _dense(b)
     dev = x.device
     dx = torch.empty_like(x) if need[0] else None
@@ -634,6 +643,7 @@ class _GroupNormGradFn(Function):
     @once_differentiable
     def backward(ctx, ggx, ggw, ggb):
         dy, x, w, b, seg_off, key, stats = ctx.saved_tensors
+        _no_tangents(ggx, ggw, ggb, dy, x, w, b)
         meta, need = ctx.meta, ctx.needs_input_grad
         dy, x, w, b, ggx, ggw, ggb = _dense(dy), _dense(x), _dense(w), _dense(b), _dense(ggx), _dense(ggw), _dense(ggb)
         dev = x.device

@@ -7,7 +7,7 @@ import torch
 pytestmark = pytest.mark.gpu
 
 from oracle import norm_drop_ref as R
-from tests.test_gpu_norm_drop import BF16, F16, F32, MIXED, batch, check, dev, through_autograd
+from tests.test_gpu_norm_drop import BF16, F16, F32, MIXED, batch, check, dev, key, through_autograd
 
 
 def seg_on_device(seg):
@@ -120,3 +120,33 @@ def test_rows_that_are_not_there_add_nothing_to_a_constant_cloud(act, value, eps
     got = through_autograd(t, so, G, 2, 0.2, activation=act, eps=eps)
     for k in want:
         assert torch.equal(got[k], want[k]), k
+
+
+# ------------------------------------------------------------------------------------------------------- forward-mode derivatives
+def test_forward_mode_derivatives_are_refused_not_lost():
+    from torch.autograd import forward_ad
+    from dd3d_amd import ops
+    x, so = torch.randn(40, 8, device=dev()), torch.tensor([0, 40], dtype=torch.int32, device=dev())
+    w, v = torch.ones(8, device=dev()), torch.randn(40, 8, device=dev())
+    k = key()
+    want = ops.group_norm(x, so, 2, w), ops.dropout(x, 0.3, k)
+    with forward_ad.dual_level():
+        xd, wd = forward_ad.make_dual(x, v), forward_ad.make_dual(w, torch.ones_like(w))
+        calls = [lambda: ops.dropout(xd, 0.3, k), lambda: ops.group_norm(xd, so, 2, w), lambda: ops.group_norm(x, so, 2, wd),
+                 lambda: ops.group_norm(x, so, 2, None, wd)]
+        for call in calls:
+            with pytest.raises(NotImplementedError):
+                call()
+            with torch.no_grad(), pytest.raises(NotImplementedError):
+                call()
+        # a tangent on the incoming gradient, in the first and in the second backward pass
+        xr, gd = x.clone().requires_grad_(), forward_ad.make_dual(torch.ones_like(x), v)
+        for y in (ops.dropout(xr, 0.3, k), ops.group_norm(xr, so, 2, w)):
+            for again in (False, True):
+                with pytest.raises(NotImplementedError):
+                    torch.autograd.grad(y, xr, gd, retain_graph=True, create_graph=again)
+        dx, = torch.autograd.grad(ops.group_norm(xr, so, 2, w), xr, v, create_graph=True)
+        with pytest.raises(NotImplementedError):
+            torch.autograd.grad(dx, xr, gd)
+        # without a tangent the calls are the ordinary ones
+        assert torch.equal(ops.group_norm(x, so, 2, w), want[0]) and torch.equal(ops.dropout(x, 0.3, k), want[1])

@@ -44,11 +44,6 @@ __device__ __forceinline__ float widen_bits(uint16_t h, int dt) {
 }
 
 // parameter vectors (weight, bias and their gradients) are fp32 or of the rows' type: a code, uniform over the launch
-__device__ __forceinline__ float load_param(const void* p, int pdt, int64_t i) {
-    if (pdt == DD3D_F32) return ((const float*)p)[i];
-    if (pdt == DD3D_F16) return widen(((const half_t*)p)[i]);
-    return widen(((const bf16_t*)p)[i]);
-}
 __device__ __forceinline__ void store_param(void* p, int pdt, int64_t i, float v) {
     if (pdt == DD3D_F32) ((float*)p)[i] = v;
     else if (pdt == DD3D_F16) ((half_t*)p)[i] = narrow<half_t>(v);
@@ -65,9 +60,11 @@ __device__ __forceinline__ void store_param(void* p, int pdt, int64_t i, float v
 __host__ __device__ __forceinline__ int act_family(int act) { return act <= DD3D_ACT_LEAKY ? DD3D_FAM_LINEAR : act == DD3D_ACT_SILU ? DD3D_FAM_SILU : DD3D_FAM_GELU; }
 
 // The upper tail Q(a) = 1 - Phi(a) of the normal distribution, a = |u|, is n-shaped: Q(a) = exp(-a^2 / 2) t P(t) with t = 1 / (1 + 0.35 a) and P a
-// degree-8 polynomial fitted for least relative error over a in [0, 14] (3.2e-8).  So the far tail keeps its relative accuracy, one
-// exponential serves Phi and the density alike, and on either side only one subtraction is left:
+// degree-8 polynomial fitted for least relative error over a in [0, 14] (6.1e-8 with the coefficients as printed).  So one exponential serves Phi
+// and the density alike, and on either side only one subtraction is left:
 //   u Phi(u) = max(u, 0) - a Q(a),   Phi(u) + u n(u) = u > 0 ? 1 + r : -r,  r = a n(a) - Q(a),   2 n - u^2 n = n (2 - u^2).
+// The exponent is a product of rounded numbers, off by up to five half steps of a^2 / 2, and so is Q, relative to itself: 3e-6 at a = 6, 1.3e-5 at 13, where
+// Q is 1e-9 and 6e-39.  Carrying the square's residual would take five instructions more in every GELU.
 // SHORT: results that are rounded to half width take degree 5 over t = 1 / (1 + 0.3 a), relative error 8.2e-6, a sixtieth of fp16's half step.
 template <bool SHORT>
 __device__ __forceinline__ void normal_tail(float a, float* e, float* pt) {

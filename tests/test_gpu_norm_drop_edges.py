@@ -40,6 +40,41 @@ def test_huge_finite_preactivations_twice_differentiated(act, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+def test_the_activations_element_by_element(act, dtype):
+    """weight = 0 makes the bias the pre-activation, and each result is held against its own size, not its cloud's.  GELU's tail Q = e t P(t): the
+    exponent a^2 / 2 is off by 5 half steps of itself (two roundings of the factor, squared, and one of the square); the hardware's exponential and
+    reciprocal, nine steps of the polynomial and two products come to less than 24 half steps; the short polynomial for half-width values is off by
+    8.3e-6.  SiLU's exponent u is off by 2 half steps, its exponential, sum, reciprocal and product by less than 12."""
+    from dd3d_amd import ops
+    C = 4096
+    u = torch.linspace(-12, 12, C)
+    b = u.to(dev()).requires_grad_()
+    x = torch.randn(3, C, generator=torch.Generator().manual_seed(38)).to(dtype).to(dev())
+    dy = torch.zeros_like(x)
+    dy[1] = 1.0                                    # the bias' gradient is one row's derivative
+    y = ops.group_norm(x, seg_on_device([0, 3]), 64, torch.zeros(C, device=dev()), b, activation=act)
+    db, = torch.autograd.grad(y, b, dy)
+    u = u.double()
+    a, half = u.abs(), 2.0 ** -24
+    if act == "gelu":
+        tail = lambda v: torch.special.erfc(v / math.sqrt(2)) / 2  # noqa: E731  (1 + erf, and so torch's ndtr, has no digit of it left below -8)
+        Q, n = tail(a), torch.exp(-a * a / 2) / math.sqrt(2 * math.pi)
+        f, d = u * tail(-u), tail(-u) + u * n
+        steps = (2.5 * a * a + 24) * half
+        value, slope = a * Q * (steps + (8.3e-6 if dtype != F32 else 0.0)) + half * u.clamp(min=0), (Q + a * n) * steps + half * (u > 0)
+    else:
+        s = torch.sigmoid(u)
+        f, d = u * s, s * (1 + u * (1 - s))
+        steps = (2 * a + 12) * half
+        value, slope = f.abs() * steps, s * (1 + a) * steps
+    if dtype != F32:                               # the rounding to the rows' type, of fp16's subnormal numbers at least 2^-25
+        value = value + f.abs() * torch.finfo(dtype).eps / 2 * 1.001 + (2.0 ** -25 if dtype == F16 else 0.0)
+    assert bool(((y.detach().cpu().double() - f).abs() <= value).all())
+    assert bool(((db.cpu().double() - d).abs() <= slope).all())
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
 def test_gelu_at_minus_infinity_is_its_limit(dtype):
     from dd3d_amd import ops
     seg, t = batch(MIXED, 8, dtype, seed=36)

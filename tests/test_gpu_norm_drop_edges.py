@@ -7,7 +7,7 @@ import torch
 pytestmark = pytest.mark.gpu
 
 from oracle import norm_drop_ref as R
-from tests.test_gpu_norm_drop import BF16, F16, F32, MIXED, batch, check, dev, key, through_autograd
+from tests.test_gpu_norm_drop import BF16, F16, F32, MIXED, SEED, batch, check, dev, key, through_autograd
 
 
 def seg_on_device(seg):
@@ -185,3 +185,31 @@ def test_forward_mode_derivatives_are_refused_not_lost():
             torch.autograd.grad(dx, xr, gd)
         # without a tangent the calls are the ordinary ones
         assert torch.equal(ops.group_norm(x, so, 2, w), want[0]) and torch.equal(ops.dropout(x, 0.3, k), want[1])
+
+
+# ------------------------------------------------------------------------------------------------- wide slabs, and beyond 32 bits
+@pytest.mark.parametrize("C,G", [(4096, 1), (4096, 2), (2047, 1), (2052, 1)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_slabs_of_more_than_256_vectors_cut_by_windows(C, G, dtype):
+    seg, t = batch([1500, 3, 700], C, dtype, seed=39)
+    check(through_autograd(t, seg_on_device(seg), G, 2, 0.2, activation="silu"), seg, t, G, "silu", 0.2)
+
+
+def test_gradients_of_elements_beyond_32_bits():
+    """2^31 + elements: the last rows' gradients, first and second, and the mask drawn again for them.  The first cloud is all zeros with zero
+    gradients, so the parameters' are sums over the last two."""
+    from dd3d_amd import ops
+    M, C, G, p = 16_800_000, 128, 8, 0.5
+    seg, t = batch([200, 300], C, BF16, seed=40)
+    wide = lambda v: torch.cat([torch.zeros(M - 500, C, dtype=BF16, device=dev()), v.to(dev())])  # noqa: E731
+    x, dy = wide(t["x"]).requires_grad_(), wide(t["dy"]).requires_grad_()
+    w, b = t["w"].to(dev()).requires_grad_(), t["b"].to(dev()).requires_grad_()
+    y = ops.group_norm(x, seg_on_device([0, M - 500, M - 300, M]), G, w, b, activation="silu", dropout=p, key=key())
+    first = torch.autograd.grad(y, (x, w, b), dy, create_graph=True)
+    second = torch.autograd.grad(first, (dy, x, w, b), (wide(t["ggx"]), t["ggw"].to(dev()), t["ggb"].to(dev())))
+    D = R.keep_mask(500, C, p, SEED, 5, first_row=M - 500).double() / (1 - p)
+    ref = R.group_norm(t["x"], seg, G, t["w"], t["b"], name="silu", D=D, dy=t["dy"], ggx=t["ggx"], ggw=t["ggw"], ggb=t["ggb"], order=2)
+    for n, v in zip(("dx", "dw", "db", "ddy", "ddx", "ddw", "ddb"), (*first, *second)):
+        far = R.off(n, v[-500:] if v.dim() == 2 else v, ref, v.dtype, ref["cond"][0])
+        assert far <= 1, f"{n}: {far:.3g} times what its roundings allow"
+    assert not first[0][:-500].any() and not second[1][:-500].any()

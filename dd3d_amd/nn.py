@@ -97,6 +97,8 @@ class MinkowskiGroupNorm(nn.Module):
         self.register_buffer("rng_state", ops.random_state(seed) if self.dropout > 0.0 else None, persistent=False)
 
     def forward(self, x: SparseTensor) -> SparseTensor:
+        if x.F.shape[1] != self.num_channels:   # (without weight and bias nothing else would notice)
+            raise ValueError(f"a group norm of {self.num_channels} channels got {x.F.shape[1]}")
         cm, ts = x.coordinate_manager, x.tensor_stride
         p = self.dropout if self.training else 0.0
         out = ops.group_norm(x.F, cm.seg_off(ts), self.num_groups, self.weight, self.bias, self.eps, self.activation, self.negative_slope, p,

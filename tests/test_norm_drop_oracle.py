@@ -178,3 +178,15 @@ def test_modules_keep_the_norms_parameters_and_no_generator_state():
     assert torch.equal(a, ME.MinkowskiDropout().rng_state)
     assert ME.MinkowskiDropout(0.5).eval()(x := object()) is x and ME.MinkowskiDropout(0.0)(x) is x
     assert "activation=silu" in repr(m) and "p=0.5" in repr(ME.MinkowskiDropout())
+
+
+def test_the_module_takes_its_own_number_of_channels_only():
+    """Without weight and bias a tensor of another width would be normalised in groups that nobody asked for."""
+    from types import SimpleNamespace
+    from dd3d_amd import nn as ME
+    x = SimpleNamespace(F=torch.zeros(6, 16), coordinate_manager=SimpleNamespace(seg_off=lambda ts: torch.tensor([0, 6], dtype=torch.int32)), tensor_stride=1)
+    for affine in (False, True):
+        with pytest.raises(ValueError, match="8 channels got 16"):
+            ME.MinkowskiGroupNorm(2, 8, affine=affine)(x)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        ME.MinkowskiGroupNorm(2, 16, affine=False)(x)

@@ -670,7 +670,7 @@ def group_norm(x: torch.Tensor, seg_off: torch.Tensor, num_groups: int, weight: 
     if x.dim() != 2:
         raise ValueError(f"x has to be rows [M, C], got {tuple(x.shape)}")
     M, C = x.shape
-    if not 0 < num_groups <= C or C % num_groups:
+    if not 0 < num_groups <= C or C % num_groups or num_groups != int(num_groups):
         raise ValueError(f"{C} channels do not divide into {num_groups} groups")
     if C > _MAX_NORM_CHANNELS or M > _MAX_NORM_ROWS:
         raise ValueError(f"group_norm takes up to {_MAX_NORM_CHANNELS} channels and 2^31 - 65536 rows, got [{M}, {C}]")

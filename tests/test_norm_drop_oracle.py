@@ -190,3 +190,9 @@ def test_the_module_takes_its_own_number_of_channels_only():
             ME.MinkowskiGroupNorm(2, 8, affine=affine)(x)
     with pytest.raises(RuntimeError, match="no CPU fallback"):
         ME.MinkowskiGroupNorm(2, 16, affine=False)(x)
+
+
+def test_a_fraction_of_groups_is_refused_by_name():
+    from dd3d_amd import ops
+    with pytest.raises(ValueError, match="do not divide into 2.5 groups"):
+        ops.group_norm(torch.zeros(6, 5), torch.tensor([0, 6], dtype=torch.int32), 2.5)

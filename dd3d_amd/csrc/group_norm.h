@@ -87,8 +87,8 @@ __device__ __forceinline__ R again(R r) {
 }
 
 // ---- where this thread stands ---------------------------------------------------------------------------------------------------
-// The compile-time side of a launch.  NS: statistics a vector needs -- 1 where it lies inside one group (Cg % V == 0), 2 where it holds two
-// groups of four, else one per channel.  AL: whole, aligned vectors.
+// The compile-time side of a launch.  NS: statistics a vector needs -- 1 where it lies inside one group (Cg % V == 0), else one per channel.  AL:
+// whole, aligned vectors.
 // Vectors a thread holds in the three passes: vectors of four in the variants for short and for long clouds, vectors of eight; and the
 // waves per SIMD that the registers of that many rows leave.  More rows spare a long cloud its second reading until registers run out
 // (400 clouds of 750 rows of 128 fp32 channels, 8 against 16: forward 99 and 74 us, backward 152 and 126); clouds that fit 8 gain from the

@@ -57,10 +57,13 @@ inline gn::Plan plan(const gn::Norm& a, int act, int esize, bool aligned, int su
     gn::Plan p;
     gn::Geo& g = p.g;
     p.fam = act_family(act);
-    p.V = esize == 2 && aligned && a.C % 8 == 0 && ((a.Cg % 8 == 0 && a.Cg <= 2048) || a.Cg == 4) ? 8 : 4;
+    // Eight channels of half width to a vector where one statistic serves them all.  Two of them (groups of four) cost more registers than the wide
+    // accesses give: 2560 clouds of 82 x 128 bf16 in groups of four, forward / backward / second gradient 47 / 82 / 137 us in vectors of four, 49 / 95 / 187
+    // in vectors of eight; 7 clouds of 300 000 x 96 52 / 92 / 150 and 51 / 88 / 184; 400 clouds of 200 000 x 128 with dropout 76 / 132 / 183 and 68 / 117 / 175.
+    p.V = esize == 2 && aligned && a.Cg % 8 == 0 && a.Cg <= 2048 ? 8 : 4;
     const int m0 = p.V / gcd(a.Cg, p.V);   // groups whose channels fill whole vectors
     p.al = aligned && a.C % p.V == 0 && m0 * a.Cg <= 4096;
-    p.ns = p.al && a.Cg % p.V == 0 ? 1 : p.V == 8 ? 2 : 4;
+    p.ns = p.al && a.Cg % p.V == 0 ? 1 : 4;
     auto lanes = [&](int k) { return p.al || k >= a.G || k * a.Cg % 4 == 0 ? (k * a.Cg + p.V - 1) / p.V : (k * a.Cg + 6) / 4; };
     auto whole = [&](int k) { return k >= a.G ? a.G : p.al ? std::min(a.G, (k + m0 - 1) / m0 * m0) : k; };
     // Slab width: 64 bytes of a row at least (its neighbour reads the other half of the line into the same L2), doubled while a short

@@ -29,7 +29,7 @@ int with_family(const Plan& p, F f) {
 template <typename T, int NRS, int NRL, int NR8, typename F>
 int with_variant(const Plan& p, F f) {
     if constexpr (sizeof(T) == 2) {
-        if (p.V == 8) return p.ns == 1 ? with_family<T, NR8, NR8, 8, true, 1>(p, f) : with_family<T, NR8, NR8, 8, true, 2>(p, f);
+        if (p.V == 8) return with_family<T, NR8, NR8, 8, true, 1>(p, f);
     }
     if (!p.al) return with_family<T, NRS, NRL, 4, false, 4>(p, f);
     return p.ns == 1 ? with_family<T, NRS, NRL, 4, true, 1>(p, f) : with_family<T, NRS, NRL, 4, true, 4>(p, f);

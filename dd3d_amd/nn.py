@@ -112,7 +112,8 @@ class MinkowskiGroupNorm(nn.Module):
 
 class MinkowskiDropout(nn.Module):
     """Dropout on the feature rows while training (``ops.dropout``: the mask is computed from a seed and a call count, never stored); takes
-    and returns a SparseTensor or the rows of MinkowskiGlobalAvgPooling.  ``seed`` as in MinkowskiGroupNorm."""
+    and returns a SparseTensor or the rows of MinkowskiGlobalAvgPooling.  ``seed`` as in MinkowskiGroupNorm.  Every forward pass draws a key, also
+    one that recomputes another (activation checkpointing): draw the key outside and call ``ops.dropout`` there."""
 
     def __init__(self, p=0.5, seed=None):
         super().__init__()

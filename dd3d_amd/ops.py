@@ -665,7 +665,8 @@ def group_norm(x: torch.Tensor, seg_off: torch.Tensor, num_groups: int, weight: 
     Cloud ``b`` owns the rows ``seg_off[b]:seg_off[b + 1]`` (int32 [B + 1] on the device, ascending: ``CoordinateManager.seg_off``); mean and
     biased variance are taken over its rows and the ``C / num_groups`` channels of a group.  Rows in no cloud come out as zeros.
     ``weight`` / ``bias``: C values in fp32 or the rows' type; ``activation``: none, relu, leaky_relu (``negative_slope``), silu, gelu (exact).
-    ``dropout`` > 0 needs ``key`` and drops the elements that ``ops.dropout`` drops under that key.  Differentiable twice."""
+    ``dropout`` > 0 needs ``key`` and drops the elements that ``ops.dropout`` drops under that key.  Differentiable twice, in reverse mode
+    (a forward-mode tangent raises NotImplementedError)."""
     _rows_dtype(x, "x")
     if x.dim() != 2:
         raise ValueError(f"x has to be rows [M, C], got {tuple(x.shape)}")

@@ -13,6 +13,7 @@
 #define DD3D_ACT_LEAKY 2
 #define DD3D_ACT_SILU 3
 #define DD3D_ACT_GELU 4
+#define DD3D_ACT_LOW_MEANS 16   // with any of them: the group norm's means in two floats
 
 // ---- element types: every value is widened to fp32 on the way in and rounded to nearest even once on the way out ----------------
 typedef _Float16 half_t;

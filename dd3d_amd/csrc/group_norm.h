@@ -16,7 +16,9 @@
 //     (every workgroup for itself, in window order) and walks the rows again.  Which clouds are large is read from seg_off on the device.
 // Sums are fp32: per thread over its rows, then lanes, waves, windows in a fixed order.  Variances come from differences to a mean
 // at every level (thread, workgroup, windows), never from a mean of squares; and the mean of those differences is added to the mean they were
-// taken to, so that neither the sum's roundings nor a reciprocal's stay in it: a constant cloud is centred to zeros.
+// taken to, so that neither the sum's roundings nor a reciprocal's stay in it: a constant cloud is centred to zeros.  Of fp32 rows a mean is held in
+// two floats, as its rounding to one is a visible part of the spread of values that lie close together (3000 clouds, half of them of two or three rows,
+// a group a channel: dx is 4.6e-6 off with one float, 2.2e-7 with two).  Values of half width cannot lie that close.
 #pragma once
 #include "feature_math.h"
 
@@ -31,6 +33,7 @@ struct Norm {
     const int* seg;
     const void *W, *Bi;
     float eps, slope;
+    bool low;                  // behind the B * G means lie what their roundings left of them
     Drop drop;
 };
 
@@ -101,7 +104,7 @@ struct Cfg {
     typedef T_ T;
     static constexpr int V = V_, FAM = FAM_, THREADS = THREADS_, NR = NR_, NS = NS_, WAVES = THREADS_ / 64;
     static constexpr int PER = V_ / NS_;   // channels that share a statistic
-    static constexpr bool AL = AL_;
+    static constexpr bool AL = AL_, LOW = sizeof(T_) == 4;   // LOW: means in two floats
     static constexpr int FWD_WAVES = THREADS_ > 256 || NR_ <= 8 ? 4 : 3, BWD_WAVES = THREADS_ > 256 ? 4 : NR_ > 8 ? 2 : 3,
                          BWD2_WAVES = THREADS_ > 256 ? 4 : NS_ == 1 ? 3 : 2;
     static constexpr int at(int i) { return i / PER; }
@@ -188,6 +191,13 @@ __device__ __forceinline__ float rsqrt_newton(float v) {
 __device__ __forceinline__ float done(float v) {
     asm volatile("" : "+v"(v));
     return v;
+}
+
+// how far the means' second floats lie behind the first ones: multiplied where it is used, as two more scalars over a whole kernel push others out
+__device__ __forceinline__ int64_t means(const Norm& a) {
+    int b = a.B;
+    asm volatile("" : "+s"(b));
+    return (int64_t)b * a.G;
 }
 
 // ---- rows of a cloud ------------------------------------------------------------------------------------------------------------
@@ -614,6 +624,12 @@ __device__ __forceinline__ float about_mean(float q, float e, float shift) {
     return r < q * 0x1p-18f ? 0.f : r;
 }
 
+// (x - mean) / standard deviation from x less the mean's first float; low: the second one times -rstd
+template <typename Z>
+__device__ __forceinline__ float normal(float d, float rstd, float low) {
+    return Z::LOW ? fmaf(d, rstd, low) : d * rstd;
+}
+
 template <typename Z>
 struct Fwd {
     typedef typename Z::T T;
@@ -626,8 +642,8 @@ struct Fwd {
     float* lds;
     PhiloxKey key;
 
-    // per-thread count, mean and centred sum of squares, joined with those of one more chunk
-    __device__ __forceinline__ void add_rows(int all, const typename Z::Row (&z)[NR], float& cnt, float (&mu)[NS], float (&m2)[NS]) {
+    // per-thread count, mean (mu + low) and centred sum of squares, joined with those of one more chunk
+    __device__ __forceinline__ void add_rows(int all, const typename Z::Row (&z)[NR], const float (&k)[NS], float& cnt, float (&mu)[NS], float (&low)[NS], float (&m2)[NS]) {
         const int left = s.on ? all : 0;
         float n1 = 0.f, sx[NS], e[NS], q[NS];
 #pragma unroll
@@ -640,10 +656,11 @@ struct Fwd {
             for (int i = 0; i < V; ++i) sx[Z::at(i)] += raw_get(z[n], i);   // (zeros past the end)
         }
         if (n1 == 0.f) return;
-        // (reciprocals to a step: sx need only be near the chunk's mean; the first chunk's is taken as it is)
-        const float inv = __builtin_amdgcn_rcpf(n1), sum = cnt + n1, part = cnt > 0.f ? n1 * __builtin_amdgcn_rcpf(sum) : 1.f, cross = cnt * part;
+        // (reciprocals to a step: sx need only be near the chunk's mean, and is the reference where that is as near: equal values then leave nothing
+        // in the mean's second float)
+        const float inv = __builtin_amdgcn_rcpf(n1), sum = cnt + n1, part = n1 * __builtin_amdgcn_rcpf(sum), cross = cnt * part;
 #pragma unroll
-        for (int i = 0; i < NS; ++i) sx[i] *= inv;
+        for (int i = 0; i < NS; ++i) sx[i] = Z::LOW && fabsf(fmaf(sx[i], inv, -k[i])) <= fabsf(k[i]) * 0x1p-18f ? k[i] : sx[i] * inv;
 #pragma unroll
         for (int n = 0; n < NR; ++n)
             if (s.rl + n * g.RL < left) {
@@ -657,9 +674,11 @@ struct Fwd {
             }
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
-            const float shift = e[i] * inv, d = sx[i] + shift - mu[i];
-            mu[i] = fmaf(d, part, mu[i]);
+            const float shift = e[i] * inv, m = sx[i] + shift, l = Z::LOW ? (sx[i] - m) + shift : 0.f, d = Z::LOW ? (m - mu[i]) + (l - low[i]) : m - mu[i];
             m2[i] += fmaf(d * cross, d, about_mean(q[i], e[i], shift));
+            const float t = Z::LOW ? fmaf(d, part, low[i]) : d * part, next = mu[i] + t;
+            low[i] = Z::LOW ? cnt > 0.f ? (mu[i] - next) + t : l : 0.f;
+            mu[i] = cnt > 0.f ? next : m;   // (the first chunk's as it is)
         }
         cnt = sum;
     }
@@ -672,45 +691,46 @@ struct Fwd {
         for (int i = 0; i < NS; ++i) k[i] = widen(at[s.j[i] * a.Cg]);
     }
 
-    // the thread's part -> v[0] = mean, v[1] = centred sum of squares of its groups over `rows` rows
-    __device__ __forceinline__ void join(int rows, const float (&k)[NS], float cnt, const float (&mu)[NS], const float (&m2)[NS], float (&v)[2][NS]) {
+    // the thread's part -> v[0] + v[2] = mean, v[1] = centred sum of squares of its groups over `rows` rows
+    __device__ __forceinline__ void join(int rows, const float (&k)[NS], float cnt, const float (&mu)[NS], const float (&low)[NS], const float (&m2)[NS], float (&v)[3][NS]) {
         const float inv = 1.f / ((float)rows * (float)a.Cg);
         float sum[1][NS], eq[2][NS];
 #pragma unroll
-        for (int i = 0; i < NS; ++i) sum[0][i] = cnt * (mu[i] - k[i]);
+        for (int i = 0; i < NS; ++i) sum[0][i] = cnt * (Z::LOW ? (mu[i] - k[i]) + low[i] : mu[i] - k[i]);
         group_sums<1, Z>(sum, a, g, s, lds);
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
             v[0][i] = fmaf(sum[0][i], inv, k[i]);
-            const float d = mu[i] - v[0][i];
+            const float d = Z::LOW ? (mu[i] - v[0][i]) + low[i] : mu[i] - v[0][i];
             eq[0][i] = d * cnt;
             eq[1][i] = cnt > 0.f ? fmaf(eq[0][i], d, m2[i]) : 0.f;
         }
         group_sums<2, Z>(eq, a, g, s, lds);
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
-            const float shift = eq[0][i] * inv;
-            v[0][i] += shift;
+            const float shift = eq[0][i] * inv, m = v[0][i] + shift;
             v[1][i] = about_mean(eq[1][i], eq[0][i], shift);
+            v[2][i] = Z::LOW ? (v[0][i] - m) + shift : 0.f;
+            v[0][i] = m;
         }
     }
 
     // statistics of rows that take several chunks
-    __device__ __forceinline__ void stats(const Range& r, float (&v)[2][NS]) {
-        float cnt = 0.f, k[NS], mu[NS], m2[NS];
+    __device__ __forceinline__ void stats(const Range& r, float (&v)[3][NS]) {
+        float cnt = 0.f, k[NS], mu[NS], low[NS], m2[NS];
         reference(r.r0, k);
 #pragma unroll
-        for (int i = 0; i < NS; ++i) mu[i] = m2[i] = 0.f;
+        for (int i = 0; i < NS; ++i) mu[i] = low[i] = m2[i] = 0.f;
         for (int base = r.r0; base < r.r1; base += NR * g.RL) {
             typename Z::Row z[NR];
             Chunk<Z>(X + row_at(a, base), a.C, r.r1 - base, g).load_all(g, s, z);
-            add_rows(r.r1 - base, z, cnt, mu, m2);
+            add_rows(r.r1 - base, z, k, cnt, mu, low, m2);
         }
-        join(r.r1 - r.r0, k, cnt, mu, m2, v);
+        join(r.r1 - r.r0, k, cnt, mu, low, m2, v);
     }
 
     // 1 / standard deviation from v of a whole cloud of `rows` rows; `keep`: this workgroup writes the statistics
-    __device__ __forceinline__ void finish(const float (&v)[2][NS], int b, int rows, bool keep, float* mean_out, float* rstd_out, float (&rstd)[NS]) {
+    __device__ __forceinline__ void finish(const float (&v)[3][NS], int b, int rows, bool keep, float* mean_out, float* rstd_out, float (&rstd)[NS]) {
         const float inv = 1.f / ((float)rows * (float)a.Cg);
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
@@ -718,16 +738,17 @@ struct Fwd {
             if (mean_out && keep && writes_group(a, s, i)) {
                 const int64_t at = (int64_t)b * a.G + s.slab * g.k + s.j[i];
                 mean_out[at] = v[0][i], rstd_out[at] = rstd[i];
+                if (Z::LOW && a.low) mean_out[at + means(a)] = v[2][i];
             }
         }
     }
 
     // y of rows that take several chunks
-    __device__ __forceinline__ void apply(const Range& r, const float (&mean)[NS], const float (&rstd)[NS]) {
+    __device__ __forceinline__ void apply(const Range& r, const float (&v)[3][NS], const float (&rstd)[NS]) {
         for (int base = r.r0; base < r.r1; base += NR * g.RL) {
             typename Z::Row z[NR];
             Chunk<Z>(X + row_at(a, base), a.C, r.r1 - base, g).load_all(g, s, z);
-            rows_out(base, r.r1 - base, mean, rstd, z);
+            rows_out(base, r.r1 - base, v, rstd, z);
         }
     }
 
@@ -736,23 +757,25 @@ struct Fwd {
         const int rows = r.r1 - r.r0;
         typename Z::Row z[NR];
         Chunk<Z>(X + row_at(a, r.r0), a.C, rows, g).load_all(g, s, z);
-        float cnt = 0.f, k[NS], mu[NS], m2[NS], v[2][NS], rstd[NS];
+        float cnt = 0.f, k[NS], mu[NS], low[NS], m2[NS], v[3][NS], rstd[NS];
         reference(r.r0, k);
 #pragma unroll
-        for (int i = 0; i < NS; ++i) mu[i] = m2[i] = 0.f;
-        add_rows(rows, z, cnt, mu, m2);
-        join(rows, k, cnt, mu, m2, v);
+        for (int i = 0; i < NS; ++i) mu[i] = low[i] = m2[i] = 0.f;
+        add_rows(rows, z, k, cnt, mu, low, m2);
+        join(rows, k, cnt, mu, low, m2, v);
         finish(v, b, rows, true, mean_out, rstd_out, rstd);
-        rows_out(r.r0, rows, v[0], rstd, z);
+        rows_out(r.r0, rows, v, rstd, z);
     }
 
-    __device__ __forceinline__ void rows_out(int base, int all, const float (&mean)[NS], const float (&rstd)[NS], const typename Z::Row (&z)[NR]) {
+    __device__ __forceinline__ void rows_out(int base, int all, const float (&v)[3][NS], const float (&rstd)[NS], const typename Z::Row (&z)[NR]) {
         const Chunk<Z> to(Y + row_at(a, base), a.C, all, g);
         const uint64_t words = words_at(g, base);
         const uint32_t off = here(s.off), word = here(s.word);
-        float scale[V];
+        float scale[V], low[NS];   // (of half-width rows one factor a channel: an operation less)
 #pragma unroll
         for (int i = 0; i < V; ++i) scale[i] = rstd[Z::at(i)] * s.w[i];
+#pragma unroll
+        for (int i = 0; i < NS; ++i) low[i] = -v[2][i] * rstd[i];
 #pragma unroll
         for (int n = 0; n < NR; ++n) {
             row_border();
@@ -760,8 +783,11 @@ struct Fwd {
             float y[V], d1, d2;
             const typename Z::Row x = again(z[n]);
 #pragma unroll
-            for (int i = 0; i < V; ++i)
-                y[i] = activate<Z::FAM, 0, sizeof(T) == 2>(fmaf(raw_get(x, i) - mean[Z::at(i)], scale[i], s.b[i]), a.slope, &d1, &d2);
+            for (int i = 0; i < V; ++i) {
+                const float d = raw_get(x, i) - v[0][Z::at(i)];
+                const float u = Z::LOW ? fmaf(normal<Z>(d, rstd[Z::at(i)], low[Z::at(i)]), s.w[i], s.b[i]) : fmaf(d, scale[i], s.b[i]);
+                y[i] = activate<Z::FAM, 0, sizeof(T) == 2>(u, a.slope, &d1, &d2);
+            }
             if (a.drop.key) {
                 Words<V>(key, words + (word + n * (uint32_t)(g.RL * g.quads))).drop(a.drop, y);
             }
@@ -770,7 +796,7 @@ struct Fwd {
     }
 };
 
-// part [2 * NW][G][2]: mean and centred sum of squares of a window's piece of a large cloud.  MODE 0: the clouds, and the windows' partial
+// part [2 * NW][G][3]: mean, centred sum of squares and low part of the mean of a window's piece of a large cloud.  MODE 0: the clouds, and the windows' partial
 // sums; MODE 1: the windows' rows
 template <typename Z, int MODE>
 __global__ __launch_bounds__(Z::THREADS, Z::FWD_WAVES) void k_fwd(Norm a, Geo g, const typename Z::T* X, typename Z::T* Y, float* mean_out, float* rstd_out,
@@ -786,7 +812,7 @@ __global__ __launch_bounds__(Z::THREADS, Z::FWD_WAVES) void k_fwd(Norm a, Geo g,
     Spot<Z> s;
     locate(a, g, unit, slab, s);
     Fwd<Z> f{a, g, s, X, Y, lds, drop_key(a.drop)};
-    float v[2][Z::NS], rstd[Z::NS];
+    float v[3][Z::NS], rstd[Z::NS];
     for (int i = 0, b = s.unit;; ++i, b += g.U) {
         if (MODE == 0) {
             Range r;
@@ -799,6 +825,7 @@ __global__ __launch_bounds__(Z::THREADS, Z::FWD_WAVES) void k_fwd(Norm a, Geo g,
                         for (int j = threadIdx.x; j < s.gs; j += Z::THREADS) {
                             const int64_t at = (int64_t)b * a.G + s.slab * g.k + j;
                             mean_out[at] = rstd_out[at] = 0.f;
+                            if (Z::LOW && a.low) mean_out[at + means(a)] = 0.f;
                         }
                     continue;
                 }
@@ -813,9 +840,9 @@ __global__ __launch_bounds__(Z::THREADS, Z::FWD_WAVES) void k_fwd(Norm a, Geo g,
             f.stats(r, v);
             if (whole) {
                 f.finish(v, b, r.r1 - r.r0, true, mean_out, rstd_out, rstd);
-                f.apply(r, v[0], rstd);
+                f.apply(r, v, rstd);
             } else {
-                put_part<2, Z>(part, i ? p[1].slot : p[0].slot, v, a, g, s);
+                put_part<3, Z>(part, i ? p[1].slot : p[0].slot, v, a, g, s);
             }
             continue;
         }
@@ -826,26 +853,30 @@ __global__ __launch_bounds__(Z::THREADS, Z::FWD_WAVES) void k_fwd(Norm a, Geo g,
         float* out = lds + g.red + g.kb * g.CL * Z::NS;
         __syncthreads();
         for (int j = s.wave; j < s.gs; j += Z::WAVES) {
-            const float* from = part + (s.slab * g.k + j) * 2;
-            const float inv = 1.f / (float)rows;
+            const float* from = part + (s.slab * g.k + j) * 3;
+            const auto piece = [&](int o) { return from + (int64_t)piece_slot(g, q.all, o) * a.G * 3; };
+            const float inv = 1.f / (float)rows, k = piece(0)[0];
             float m = 0.f, e = 0.f, m2 = 0.f;
-            for (int o = s.lane; o < n; o += 64) m = fmaf(from[(int64_t)piece_slot(g, q.all, o) * a.G * 2], (float)piece_rows(g, q.all, o) * inv, m);
-            m = wave_sum(m);
-            for (int o = s.lane; o < n; o += 64) e = fmaf(from[(int64_t)piece_slot(g, q.all, o) * a.G * 2] - m, (float)piece_rows(g, q.all, o) * inv, e);
-            m += wave_sum(e);
+            for (int o = s.lane; o < n; o += 64) m = fmaf(piece(o)[0] - k, (float)piece_rows(g, q.all, o) * inv, m);
+            m = k + wave_sum(m);
+            for (int o = s.lane; o < n; o += 64) e = fmaf((piece(o)[0] - m) + piece(o)[2], (float)piece_rows(g, q.all, o) * inv, e);
+            e = wave_sum(e);
+            const float mean = m + e, low = Z::LOW ? (m - mean) + e : 0.f;
             for (int o = s.lane; o < n; o += 64) {
-                const float* z = from + (int64_t)piece_slot(g, q.all, o) * a.G * 2;
-                const float d = z[0] - m;
+                const float* z = piece(o);
+                const float d = (z[0] - mean) + (z[2] - low);
                 m2 += fmaf(d * d, (float)piece_rows(g, q.all, o) * (float)a.Cg, z[1]);
             }
             m2 = wave_sum(m2);
-            if (s.lane == 0) out[j] = m, out[g.k + j] = m2;
+            if (s.lane == 0) out[j] = mean, out[g.k + j] = m2, out[2 * g.k + j] = low;
         }
         __syncthreads();
 #pragma unroll
-        for (int h = 0; h < Z::NS; ++h) v[0][h] = out[s.j[h]], v[1][h] = out[g.k + s.j[h]];
+        for (int h = 0; h < Z::NS; ++h)
+#pragma unroll
+            for (int c = 0; c < 3; ++c) v[c][h] = out[c * g.k + s.j[h]];
         f.finish(v, q.b, rows, q.all.r0 == q.part.r0, mean_out, rstd_out, rstd);
-        f.apply(q.part, v[0], rstd);
+        f.apply(q.part, v, rstd);
     }
 }
 
@@ -857,6 +888,17 @@ __device__ __forceinline__ void row_rstd(const float (&rstd)[NS], bool there, fl
     for (int i = 0; i < NS; ++i) rs[i] = there ? rstd[i] : 0.f;
 }
 
+// the statistics of cloud b
+template <typename Z>
+__device__ __forceinline__ void read_stats(const Norm& a, const Geo& g, const Spot<Z>& s, int b, const float* mean_in, const float* rstd_in, float (&mean)[Z::NS],
+                                           float (&rstd)[Z::NS], float (&low)[Z::NS]) {
+    const int64_t at = (int64_t)b * a.G + s.slab * g.k;
+#pragma unroll
+    for (int i = 0; i < Z::NS; ++i) {
+        mean[i] = mean_in[at + s.j[i]], rstd[i] = rstd_in[at + s.j[i]];
+        low[i] = Z::LOW && a.low ? -mean_in[at + s.j[i] + means(a)] * rstd[i] : 0.f;
+    }
+}
 // ---- first gradient -------------------------------------------------------------------------------------------------------------
 // Bound by HBM and, at two to three waves per SIMD, by the latency of its loads; with dropout (400 000 x 128 fp32, GELU: 182 us, 3.4 TB/s) by having
 // two waves only, whose vector instructions take 56% of the cycles; half-width rows by vector instructions (80 to 90%).  What a thread keeps of a
@@ -874,7 +916,7 @@ struct Bwd {
     T* dX;
     float* lds;
     PhiloxKey key;
-    float mean[NS], rstd[NS], par[2][V];   // parameter gradients of this thread's channels: dw, db
+    float mean[NS], rstd[NS], low[NS], par[2][V];   // low: what is left of the mean, times -rstd; parameter gradients of this thread's channels: dw, db
 
     struct Held {
         typename Z::Row x[NR], d[NR];
@@ -883,9 +925,7 @@ struct Bwd {
     };
 
     __device__ __forceinline__ void load_stats(int b, const float* mean_in, const float* rstd_in) {
-        const int64_t at = (int64_t)b * a.G + s.slab * g.k;
-#pragma unroll
-        for (int i = 0; i < NS; ++i) mean[i] = mean_in[at + s.j[i]], rstd[i] = rstd_in[at + s.j[i]];
+        read_stats<Z>(a, g, s, b, mean_in, rstd_in, mean, rstd, low);
     }
 
     __device__ __forceinline__ void load(int base, int all, Held& h) {
@@ -901,7 +941,7 @@ struct Bwd {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             float d1, d2;
-            xh[i] = (raw_get(x, i) - mean[Z::at(i)]) * rs[Z::at(i)];
+            xh[i] = normal<Z>(raw_get(x, i) - mean[Z::at(i)], rs[Z::at(i)], low[Z::at(i)]);
             activate<Z::FAM, 1>(fmaf(xh[i], s.w[i], s.b[i]), a.slope, &d1, &d2);
             gr[i] *= d1;
         }
@@ -1080,7 +1120,7 @@ struct Bwd2 {
     PhiloxKey key;
     typename Z::Row* mine;                 // this thread's rows in LDS: [NR][x, dy, P], a workgroup's width apart; NULL: none
     float q[V], t[V];                      // cotangents of dw and db
-    float mean[NS], rstd[NS], par[2][V];   // d(w), d(b)
+    float mean[NS], rstd[NS], low[NS], par[2][V];   // low: what is left of the mean, times -rstd; d(w), d(b)
 
     struct Held {
         typename Z::Row x[NR], d[NR], p[NR];
@@ -1098,9 +1138,7 @@ struct Bwd2 {
     static constexpr bool HOLD = V == 4 && NS == 1 && Z::THREADS == 256;
 
     __device__ __forceinline__ void load_stats(int b, const float* mean_in, const float* rstd_in) {
-        const int64_t at = (int64_t)b * a.G + s.slab * g.k;
-#pragma unroll
-        for (int i = 0; i < NS; ++i) mean[i] = mean_in[at + s.j[i]], rstd[i] = rstd_in[at + s.j[i]];
+        read_stats<Z>(a, g, s, b, mean_in, rstd_in, mean, rstd, low);
     }
 
     __device__ __forceinline__ void load(int base, int all, Held& h, bool from_lds) {
@@ -1142,7 +1180,7 @@ struct Bwd2 {
     };
     __device__ __forceinline__ Elem element(const RowOf& r, int i) {
         Elem e;
-        e.xh = (r.x[i] - mean[Z::at(i)]) * r.rs[Z::at(i)];
+        e.xh = normal<Z>(r.x[i] - mean[Z::at(i)], r.rs[Z::at(i)], low[Z::at(i)]);
         e.p = r.p[i], e.dy = r.dy[i];
         activate<Z::FAM, 2>(fmaf(e.xh, s.w[i], s.b[i]), a.slope, &e.d1, &e.d2);
         return e;

@@ -110,7 +110,7 @@ inline gn::Plan plan(const gn::Norm& a, int act, int esize, bool aligned, int su
     g.kb = std::max(1, std::min(sums, 8192 / (g.RL * cols)));
     g.red = g.fast ? 2 * sums * (threads / 64) * g.k : g.kb * g.RL * cols;
     if (params) g.red = std::max(g.red, (g.lcl >= 0 ? threads / 64 : g.RL) * g.CL * p.V);
-    p.lds = sizeof(float) * std::max<size_t>((size_t)g.red + g.kb * cols + sums * g.k, params ? threads : 0);
+    p.lds = sizeof(float) * std::max<size_t>((size_t)g.red + g.kb * cols + std::max(sums, 3) * g.k, params ? threads : 0);
     return p;
 }
 
@@ -128,7 +128,7 @@ inline Layout layout(int64_t M, int C, int B, int G, int order) {
         at = align_up64(at + words * 4, 256);
         return here;
     };
-    l.part = take(2 * windows * G * (order == 2 ? 14 : 2));
+    l.part = take(2 * windows * G * (order == 2 ? 14 : order == 1 ? 2 : 3));
     l.slots = take(units * 2 * C);
     l.found = take(windows);
     l.bytes = at;
@@ -148,11 +148,13 @@ inline bool aligned16(std::initializer_list<const void*> ps) {
     return (m & 15) == 0;
 }
 
-// argument checks shared by the three entry points; 0 = fill in `a` and go on
-inline int check(int dtype, int64_t M, int C, const int32_t* seg, int B, int G, const void* W, const void* Bi, int pdt, int act, float slope, double p,
+// argument checks shared by the three entry points; 0 = fill in `a`, take the statistics' flag off `act` and go on
+inline int check(int dtype, int64_t M, int C, const int32_t* seg, int B, int G, const void* W, const void* Bi, int pdt, int& act, float slope, double p,
                  const int64_t* key, gn::Norm* a) {
     if (M < 0 || B < 0 || C <= 0 || G <= 0 || C % G != 0) return DD3D_EARG;
     if (M > gn::MOST || C > 4096 || (int64_t)B * G > gn::MOST) return DD3D_ESIZE;
+    a->low = act >= 0 && (act & DD3D_ACT_LOW_MEANS);
+    if (a->low) act &= ~DD3D_ACT_LOW_MEANS;
     if (dtype < DD3D_F32 || dtype > DD3D_BF16 || (pdt != DD3D_F32 && pdt != dtype) || act < DD3D_ACT_NONE || act > DD3D_ACT_GELU) return DD3D_EARG;
     if (slope != slope || (B > 0 && !seg) || !make_drop(p, key, &a->drop)) return DD3D_EARG;
     a->M = (int)M, a->C = C, a->B = B, a->G = G, a->Cg = C / G, a->pdt = pdt, a->seg = seg, a->W = W, a->Bi = Bi;

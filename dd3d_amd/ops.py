@@ -440,6 +440,7 @@ class NormActPoolFn(Function):
 # mode, and they take fp32, fp16 and bf16 rows (arithmetic in fp32, one rounding at the end).
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "leaky_relu": 2, "silu": 3, "gelu": 4}
+_LOW_MEANS = 16   # with an activation's number: the statistics hold the means in two floats
 _MAX_NORM_CHANNELS = 4096
 _MAX_NORM_ROWS = 2 ** 31 - 65536   # the kernels count rows and clouds in 32 bits and step past the end
 
@@ -587,16 +588,16 @@ def _norm_fwd(x, w, b, seg_off, key, meta, eps, keep):
     x, w, b = _dense(x), _dense(w), _dense(b)
     dev = x.device
     y = torch.empty_like(x)
-    stats = torch.empty((2, seg_off.numel() - 1, meta.G), dtype=_F32, device=dev) if keep else None   # mean and 1 / standard deviation
+    stats = torch.empty((3, seg_off.numel() - 1, meta.G), dtype=_F32, device=dev) if keep else None   # mean in two floats and 1 / standard deviation
     ws, n = meta.workspace(x, seg_off, 0)
-    _launch(dev, "dd3d_group_norm_fwd", x.data_ptr(), *meta.shape(x, seg_off, w, b), eps, meta.act, meta.slope, meta.p, _addr(key), y.data_ptr(), *_stats(stats),
+    _launch(dev, "dd3d_group_norm_fwd", x.data_ptr(), *meta.shape(x, seg_off, w, b), eps, meta.act + (_LOW_MEANS if keep else 0), meta.slope, meta.p, _addr(key), y.data_ptr(), *_stats(stats),
             _addr(ws), n, L.raw_stream(dev))
     return y, stats
 
 
 def _stats(stats):
     at = stats.data_ptr() if stats is not None else 0
-    return (at, at + 2 * stats.numel()) if at else (None, None)   # the second half of 4-byte values
+    return (at, at + stats.numel() // 3 * 8) if at else (None, None)   # the last third of 4-byte values
 
 
 def _norm_grad(dy, x, w, b, seg_off, key, stats, meta, need):
@@ -607,7 +608,7 @@ def _norm_grad(dy, x, w, b, seg_off, key, stats, meta, need):
     dw = torch.empty_like(w) if need[1] else None
     db = torch.empty_like(b) if need[2] else None
     ws, n = meta.workspace(x, seg_off, 1)
-    _launch(dev, "dd3d_group_norm_bwd", dy.data_ptr(), x.data_ptr(), *meta.shape(x, seg_off, w, b), meta.act, meta.slope, meta.p, _addr(key), *_stats(stats),
+    _launch(dev, "dd3d_group_norm_bwd", dy.data_ptr(), x.data_ptr(), *meta.shape(x, seg_off, w, b), meta.act + _LOW_MEANS, meta.slope, meta.p, _addr(key), *_stats(stats),
             _addr(dx), _addr(dw), _addr(db), _addr(ws), n, L.raw_stream(dev))
     return dx, dw, db
 
@@ -652,7 +653,7 @@ class _GroupNormGradFn(Function):
         ddw = torch.empty_like(w) if need[2] else None
         ddb = torch.empty_like(b) if need[3] else None
         ws, n = meta.workspace(x, seg_off, 2)
-        _launch(dev, "dd3d_group_norm_bwd2", _addr(ggx), _addr(ggw), _addr(ggb), dy.data_ptr(), x.data_ptr(), *meta.shape(x, seg_off, w, b), meta.act,
+        _launch(dev, "dd3d_group_norm_bwd2", _addr(ggx), _addr(ggw), _addr(ggb), dy.data_ptr(), x.data_ptr(), *meta.shape(x, seg_off, w, b), meta.act + _LOW_MEANS,
                 meta.slope, meta.p, _addr(key), *_stats(stats), _addr(ddy), _addr(ddx), _addr(ddw), _addr(ddb), _addr(ws), n, L.raw_stream(dev))
         return ddy, ddx, ddw, ddb, None, None, None, None, None
 

@@ -268,7 +268,9 @@ int dd3d_global_avg_pool_bwd(const float* g, int64_t M, const int32_t* seg_off, 
  * (slope below zero), 3 SiLU, 4 GELU (the normal distribution's).  p, key: as in dd3d_dropout (key nullable with p = 0).
  * Rows of [0, M) that belong to no cloud come out as zeros; rows from M on are not touched.  C <= 4096, M and B*G <= 2^31 - 65536,
  * eps >= 2^-126.
- *   fwd : Y = dropout(act(xhat*weight + bias)); mean / rstd [B,G] fp32 are kept for the gradients (nullable pair; zeros for an empty cloud)
+ *   fwd : Y = dropout(act(xhat*weight + bias)); mean / rstd [B,G] fp32 are kept for the gradients (nullable pair; zeros for an empty cloud).
+ *         act + 16, in all three calls: mean is [2,B,G], the means and behind them what the rounding to fp32 left of them (for half-width rows
+ *         neither written nor read).  Without it the gradients of fp32 rows see differences to the rounded mean.
  *   bwd : dX (nullable), dweight / dbias [C] in pdtype (each nullable) from dY
  *   bwd2: the gradient of bwd: from the cotangents ggX[M,C], ggW[C], ggB[C] of its three results (each nullable) the cotangents of its
  *         inputs dY, X, weight, bias (each result nullable)

@@ -140,6 +140,43 @@ def test_a_spike_in_a_clouds_first_element_costs_no_accuracy():
         assert bool(((y[r0:r1].reshape(r1 - r0, 4, 4) - want).abs() <= allow).all())
 
 
+@pytest.mark.parametrize("C,G", [(43, 43), (16, 16), (8, 2), (64, 64), (16, 4)])
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+def test_values_that_lie_close_together(C, G, act):
+    """Clouds of a few rows a thousandth apart: half a step of the mean is a visible part of their spread, and is not in the results.  Held against
+    the count of roundings without the conditioning (largest value over spread) that the other tests grant."""
+    lens = [2, 3, 2, 1, 4, 2, 40, 2, 700] * 6
+    seg, t = batch(lens, C, F32, seed=41)
+    base = t["x"][torch.tensor(seg[:-1])].repeat_interleave(torch.tensor(lens), 0)
+    t["x"] = base + 1e-3 * torch.randn(base.shape, generator=torch.Generator().manual_seed(42))
+    got = through_autograd(t, seg_on_device(seg), G, 2, activation=act)
+    ref = R.group_norm(t["x"], seg, G, t["w"], t["b"], 1e-5, act, dy=t["dy"], ggx=t["ggx"], ggw=t["ggw"], ggb=t["ggb"], order=2)
+    for n, v in got.items():
+        far = R.off(n, v, ref, F32, torch.ones(()))
+        assert far <= 1, f"{n}: {far:.3g} times what its roundings allow"
+
+
+@pytest.mark.parametrize("C,G", [(16, 4), (7, 7), (24, 2), (128, 8)])
+def test_the_mean_in_two_floats(C, G):
+    """Sums of differences below 2^4: at most 64 in a thread, 128 over threads and 64 for chunks, windows and reciprocals, a half step each."""
+    from dd3d_amd import _lib as L
+    for dtype in (F32, BF16):
+        lens = [32, 45, 0, 1, 700, 9000, 20011]
+        seg, t = batch(lens, C, dtype, seed=43)
+        x, so, B, M = (t["x"].float().clamp(-7, 7) + 1e6).to(dtype).to(dev()), seg_on_device(seg), len(lens), seg[-1]
+        y, mean, rstd = torch.empty_like(x), torch.full((2, B, G), 7.0, device=dev()), torch.empty(B, G, device=dev())
+        ws = torch.empty(max(1, L.lib.dd3d_group_norm_ws_bytes(M, C, B, G, 0)), dtype=torch.uint8, device=dev())
+        L.call("dd3d_group_norm_fwd", L.ptr(x), 0 if dtype == F32 else 2, M, C, L.ptr(so), B, G, None, None, 0, 1e-5, 16, 0.0, 0.0, None, L.ptr(y), L.ptr(mean),
+               L.ptr(rstd), L.ptr(ws), ws.numel(), L.stream())
+        if dtype != F32:
+            assert bool((mean[1] == 7.0).all())      # half-width rows leave the second floats alone
+            continue
+        assert float(mean[1].abs().max()) <= 2.0 ** -5      # half a step at 2^19
+        for b, (r0, r1) in enumerate(zip(seg[:-1], seg[1:])):
+            want = x[r0:r1].double().reshape(r1 - r0, G, -1).mean((0, 2)) if r1 > r0 else torch.zeros(G, dtype=torch.float64, device=dev())
+            assert float((mean[:, b].double().sum(0) - want).abs().max()) <= 256 * 2.0 ** -24 * 2.0 ** 4
+
+
 @pytest.mark.parametrize("act", ["none", "silu", "gelu"])
 @pytest.mark.parametrize("value,eps", [(2.0 ** 57, 1e-5), (2.0 ** 20, 1e-30), (2.0 ** 70, 1e-36)])
 @pytest.mark.parametrize("C,G,dtype", [(16, 4, F32), (9, 3, F32), (32, 2, BF16)])

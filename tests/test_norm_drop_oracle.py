@@ -196,3 +196,13 @@ def test_a_fraction_of_groups_is_refused_by_name():
     from dd3d_amd import ops
     with pytest.raises(ValueError, match="do not divide into 2.5 groups"):
         ops.group_norm(torch.zeros(6, 5), torch.tensor([0, 6], dtype=torch.int32), 2.5)
+
+
+def test_the_flag_of_the_two_float_means_takes_no_other_number():
+    from dd3d_amd import _lib as L
+    def fwd(act):
+        return L.lib.dd3d_group_norm_fwd(256, 0, 1000, 8, 256, 1, 2, None, None, 0, 1e-5, act, 0.0, 0.0, None, 256, None, None, None, 0, None)
+    for act in (5, 16 + 5, 15, 32, 48, -1, -16, -12):
+        assert fwd(act) == -1, act
+    for act in (0, 4, 16, 16 + 4):
+        assert fwd(act) == -3, act      # as far as the workspace, which is missing

@@ -1,10 +1,10 @@
 // Device code of the group norm (formulas: group_norm.hip), shared by its three passes and instantiated per row type and pass in group_norm_*.hip.
 //
 // The passes need sums over (cloud, group) before anything can be written, so a row has to be read twice unless it stays on chip in between.
-// Large batches of fp32 rows are bound by HBM: 210 000 x 128 in 2560 clouds, SiLU, forward 49 us (4.4 TB/s), backward 82 (3.9); second
-// gradient of 300 000 x 128 in 400 clouds, GELU, 221 (3.5, and 4.8 with what it reads twice).  Half-width rows are bound by vector instructions,
-// which fill 99% of the SIMDs' cycles in the forward pass of 210 000 x 128 bf16 with GELU (46 us), as is the forward pass with GELU and dropout (400 000
-// x 128 fp32: 117 us, 80%; 22 of a row's 187 instructions read spilled scalars back).  Layout of the work:
+// Large batches of fp32 rows are bound by HBM: 210 000 x 128 in 2560 clouds, SiLU, forward 50 us (4.3 TB/s), backward 84 (3.8); second
+// gradient of 300 000 x 128 in 400 clouds, GELU, 222 (3.5, and 4.8 with what it reads twice).  Half-width rows are bound by vector instructions,
+// which fill 99% of the SIMDs' cycles in the forward pass of 210 000 x 128 bf16 with GELU (45 us), as is the forward pass with GELU and dropout (400 000
+// x 128 fp32: 119 us, 83%; 28 of a row's 198 instructions read spilled scalars back).  Layout of the work:
 //   * a SLAB is a run of whole groups, 64 bytes of a row at least; a workgroup owns one slab of one cloud after another.  Thread t holds V
 //     channels (one 16-byte vector) of the rows rl, rl + RL, ...: the rows of a chunk of NR * RL are loaded at once into registers, so up to
 //     that many loads are in flight per thread, and stay there while the workgroup forms the sums -- HBM sees every row once.  Four waves
@@ -900,8 +900,8 @@ __device__ __forceinline__ void read_stats(const Norm& a, const Geo& g, const Sp
     }
 }
 // ---- first gradient -------------------------------------------------------------------------------------------------------------
-// Bound by HBM and, at two to three waves per SIMD, by the latency of its loads; with dropout (400 000 x 128 fp32, GELU: 182 us, 3.4 TB/s) by having
-// two waves only, whose vector instructions take 56% of the cycles; half-width rows by vector instructions (80 to 90%).  What a thread keeps of a
+// Bound by HBM and, at two to three waves per SIMD, by the latency of its loads; with dropout (400 000 x 128 fp32, GELU: 184 us, 3.3 TB/s) by having
+// two waves only, whose vector instructions take 55% of the cycles; half-width rows by vector instructions (80 to 90%).  What a thread keeps of a
 // row between the sums and the result: the normalised values and g (fp32 rows: in the registers the loaded rows had), or the rows as loaded and the
 // bits dropout kept (half-width rows: half the registers, the derivative is computed again).
 template <typename Z>
@@ -1104,8 +1104,8 @@ __global__ __launch_bounds__(Z::THREADS, Z::BWD_WAVES) void k_bwd(Norm a, Geo g,
 }
 
 // ---- second gradient ------------------------------------------------------------------------------------------------------------
-// Three matrices in, two out, and 14 sums an element: fp32 rows by HBM where they are read twice (vector instructions take 76% of the cycles, with
-// dropout 93%), half-width rows by vector instructions (98%).  The three matrices stay as loaded; the activation's derivatives are computed
+// Three matrices in, two out, and 14 sums an element: fp32 rows by HBM where they are read twice (vector instructions take 75% of the cycles, with
+// dropout 92%), half-width rows by vector instructions (all of them).  The three matrices stay as loaded; the activation's derivatives are computed
 // again in every pass over them.
 template <typename Z>
 struct Bwd2 {
@@ -1133,7 +1133,7 @@ struct Bwd2 {
     static constexpr int KS = Z::FAM == DD3D_FAM_LINEAR ? 7 : 14;
     // A cloud's rows are needed twice, and what lies between has more of them in flight than the L2 holds (400 clouds of 750 rows of 128 fp32
     // channels: 972 MiB read instead of 439).  So LDS keeps the first chunk of a cloud and the registers its last: 242 us without, 227 with
-    // the LDS alone, 221 and 706 MiB with both.  The other variants' registers are full already (vectors of eight, and sixteen waves
+    // the LDS alone, 222 and 701 MiB with both.  The other variants' registers are full already (vectors of eight, and sixteen waves
     // a workgroup, spill some with SiLU and GELU; one statistic a channel takes up to 241 at two waves a SIMD) and walk all rows twice.
     static constexpr bool HOLD = V == 4 && NS == 1 && Z::THREADS == 256;
 

@@ -59,7 +59,8 @@ inline gn::Plan plan(const gn::Norm& a, int act, int esize, bool aligned, int su
     p.fam = act_family(act);
     // Eight channels of half width to a vector where one statistic serves them all.  Two of them (groups of four) cost more registers than the wide
     // accesses give: 2560 clouds of 82 x 128 bf16 in groups of four, forward / backward / second gradient 47 / 82 / 137 us in vectors of four, 49 / 95 / 187
-    // in vectors of eight; 7 clouds of 300 000 x 96 52 / 92 / 150 and 51 / 88 / 184; 400 clouds of 200 000 x 128 with dropout 76 / 132 / 183 and 68 / 117 / 175.
+    // in vectors of eight; 7 clouds of 300 000 x 96 in all 52 / 92 / 150 and 51 / 88 / 184; 400 clouds of 200 000 x 128 fp16 in all with dropout 76 / 132 / 183
+    // and 68 / 117 / 175.
     p.V = esize == 2 && aligned && a.Cg % 8 == 0 && a.Cg <= 2048 ? 8 : 4;
     const int m0 = p.V / gcd(a.Cg, p.V);   // groups whose channels fill whole vectors
     p.al = aligned && a.C % p.V == 0 && m0 * a.Cg <= 4096;
